@@ -467,6 +467,130 @@ void* ppn_stream(ppn_engine* e);
  * one "launch" is the whole step: schedule pre-pass + launch order + small-storage launch + large-storage launch, one bracket. */
 int ppn_kernel_time(ppn_engine* e, int32_t reset, double* total_ms, int64_t* launches);
 
+/* ---- operators of learned policies ------------------------------------------------------------------------
+ * What a policy that acts on the batch, or learns from its rollouts, needs next to the step engine: memory over
+ * the rows an environment has shown (a short causal convolution, a selective state space scan), and the cross
+ * entropy over a catalogue of switching actions.  These calls need no engine: DEVICE pointers in, kernels queued
+ * on `stream` (a hipStream_t; NULL = the null stream) of the current device, nothing synchronised, nothing
+ * allocated; the caller passes workspaces of the size the *_workspace function names, 16-byte aligned, private
+ * to the call until the stream has passed it.  0 or a negative PPN_E_* code; ppn_policy_error() has the text of
+ * this thread's last refusal.  Safe from several threads at once.  Every struct is 64-bit fields only and begins
+ * with struct_bytes = sizeof(it).  Strides count elements; the channel / state stride is always 1.  Sums, states,
+ * statistics and parameters are 32-bit floats; `type` is the type of the activations. */
+enum { PPN_T_F32 = 0, PPN_T_BF16 = 1, PPN_T_F16 = 2 };
+const char* ppn_policy_error(void);
+
+/* Short causal convolution over the rows of `batch` environments:
+ *   y[b,t,d] = act(bias[d] + sum_k weight[d,k] x[b, t - taps + 1 + k, d]),   rows in front of t = 0: initial (or 0).
+ * starts[b,t] != 0 marks the first row of an episode: taps in front of it are zero.  final_state: the last taps - 1
+ * rows of the episode that is running at the end ([batch x taps-1 x channels], rows of an earlier episode zero).
+ * Backward: dy, dfinal (or NULL) in; dx, dweight, dbias (or NULL), dinitial (or NULL) out. */
+typedef struct ppn_conv_args {
+  int64_t struct_bytes, type, silu, batch, time, channels, taps;
+  const void* x; int64_t x_batch, x_time;
+  const float* weight;                 /* [channels x taps] */
+  const float* bias;                   /* [channels] or NULL */
+  const void* initial;                 /* [batch x taps-1 x channels] or NULL */
+  const uint8_t* starts; int64_t starts_batch, starts_time;   /* or NULL */
+  void* y; int64_t y_batch, y_time;
+  void* final_state;                   /* or NULL */
+  const void* dy; int64_t dy_batch, dy_time;
+  const void* dfinal;
+  void* dx; int64_t dx_batch, dx_time;
+  float* dweight; float* dbias; void* dinitial;
+  void* workspace; int64_t workspace_bytes;
+} ppn_conv_args;
+int ppn_conv_forward(const ppn_conv_args* a, void* stream);
+int64_t ppn_conv_backward_workspace(const ppn_conv_args* a);
+int ppn_conv_backward(const ppn_conv_args* a, void* stream);
+
+/* One row of each of `rows` environments: row i belongs to environment env_ids[i] (i when NULL), whose window
+ * state[env] ([taps-1 x channels]) moves on by one row.  A row with a negative id is padding: y = 0, no state is touched.
+ * An id >= environments, or one that an earlier row has, gives y = NaN and touches no state. */
+typedef struct ppn_conv_step_args {
+  int64_t struct_bytes, type, silu, rows, environments, channels, taps;
+  const void* x; int64_t x_row;
+  const float* weight; const float* bias;
+  void* state;                         /* [environments x taps-1 x channels], updated */
+  const int32_t* env_ids;              /* [rows] or NULL (then rows <= environments) */
+  const uint8_t* starts;               /* [rows] or NULL */
+  void* y; int64_t y_row;
+} ppn_conv_step_args;
+int ppn_conv_step(const ppn_conv_step_args* a, void* stream);
+
+/* Selective state space scan; group of channel d: g(d) = d / (channels / groups):
+ *   delta = dt + dt_bias, then log(1 + e^delta) when softplus;   h[t,d,n] = exp(delta A[d,n]) h[t-1,d,n] + delta B[t,g(d),n] x[t,d]
+ *   y[t,d] = (sum_n C[t,g(d),n] h[t,d,n] + D[d] x[t,d]) * z / (1 + e^-z)    (D, z, dt_bias or NULL)
+ * h is 0 in front of a row marked in starts, `initial` (or 0) in front of row 0.  1 <= states <= 64.
+ * `checkpoints` (training; NULL otherwise): ppn_scan_checkpoint_bytes bytes the backward pass reads again.
+ * Backward: dy, dfinal (or NULL) in; dx, ddt, dB, dC and (each or NULL) dA, dD, dz, ddt_bias, dinitial out. */
+typedef struct ppn_scan_args {
+  int64_t struct_bytes, type, softplus, batch, time, channels, groups, states;
+  const void* x; int64_t x_batch, x_time;
+  const void* dt; int64_t dt_batch, dt_time;
+  const float* A;                      /* [channels x states] */
+  const void* B; int64_t B_batch, B_time, B_group;
+  const void* C; int64_t C_batch, C_time, C_group;
+  const float* D; const float* dt_bias;
+  const void* z; int64_t z_batch, z_time;
+  const uint8_t* starts; int64_t starts_batch, starts_time;
+  const float* initial;                /* [batch x channels x states] */
+  void* y; int64_t y_batch, y_time;
+  float* final_state;                  /* [batch x channels x states] or NULL */
+  float* checkpoints;
+  const void* dy; int64_t dy_batch, dy_time;
+  const float* dfinal;
+  void* dx; int64_t dx_batch, dx_time;
+  void* ddt; int64_t ddt_batch, ddt_time;
+  void* dz; int64_t dz_batch, dz_time;
+  void* dB; void* dC;                  /* [batch x time x groups x states], contiguous */
+  float* dA; float* dD; float* ddt_bias; float* dinitial;
+  void* workspace; int64_t workspace_bytes;
+} ppn_scan_args;
+int64_t ppn_scan_checkpoint_bytes(const ppn_scan_args* a);
+int64_t ppn_scan_forward_workspace(const ppn_scan_args* a);
+int ppn_scan_forward(const ppn_scan_args* a, void* stream);
+int64_t ppn_scan_backward_workspace(const ppn_scan_args* a);
+int ppn_scan_backward(const ppn_scan_args* a, void* stream);
+
+/* One row of each of `rows` environments; ids and starts as in ppn_conv_step. */
+typedef struct ppn_scan_step_args {
+  int64_t struct_bytes, type, softplus, rows, environments, channels, groups, states;
+  const void* x; int64_t x_row;
+  const void* dt; int64_t dt_row;
+  const float* A;
+  const void* B; int64_t B_row, B_group;
+  const void* C; int64_t C_row, C_group;
+  const float* D; const float* dt_bias;
+  const void* z; int64_t z_row;
+  float* state;                        /* [environments x channels x states], updated */
+  const int32_t* env_ids; const uint8_t* starts;
+  void* y; int64_t y_row;
+} ppn_scan_step_args;
+int ppn_scan_step(const ppn_scan_step_args* a, void* stream);
+
+/* Cross entropy over a catalogue of actions, without keeping the logits:
+ *   loss[i] = log sum_{v allowed} exp(hidden[i] . weight[v]) - hidden[i] . weight[target[i]]
+ * allowed: bit v & 31 of word v >> 5 of row i (NULL: every action).  target = ignore_index, or a row with nothing
+ * allowed: loss 0, no gradient.  A target that is not allowed: loss +inf.  A target outside 0..actions-1: loss NaN, and so
+ * its gradients.  lse (log of the sum; saved for the backward pass): +inf where the row has no gradient.
+ * Backward: dloss[rows] in; dhidden [rows x features], dweight [actions x features] (each or NULL) out, contiguous. */
+typedef struct ppn_loss_args {
+  int64_t struct_bytes, type, rows, actions, features, ignore_index;
+  const void* hidden; int64_t hidden_row;
+  const void* weight; int64_t weight_row;
+  const int64_t* target;
+  const int32_t* allowed; int64_t allowed_row;
+  float* loss; float* lse;
+  const float* dloss;
+  void* dhidden; void* dweight;
+  void* workspace; int64_t workspace_bytes;
+} ppn_loss_args;
+int64_t ppn_loss_forward_workspace(const ppn_loss_args* a);
+int ppn_loss_forward(const ppn_loss_args* a, void* stream);
+int64_t ppn_loss_backward_workspace(const ppn_loss_args* a);
+int ppn_loss_backward(const ppn_loss_args* a, void* stream);
+
 /* ---- introspection --------------------------------------------------------------------------------- */
 int32_t ppn_dim(const ppn_engine* e, int32_t which);   /* 0 nS, 1 nP, 2 nL, 3 nl, 4 action_len, 5 obs_len,
                                                           6 batch, 7 lds_bytes, 8 max_active_buses,

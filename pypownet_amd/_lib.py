@@ -90,7 +90,32 @@ EXPORTS = ['ppn_create', 'ppn_destroy', 'ppn_last_error', 'ppn_set_thermal_limit
            'ppn_read', 'ppn_write', 'ppn_sync', 'ppn_stream', 'ppn_kernel_time', 'ppn_dim', 'ppn_version', 'ppn_set_reward',
            'ppn_simulate_candidates', 'ppn_read_observation', 'ppn_observation_length', 'ppn_wait', 'ppn_runpf_arrays', 'ppn_rollout',
            'ppn_policy_actions', 'ppn_rollout_policy', 'ppn_step_observe', 'ppn_async_start', 'ppn_send', 'ppn_recv', 'ppn_async_stop',
-           'ppn_async_stream', 'ppn_async_stat', 'ppn_restart_memo', 'ppn_restart_memo_stat']
+           'ppn_async_stream', 'ppn_async_stat', 'ppn_restart_memo', 'ppn_restart_memo_stat',
+           'ppn_policy_error', 'ppn_conv_forward', 'ppn_conv_backward_workspace', 'ppn_conv_backward', 'ppn_conv_step', 'ppn_scan_checkpoint_bytes',
+           'ppn_scan_forward_workspace', 'ppn_scan_forward', 'ppn_scan_backward_workspace', 'ppn_scan_backward', 'ppn_scan_step',
+           'ppn_loss_forward_workspace', 'ppn_loss_forward', 'ppn_loss_backward_workspace', 'ppn_loss_backward']
+
+
+# Structs of the policy operators (include/ppn.h): 64-bit fields only, in this order, so a call packs them with one struct.pack.
+POLICY_STRUCTS = {
+    'ppn_conv_args': (
+        'struct_bytes type silu batch time channels taps x x_batch x_time weight bias initial starts starts_batch starts_time y '
+        'y_batch y_time final_state dy dy_batch dy_time dfinal dx dx_batch dx_time dweight dbias dinitial workspace '
+        'workspace_bytes ').split(),
+    'ppn_conv_step_args': (
+        'struct_bytes type silu rows environments channels taps x x_row weight bias state env_ids starts y y_row ').split(),
+    'ppn_scan_args': (
+        'struct_bytes type softplus batch time channels groups states x x_batch x_time dt dt_batch dt_time A B B_batch B_time '
+        'B_group C C_batch C_time C_group D dt_bias z z_batch z_time starts starts_batch starts_time initial y y_batch y_time '
+        'final_state checkpoints dy dy_batch dy_time dfinal dx dx_batch dx_time ddt ddt_batch ddt_time dz dz_batch dz_time dB dC '
+        'dA dD ddt_bias dinitial workspace workspace_bytes ').split(),
+    'ppn_scan_step_args': (
+        'struct_bytes type softplus rows environments channels groups states x x_row dt dt_row A B B_row B_group C C_row C_group '
+        'D dt_bias z z_row state env_ids starts y y_row ').split(),
+    'ppn_loss_args': (
+        'struct_bytes type rows actions features ignore_index hidden hidden_row weight weight_row target allowed allowed_row loss '
+        'lse dloss dhidden dweight workspace workspace_bytes ').split(),
+}
 
 
 def _preload_torch_hip_runtime():
@@ -203,6 +228,17 @@ def bind_signatures(lib, full_abi=True):
         lib.ppn_restart_memo.restype = C.c_int
         lib.ppn_restart_memo_stat.argtypes = [vp, C.c_int32]
         lib.ppn_restart_memo_stat.restype = C.c_int64
+    if hasattr(lib, 'ppn_policy_error'):          # (the emulation build of the engine has no policy operators)
+        lib.ppn_policy_error.argtypes = []
+        lib.ppn_policy_error.restype = C.c_char_p
+        for name in ('ppn_conv_forward', 'ppn_conv_backward', 'ppn_conv_step', 'ppn_scan_forward', 'ppn_scan_backward', 'ppn_scan_step',
+                     'ppn_loss_forward', 'ppn_loss_backward'):
+            f = getattr(lib, name)
+            f.argtypes, f.restype = [C.c_char_p, vp], C.c_int          # (a packed struct, a stream)
+        for name in ('ppn_conv_backward_workspace', 'ppn_scan_checkpoint_bytes', 'ppn_scan_forward_workspace', 'ppn_scan_backward_workspace',
+                     'ppn_loss_forward_workspace', 'ppn_loss_backward_workspace'):
+            f = getattr(lib, name)
+            f.argtypes, f.restype = [C.c_char_p], C.c_int64
     lib.ppn_stream.argtypes = [vp]
     lib.ppn_stream.restype = vp
     lib.ppn_kernel_time.argtypes = [vp, C.c_int32, C.POINTER(C.c_double), C.POINTER(C.c_int64)]

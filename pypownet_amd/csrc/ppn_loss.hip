@@ -1,0 +1,536 @@
+// ppn_loss.hip -- cross entropy over a catalogue of actions, without keeping the logits.
+//
+//   loss[i] = log sum_v exp(l[i,v]) - l[i,target]      l[i,v] = hidden[i] . weight[v], over the allowed actions
+//   dl[i,v] = (exp(l[i,v] - lse[i]) - [v = target]) dloss[i]      dhidden = dl weight      dweight = dl^T hidden
+//
+// Bound by the matrix units: 2 rows x actions x features operations forward, three times that and the logits once more backward.  One
+// matrix product serves all four: C = A B^T with both operands' inner dimension contiguous, 32-bit sums, and an epilogue that differs:
+//   logits -> running maximum and sum of exponentials per row and tile (nothing else leaves the chip),
+//   logits -> dl of a piece of the catalogue, rounded to the operands' type and laid out both ways (dl and its transpose),
+//   dl and dl^T against transposed copies of weight and hidden -> the two gradients.
+// The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size.
+//
+// Rounding dl to 16 bits (as the operand of a 16-bit product it has to be) is off by half a step of each entry, 2^-9 for bfloat16 and
+// 2^-12 for float16, independent from entry to entry; the gradients' own rounding is as large.  float16's range would lose small
+// probabilities, so dl is scaled by a power of two that brings the largest |dloss| to 2^14, and the scale is taken out at the end.
+#include "ppn_policy.h"
+
+namespace ppn_policy {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of each operand (of a lane) into a 16 x 16 tile of sums: inner positions (lane / 16) * 16 bytes ..
+__device__ inline void multiply(f32x4& c, u32x4 a, u32x4 b, __bf16) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ inline void multiply(f32x4& c, u32x4 a, u32x4 b, _Float16) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ inline void multiply(f32x4& c, u32x4 a, u32x4 b, float) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+}
+
+// Operands of one product: C[m, n] = sum_k A[m, k] B[n, k]; the inner dimension padded to whole 64-byte rows, rows 16-byte aligned.
+struct Operands {
+  const void* A; int64_t lda, M;
+  const void* B; int64_t ldb, N;
+  int64_t K;                      // padded
+};
+
+struct StatsArgs { const int32_t* allowed; int64_t allowed_row; const int64_t* target; float2* partial; float* wanted; int64_t columns; };
+struct GradArgs {
+  const int32_t* allowed; int64_t allowed_row; const int64_t* target; const float* lse; const float* dloss; const float* scale;
+  void* dl; int64_t dl_row; void* dlt; int64_t dlt_row; int64_t first, rows_padded, cols_padded;
+};
+struct SumArgs { float* sums; int64_t slots; bool add; };
+
+constexpr int LINE = 64;          // bytes of the inner dimension per step
+
+// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go through LDS, two buffers, read from memory
+// one step ahead into registers.  A line's four 16-byte parts are stored with part ^ (row / 2 % 4), so that the 16 rows a fragment read
+// touches fall into different banks.
+template <typename T, int MI, int NI, int WM, int WN> struct Product {
+  static constexpr int BM = 16 * MI * WM, BN = 16 * NI * WN, THREADS = 64 * WM * WN;
+  static constexpr int LOADS = (BM + BN) * 4 / THREADS;
+  static constexpr int LDS_BYTES = 2 * (BM + BN) * LINE;
+  static_assert((BM + BN) * 4 % THREADS == 0, "");
+
+  f32x4 c[MI][NI];
+  int wave_m, wave_n, lane;
+
+  __device__ static int spot(int row, int part) { return row * LINE + ((part ^ ((row >> 1) & 3)) << 4); }
+
+  __device__ void run(const Operands& o, char* lds, int64_t m0, int64_t n0, int64_t k0, int64_t k1) {
+    const int tid = threadIdx.x;
+    lane = tid & 63;
+    const int wave = tid >> 6;
+    wave_m = wave / WN * (16 * MI), wave_n = wave % WN * (16 * NI);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) c[i][j] = f32x4{0, 0, 0, 0};
+    const char* from[LOADS];
+    int to[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int e = tid + i * THREADS, row = e >> 2, part = e & 3;
+      to[i] = spot(row, part);
+      if (row < BM) {
+        int64_t m = m0 + row < o.M ? m0 + row : o.M - 1;
+        from[i] = (const char*)o.A + (m * o.lda + k0) * (int64_t)sizeof(T) + part * 16;
+      } else {
+        int64_t n = n0 + row - BM < o.N ? n0 + row - BM : o.N - 1;
+        from[i] = (const char*)o.B + (n * o.ldb + k0) * (int64_t)sizeof(T) + part * 16;
+      }
+    }
+    const int steps = (int)((k1 - k0) * (int64_t)sizeof(T) / LINE);
+    u32x4 held[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4*)from[i];
+    for (int s = 0; s < steps; ++s) {
+      char* buf = lds + (s & 1) * (BM + BN) * LINE;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) *(u32x4*)(buf + to[i]) = held[i];
+      if (s + 1 < steps) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4*)(from[i] + (int64_t)(s + 1) * LINE);
+      }
+      __syncthreads();
+      u32x4 a[MI], b[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) a[i] = *(const u32x4*)(buf + spot(wave_m + i * 16 + (lane & 15), lane >> 4));
+#pragma unroll
+      for (int j = 0; j < NI; ++j) b[j] = *(const u32x4*)(buf + spot(BM + wave_n + j * 16 + (lane & 15), lane >> 4));
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) multiply(c[i][j], a[i], b[j], T());
+    }
+    // (the buffer written two steps on is the one read now: the barrier between them is the next step's)
+  }
+  // Sum (i, j, r) of this lane: row wave_m + 16 i + 4 (lane / 16) + r, column wave_n + 16 j + lane % 16 of the tile.
+  __device__ int row_of(int i, int r) const { return wave_m + i * 16 + (lane >> 4) * 4 + r; }
+  __device__ int col_of(int j) const { return wave_n + j * 16 + (lane & 15); }
+};
+
+// Tiles are handed to the eight dies in turn, each with its own L2: neighbours in the list below go to one die, all row tiles of a
+// column tile one after the other, so that a die reads its share of the larger operand once.
+__device__ inline int64_t tile_of(int64_t id, int64_t count) {
+  const int64_t per = count / 8, whole = per * 8;
+  return id < whole ? (id % 8) * per + id / 8 : id;
+}
+
+__device__ inline bool is_allowed(const int32_t* allowed, int64_t at, int64_t col) { return !allowed || ((allowed[at + (col >> 5)] >> (col & 31)) & 1); }
+
+template <int PATTERN> __device__ inline float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
+}
+template <typename F> __device__ inline float over_16(float v, F f) {      // over the 16 lanes of a row of lanes
+  v = f(v, dpp<0x128>(v));      // row_ror:8
+  v = f(v, dpp<0x141>(v));      // row_half_mirror
+  v = f(v, dpp<0x4e>(v));       // quad_perm 2,3,0,1
+  return f(v, dpp<0xb1>(v));    // quad_perm 1,0,3,2
+}
+
+// Forward: of every row and every 16 NI columns the maximum and the sum of exp(l - maximum); the target's logit as it goes by.
+template <typename T, int MI, int NI, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) loss_stats(Operands o, StatsArgs s, int64_t tiles_m, int64_t tiles_n) {
+  typedef Product<T, MI, NI, WM, WN> P;
+  __shared__ __align__(16) char lds[P::LDS_BYTES];
+  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), m0 = tile % tiles_m * P::BM, n0 = tile / tiles_m * P::BN;
+  P p;
+  p.run(o, lds, m0, n0, 0, o.K);
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = m0 + p.row_of(i, r);
+      const bool in = row < o.M;
+      const int64_t at = (in ? row : o.M - 1) * s.allowed_row, target = s.target[in ? row : o.M - 1];
+      float top = -INFINITY, sum = 0.0f;
+      bool live[NI];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t col = n0 + p.col_of(j);
+        live[j] = col < o.N && is_allowed(s.allowed, at, col);
+        const float l = p.c[i][j][r];
+        if (live[j] && in && col == target) s.wanted[row] = l;
+        top = live[j] ? (l != l ? l : (top > l ? top : l)) : top;      // (a NaN stays the maximum, and the sum becomes NaN with it)
+      }
+      top = over_16(top, [](float a, float b) { return a != a ? a : b != b ? b : a > b ? a : b; });
+      const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sum += live[j] ? exp_fast(p.c[i][j][r] - ref) : 0.0f;
+      sum = over_16(sum, [](float a, float b) { return a + b; });
+      if (in && (p.lane & 15) == 0) s.partial[row * s.columns + (n0 + p.wave_n) / (16 * NI)] = make_float2(top, sum);
+    }
+}
+
+// One wave a row: joins the tiles' maxima and sums.
+__global__ void __launch_bounds__(256) loss_join(const float2* partial, int64_t columns, const float* wanted, const int64_t* target, const int32_t* allowed,
+                                                 int64_t allowed_row, int64_t rows, int64_t actions, int64_t ignore, float* loss, float* lse) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  float top = -INFINITY, sum = 0.0f;
+  auto join = [&](float t, float s) {
+    if (t == -INFINITY) return;
+    const float high = t != t || top != top ? NAN : t > top ? t : top;
+    sum = (top == -INFINITY ? 0.0f : sum * exp_fast(top - high)) + s * exp_fast(t - high);
+    top = high;
+  };
+  for (int64_t c = lane; c < columns; c += 64) {
+    const float2 v = partial[row * columns + c];
+    join(v.x, v.y);
+  }
+  for (int d = 32; d; d >>= 1) {
+    const float t = __shfl_xor(top, d), s = __shfl_xor(sum, d);
+    join(t, s);
+  }
+  if (lane) return;
+  const int64_t at = target[row];
+  const bool nothing = top == -INFINITY, inside = at >= 0 && at < actions;
+  const float whole = top + 0.693147180559945309f * __builtin_amdgcn_logf(sum);
+  if (at == ignore || nothing) {
+    loss[row] = 0.0f, lse[row] = INFINITY;
+  } else if (!inside) {
+    loss[row] = NAN, lse[row] = NAN;
+  } else {
+    loss[row] = is_allowed(allowed, row * allowed_row, at) ? whole - wanted[row] : INFINITY;
+    lse[row] = whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
+  }
+}
+
+// scale[0] = the power of two dl is multiplied by, scale[1] = 1 / it.
+__global__ void __launch_bounds__(256) loss_scale(const float* dloss, const float* lse, int64_t rows, bool needed, float* scale) {
+  __shared__ float tops[256];
+  float top = 0.0f;
+  if (needed)
+    for (int64_t i = threadIdx.x; i < rows; i += 256) {
+      const float g = fabsf(dloss[i]);
+      if (lse[i] != INFINITY && g < INFINITY && g > top) top = g;
+    }
+  tops[threadIdx.x] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 256; ++i) top = tops[i] > top ? tops[i] : top;
+    int e = 0;
+    if (top > 0.0f) frexpf(top, &e);
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    scale[0] = needed && top > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
+    scale[1] = needed && top > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
+  }
+}
+
+// Backward, first product: dl of the columns first .. first + N of the catalogue, [rows x cols_padded] and [N x rows_padded], zeros in the padding.
+template <typename T, int MI, int NI, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) loss_grad(Operands o, GradArgs g, int64_t tiles_m, int64_t tiles_n) {
+  typedef Product<T, MI, NI, WM, WN> P;
+  __shared__ __align__(16) char lds[P::LDS_BYTES];
+  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), m0 = tile % tiles_m * P::BM, n0 = tile / tiles_m * P::BN;
+  P p;
+  p.run(o, lds, m0, n0, 0, o.K);
+  const float scale = g.scale[0];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    T out[NI][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = m0 + p.row_of(i, r), safe = row < o.M ? row : o.M - 1;
+      const float lse = row < o.M ? g.lse[safe] : INFINITY, up = lse == INFINITY ? 0.0f : g.dloss[safe] * scale;
+      const int64_t target = lse == INFINITY ? -1 : g.target[safe] - g.first;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t col = n0 + p.col_of(j);
+        float v = 0.0f;
+        if (lse != INFINITY && col < o.N) {
+          const bool live = is_allowed(g.allowed, safe * g.allowed_row, col + g.first);
+          v = live ? (exp_fast(p.c[i][j][r] - lse) - (col == target ? 1.0f : 0.0f)) * up : lse != lse ? lse : 0.0f;
+        }
+        out[j][r] = (T)v;
+        if (row < o.M && col < g.cols_padded) ((T*)g.dl)[row * g.dl_row + col] = out[j][r];
+      }
+    }
+    const int64_t row = m0 + p.row_of(i, 0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t col = n0 + p.col_of(j);
+      if (col < o.N && row < g.rows_padded) {      // rows_padded is a multiple of 16: the four rows are in or out together
+        struct alignas(4 * sizeof(T)) Four { T v[4]; } f = {{out[j][0], out[j][1], out[j][2], out[j][3]}};
+        *(Four*)((T*)g.dlt + col * g.dlt_row + row) = f;
+      }
+    }
+  }
+}
+
+// Backward, second products: 32-bit sums of one share of the inner dimension (grid.y shares, a slot of [M x N] floats each).
+template <typename T, int MI, int NI, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) loss_sums(Operands o, SumArgs s, int64_t share, int64_t tiles_m, int64_t tiles_n) {
+  typedef Product<T, MI, NI, WM, WN> P;
+  __shared__ __align__(16) char lds[P::LDS_BYTES];
+  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), n0 = tile % tiles_n * P::BN, m0 = tile / tiles_n * P::BM;
+  const int64_t k0 = blockIdx.y * share, k1 = k0 + share < o.K ? k0 + share : o.K;
+  P p;
+  p.run(o, lds, m0, n0, k0, k1);
+  float* sums = s.sums + blockIdx.y * o.M * o.N;
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = m0 + p.row_of(i, r);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t col = n0 + p.col_of(j);
+        if (row < o.M && col < o.N) {
+          float* at = sums + row * o.N + col;
+          *at = s.add ? *at + p.c[i][j][r] : p.c[i][j][r];
+        }
+      }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) loss_finish(const float* sums, int64_t slots, int64_t count, const float* scale, T* out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  float v = 0.0f;
+  for (int64_t s = 0; s < slots; ++s) v += sums[s * count + i];
+  out[i] = (T)(v * scale[1]);
+}
+
+// [rows x cols] with any row stride -> [rows x cols_padded], zeros in the padding.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_pad(const T* in, int64_t in_row, int64_t rows, int64_t cols, T* out, int64_t cols_padded) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * cols_padded) return;
+  const int64_t r = i / cols_padded, c = i - r * cols_padded;
+  out[i] = c < cols ? in[r * in_row + c] : (T)0.0f;
+}
+
+// [rows x cols] with any row stride -> [cols x rows_padded], zeros in the padding.  64 x 64 tiles through LDS.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_transpose(const T* in, int64_t in_row, int64_t rows, int64_t cols, T* out, int64_t rows_padded) {
+  __shared__ T tile[64][64 + 4 / sizeof(T)];
+  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 64; i += 4) {
+    const int64_t r = r0 + y + i, c = c0 + x;
+    tile[y + i][x] = r < rows && c < cols ? in[r * in_row + c] : (T)0.0f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 64; i += 4) {
+    const int64_t c = c0 + y + i, r = r0 + x;
+    if (c < cols && r < rows_padded) out[c * rows_padded + r] = tile[x][y + i];
+  }
+}
+
+// ---- plans -------------------------------------------------------------------------------------------------------------------------
+int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t inner(const ppn_loss_args* a) { return LINE / size_of(a->type); }
+
+bool in_place(const void* p, int64_t row, int64_t features, int64_t type) {
+  return features % (LINE / size_of(type)) == 0 && row * size_of(type) % 16 == 0 && aligned(p, 16);
+}
+
+struct Config { int64_t bm, bn, columns_per_wave; bool large; };
+// 256 x 128 tiles where they fill the chip's 256 CUs; 64 x 64 ones elsewhere.
+Config config_for(int64_t m, int64_t n, int64_t times) {
+  const bool large = ceil_div(m, 256) * ceil_div(n, 128) * times >= 256;
+  return large ? Config{256, 128, 64, true} : Config{64, 64, 32, false};
+}
+
+struct Layout { int64_t bytes = 0; int64_t take(int64_t n) { int64_t at = bytes; bytes += padded(n, 256); return at; } };
+
+struct ForwardPlan { Config config; int64_t columns, features_padded, hidden, weight, partial, wanted, bytes; };
+ForwardPlan plan_forward(const ppn_loss_args* a) {
+  ForwardPlan p;
+  Layout l;
+  const int64_t size = size_of(a->type);
+  p.features_padded = padded(a->features, inner(a));
+  p.config = config_for(a->rows, a->actions, 1);
+  p.columns = padded(a->actions, p.config.bn) / p.config.columns_per_wave;
+  p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
+  p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
+  p.partial = l.take(a->rows * p.columns * 8);
+  p.wanted = l.take(a->rows * 4);
+  p.bytes = l.bytes;
+  return p;
+}
+
+struct BackwardPlan {
+  int64_t features_padded, rows_padded, actions_padded, piece, hidden, weight, hidden_t, weight_t, dl, dlt, scale, dh, dw, bytes;
+  Config grad, dh_config, dw_config;
+  int64_t dh_share, dh_slots, dw_share, dw_slots;
+};
+
+// Shares of the inner dimension K that bring a product of few tiles to about 512 workgroups, at least 512 long each.
+void split_inner(const Config& c, int64_t m, int64_t n, int64_t k, int64_t unit, int64_t* share, int64_t* slots) {
+  const int64_t tiles = ceil_div(m, c.bm) * ceil_div(n, c.bn);
+  int64_t want = 512 / tiles;
+  if (want > k / 512) want = k / 512;
+  if (want < 1) want = 1;
+  *share = padded(ceil_div(k, want), unit);
+  *slots = ceil_div(k, *share);
+}
+
+BackwardPlan plan_backward(const ppn_loss_args* a) {
+  BackwardPlan p;
+  Layout l;
+  const int64_t size = size_of(a->type), unit = inner(a);
+  p.features_padded = padded(a->features, unit);
+  p.rows_padded = padded(a->rows, 32);
+  p.actions_padded = padded(a->actions, 32);
+  // a piece's dl and its transpose take 64 MB each: both stay in the last-level cache between the kernel that writes and those that read them
+  p.piece = padded((int64_t)(64 << 20) / (p.rows_padded * size), 128);
+  if (p.piece < 1024) p.piece = 1024;
+  if (p.piece > p.actions_padded) p.piece = p.actions_padded;
+  p.grad = config_for(a->rows, p.piece, 1);
+  p.dh_config = config_for(a->rows, a->features, p.piece / 1024 + 1);
+  p.dw_config = config_for(p.piece, a->features, a->rows / 1024 + 1);
+  split_inner(p.dh_config, a->rows, a->features, p.piece, unit, &p.dh_share, &p.dh_slots);
+  split_inner(p.dw_config, p.piece, a->features, p.rows_padded, unit, &p.dw_share, &p.dw_slots);
+  p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
+  p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
+  p.hidden_t = l.take(a->features * p.rows_padded * size);
+  p.weight_t = l.take(a->features * p.actions_padded * size);
+  p.dl = l.take(a->rows * p.piece * size);
+  p.dlt = l.take(p.piece * p.rows_padded * size);
+  p.scale = l.take(8);
+  p.dh = l.take(p.dh_slots * a->rows * a->features * 4);
+  p.dw = l.take(p.dw_slots * p.piece * a->features * 4);
+  p.bytes = l.bytes;
+  return p;
+}
+
+int check(const ppn_loss_args* a) {
+  if (!a || a->struct_bytes != (int64_t)sizeof *a) return fail(PPN_E_INVALID, "ppn_loss_args: struct_bytes does not match this library");
+  if (a->type < 0 || a->type > PPN_T_F16) return fail(PPN_E_INVALID, "element type %lld is unknown", (long long)a->type);
+  if (a->rows < 0 || a->actions < 1 || a->features < 1) return fail(PPN_E_INVALID, "loss: rows >= 0, actions >= 1 and features >= 1 are needed");
+  if (a->rows > (1 << 27) || a->actions > (1 << 27) || a->features > (1 << 20)) return fail(PPN_E_INVALID, "loss: a size is out of range");
+  return PPN_OK;
+}
+
+template <typename T> int pad_rows(const void* in, int64_t row, int64_t rows, int64_t cols, void* out, int64_t cols_padded, hipStream_t s) {
+  const int64_t blocks = ceil_div(rows * cols_padded, 256);
+  if (blocks > 0x7fffffff) return fail(PPN_E_INVALID, "loss: an operand is too large");
+  loss_pad<T><<<dim3(blocks), dim3(256), 0, s>>>((const T*)in, row, rows, cols, (T*)out, cols_padded);
+  return PPN_OK;
+}
+
+}  // namespace
+}  // namespace ppn_policy
+
+using namespace ppn_policy;
+
+extern "C" int64_t ppn_loss_forward_workspace(const ppn_loss_args* a) {
+  if (int rc = check(a)) return rc;
+  return plan_forward(a).bytes;
+}
+
+extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
+  if (int rc = check(a)) return rc;
+  if (a->rows == 0) return PPN_OK;
+  if (!a->hidden || !a->weight || !a->target || !a->loss || !a->lse) return fail(PPN_E_INVALID, "ppn_loss_forward: hidden, weight, target, loss and lse are needed");
+  if (a->allowed && a->allowed_row < ceil_div(a->actions, 32)) return fail(PPN_E_INVALID, "ppn_loss_forward: a row of allowed has too few words");
+  const ForwardPlan p = plan_forward(a);
+  if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_forward: the workspace is too small");
+  char* w = (char*)a->workspace;
+  hipStream_t s = (hipStream_t)stream;
+  return by_type(a->type, [&](auto* t) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    Operands o = {a->hidden, a->hidden_row, a->rows, a->weight, a->weight_row, a->actions, p.features_padded};
+    if (p.hidden >= 0) {
+      if (int rc = pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s)) return rc;
+      o.A = w + p.hidden, o.lda = p.features_padded;
+    }
+    if (p.weight >= 0) {
+      if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
+      o.B = w + p.weight, o.ldb = p.features_padded;
+    }
+    const StatsArgs st = {a->allowed, a->allowed_row, a->target, (float2*)(w + p.partial), (float*)(w + p.wanted), p.columns};
+    const int64_t tm = ceil_div(a->rows, p.config.bm), tn = ceil_div(a->actions, p.config.bn);
+    if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
+    if (p.config.large) loss_stats<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
+    else loss_stats<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
+    loss_join<<<dim3(ceil_div(a->rows, 4)), dim3(256), 0, s>>>(st.partial, p.columns, st.wanted, a->target, a->allowed, a->allowed_row, a->rows, a->actions,
+                                                               a->ignore_index, a->loss, a->lse);
+    return launched("ppn_loss_forward");
+  });
+}
+
+extern "C" int64_t ppn_loss_backward_workspace(const ppn_loss_args* a) {
+  if (int rc = check(a)) return rc;
+  return plan_backward(a).bytes;
+}
+
+extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
+  if (int rc = check(a)) return rc;
+  if (a->rows == 0) return fail(PPN_E_INVALID, "ppn_loss_backward: there are no rows");
+  if (!a->hidden || !a->weight || !a->target || !a->lse || !a->dloss) return fail(PPN_E_INVALID, "ppn_loss_backward: hidden, weight, target, lse and dloss are needed");
+  if (a->allowed && a->allowed_row < ceil_div(a->actions, 32)) return fail(PPN_E_INVALID, "ppn_loss_backward: a row of allowed has too few words");
+  const BackwardPlan p = plan_backward(a);
+  if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_backward: the workspace is too small");
+  char* w = (char*)a->workspace;
+  hipStream_t s = (hipStream_t)stream;
+  float* scale = (float*)(w + p.scale);
+  return by_type(a->type, [&](auto* t) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    const void* hidden = a->hidden;
+    const void* weight = a->weight;
+    int64_t hidden_row = a->hidden_row, weight_row = a->weight_row;
+    if (p.hidden >= 0) {
+      if (int rc = pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s)) return rc;
+      hidden = w + p.hidden, hidden_row = p.features_padded;
+    }
+    if (p.weight >= 0) {
+      if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
+      weight = w + p.weight, weight_row = p.features_padded;
+    }
+    if (a->dweight)
+      loss_transpose<T><<<dim3(ceil_div(p.rows_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->hidden, a->hidden_row, a->rows, a->features,
+                                                                                                          (T*)(w + p.hidden_t), p.rows_padded);
+    if (a->dhidden)
+      loss_transpose<T><<<dim3(ceil_div(p.actions_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->weight, a->weight_row, a->actions,
+                                                                                                             a->features, (T*)(w + p.weight_t), p.actions_padded);
+    loss_scale<<<dim3(1), dim3(256), 0, s>>>(a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale);
+    for (int64_t first = 0; first < a->actions; first += p.piece) {
+      const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 32);
+      const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
+      const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
+      const int64_t tm = ceil_div(a->rows, p.grad.bm), tn = ceil_div(n, p.grad.bn);
+      if (p.grad.large) loss_grad<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);
+      else loss_grad<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);
+      if (a->dhidden) {
+        const Operands q = {w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np};
+        const int64_t um = ceil_div(a->rows, p.dh_config.bm), un = ceil_div(a->features, p.dh_config.bn);
+        // (the last piece is shorter: a share that begins past its end adds nothing, so every slot is written by the first piece)
+        const SumArgs sums = {(float*)(w + p.dh), p.dh_slots, first > 0};
+        const dim3 grid(um * un, first > 0 ? ceil_div(np, p.dh_share) : p.dh_slots);
+        if (p.dh_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
+        else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
+      }
+      if (a->dweight) {
+        const Operands q = {w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded};
+        const int64_t um = ceil_div(n, p.dw_config.bm), un = ceil_div(a->features, p.dw_config.bn);
+        const SumArgs sums = {(float*)(w + p.dw), p.dw_slots, false};
+        const dim3 grid(um * un, p.dw_slots);
+        if (p.dw_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
+        else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
+        loss_finish<T><<<dim3(ceil_div(n * a->features, 256)), dim3(256), 0, s>>>((const float*)(w + p.dw), p.dw_slots, n * a->features, scale,
+                                                                                   (T*)a->dweight + first * a->features);
+      }
+    }
+    if (a->dhidden)
+      loss_finish<T><<<dim3(ceil_div(a->rows * a->features, 256)), dim3(256), 0, s>>>((const float*)(w + p.dh), p.dh_slots, a->rows * a->features, scale,
+                                                                                      (T*)a->dhidden);
+    return launched("ppn_loss_backward");
+  });
+}

@@ -1,0 +1,477 @@
+"""Operators of learned policies, as hand-written HIP kernels (include/ppn.h, "operators of learned policies").
+
+A policy that acts on a ``BatchedRunEnv`` sees one observation row per environment and step; these are the parts of it that are
+not plain matrix products:
+
+* ``short_conv`` / ``short_conv_step``: short causal convolution over an environment's rows,
+* ``selective_scan`` / ``selective_scan_step``: selective state space scan over an environment's rows (its memory),
+* ``action_cross_entropy``: cross entropy over a catalogue of switching actions, without keeping the logits.
+
+The window forms take ``[batch, time, ...]`` tensors of recorded rollouts -- any strides, so rollouts recorded step by step are passed as
+``recorded.transpose(0, 1)`` -- and are differentiable; ``starts`` marks the first row of an episode, where memory begins empty.  The step
+forms take one row of each listed environment and update that environment's state in place; they have no gradient.
+
+Tensors are float32, bfloat16 or float16 on the GPU, all activations of a call of one type; parameters (convolution weights, ``A``, ``D``,
+``dt_bias``) and states are float32 -- the convolution's window excepted, which holds rows and has their type.  Kernels are queued on torch's
+current stream of the tensors' device; nothing synchronises.  Workspaces come from torch's allocator, so the calls can be captured into a
+graph.  Arguments the kernels do not take are refused with TypeError / ValueError before anything is launched; gradients of gradients are
+not available.
+"""
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .engine import EngineError
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_packers = {name: struct.Struct('%dq' % len(fields)) for name, fields in _lib.POLICY_STRUCTS.items()}
+_CONV, _CONV_STEP, _SCAN, _SCAN_STEP, _LOSS = (_packers[n] for n in ('ppn_conv_args', 'ppn_conv_step_args', 'ppn_scan_args', 'ppn_scan_step_args',
+                                                                      'ppn_loss_args'))
+_library = None
+
+
+def _load():
+    global _library
+    if _library is None:
+        _library = _lib.load_library()
+    return _library
+
+
+def _call(function, packed, device):
+    """Queues one entry point on torch's current stream of `device`."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = function(packed, torch.cuda.current_stream().cuda_stream)
+    else:
+        rc = function(packed, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        _refused(rc)
+
+
+def _refused(rc):
+    text = _load().ppn_policy_error().decode()
+    raise (ValueError if rc == -1 else EngineError)(text)
+
+
+def _workspace(size, device):
+    if size < 0:
+        _refused(size)
+    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+# ---- arguments -----------------------------------------------------------------------------------------------------------------------
+
+def _need(condition, *text):
+    if not condition:
+        raise ValueError(' '.join(str(t) for t in text))
+
+
+def _leading(name, x):
+    """The tensor that names a call's type and device."""
+    if not torch.is_tensor(x):
+        raise TypeError('%s must be a torch tensor, got %s' % (name, type(x).__name__))
+    if x.dtype not in _TYPES:
+        raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, x.dtype))
+    _need(x.is_cuda, name, 'must live on a GPU: these operators have no CPU form')
+    return _TYPES[x.dtype]
+
+
+def _like(name, t, shape, dtype, device):
+    if not torch.is_tensor(t):
+        raise TypeError('%s must be a torch tensor, got %s' % (name, type(t).__name__))
+    if t.dtype != dtype:
+        raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
+    if t.device != device or tuple(t.shape) != shape:
+        raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
+
+
+def _rows(t):
+    """Neighbouring channels next to each other in memory, as the kernels read them; a copy where they are not."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _flags(name, t, shape, device):
+    if t is None:
+        return None
+    if not torch.is_tensor(t):
+        raise TypeError('%s must be a torch tensor, got %s' % (name, type(t).__name__))
+    if t.dtype not in (torch.bool, torch.uint8):
+        raise TypeError('%s must be bool or uint8, got %s' % (name, t.dtype))
+    if t.device != device or tuple(t.shape) != shape:
+        raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
+    return t
+
+
+def _window_like(x):
+    """An output with x's order in memory: time outermost where x has it outermost."""
+    b, t, d = x.shape
+    if b > 1 and t > 1 and x.stride(0) < x.stride(1):
+        return torch.empty((t, b, d), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+
+
+def _at(t):
+    """Address, batch stride, time stride."""
+    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _step_ids(env_ids, rows, environments, device):
+    if env_ids is None:
+        _need(rows <= environments, 'there are', rows, 'rows and', environments, 'environments: env_ids must say whose rows they are')
+        return None
+    if not torch.is_tensor(env_ids):
+        raise TypeError('env_ids must be a torch tensor, got %s' % type(env_ids).__name__)
+    if env_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError('env_ids must be int32 or int64, got %s' % env_ids.dtype)
+    if env_ids.device != device or tuple(env_ids.shape) != (rows,):
+        raise ValueError('env_ids must be [%d] on %s, got %s on %s' % (rows, device, list(env_ids.shape), env_ids.device))
+    if env_ids.dtype == torch.int64:
+        # (an id that does not fit stays out of range instead of wrapping round to somebody's)
+        env_ids = env_ids.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return env_ids.contiguous()
+
+
+# ---- short causal convolution --------------------------------------------------------------------------------------------------------
+
+def _conv_args(x, weight, bias, initial, starts, silu, y=None, final=None, dy=None, dfinal=None, dx=None, dweight=None, dbias=None, dinitial=None,
+               workspace=None):
+    b, t, d = x.shape
+    return _CONV.pack(_CONV.size, _TYPES[x.dtype], silu, b, t, d, weight.shape[1], *_at(x), weight.data_ptr(), _ptr(bias), _ptr(initial), *_at(starts),
+                      *_at(y), _ptr(final), *_at(dy), _ptr(dfinal), *_at(dx), _ptr(dweight), _ptr(dbias), _ptr(dinitial), _ptr(workspace),
+                      0 if workspace is None else workspace.numel())
+
+
+def _conv_forward(x, weight, bias, initial, starts, silu, want_final):
+    y = _window_like(x)
+    final = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if want_final else None
+    _call(_load().ppn_conv_forward, _conv_args(x, weight, bias, initial, starts, silu, y, final), x.device)
+    return y, final
+
+
+class _ShortConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial, starts, silu, want_final):
+        ctx.set_materialize_grads(False)
+        x, weight = _rows(x), weight.contiguous()
+        bias, initial = (None if v is None else v.contiguous() for v in (bias, initial))
+        ctx.save_for_backward(x, weight, bias, initial, starts)
+        ctx.silu = silu
+        return _conv_forward(x, weight, bias, initial, starts, silu, want_final)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, weight, bias, initial, starts = ctx.saved_tensors
+        if dy is None and dfinal is None:
+            return (None,) * 7
+        dy = torch.zeros_like(x) if dy is None else _rows(dy)
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dx, dweight = _window_like(x), torch.empty_like(weight)
+        dbias = None if bias is None else torch.empty_like(bias)
+        dinitial = None if initial is None else torch.empty_like(initial)
+        given = dict(dy=dy, dfinal=dfinal, dx=dx, dweight=dweight, dbias=dbias, dinitial=dinitial)
+        lib = _load()
+        work = _workspace(lib.ppn_conv_backward_workspace(_conv_args(x, weight, bias, initial, starts, ctx.silu, **given)), x.device)
+        _call(lib.ppn_conv_backward, _conv_args(x, weight, bias, initial, starts, ctx.silu, workspace=work, **given), x.device)
+        return dx, dweight, dbias, dinitial, None, None, None
+
+
+def _activation(activation):
+    if activation not in (None, 'silu'):
+        raise ValueError("activation must be None or 'silu', got %r" % (activation,))
+    return 1 if activation else 0
+
+
+def _conv_parameters(channels, weight, bias, device):
+    _need(torch.is_tensor(weight) and weight.dim() == 2 and 2 <= weight.shape[1] <= 8, 'weight must be a tensor [channels, taps] with 2 to 8 taps')
+    _like('weight', weight, (channels, weight.shape[1]), torch.float32, device)
+    if bias is not None:
+        _like('bias', bias, (channels,), torch.float32, device)
+
+
+def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state=None, return_final_state=False):
+    """``y[b,t,d] = act(bias[d] + sum_k weight[d,k] x[b, t - taps + 1 + k, d])`` over ``x [batch, time, channels]``; ``weight [channels, taps]``
+    (2 to 8 taps) and ``bias [channels]`` in float32; ``activation`` None or 'silu'.
+
+    ``initial_state [batch, taps - 1, channels]`` (x's type) holds the rows in front of the window, zeros when None; ``starts [batch, time]`` (bool /
+    uint8) marks first rows of episodes, in front of which every tap is zero.  Returns y, or ``(y, final_state)``: the last ``taps - 1`` rows of the
+    episode that is running at the window's end, i.e. the next window's ``initial_state`` and ``short_conv_step``'s state.  Differentiable in
+    x, weight, bias and initial_state; the parameters' gradients are summed in a fixed order."""
+    _leading('x', x)
+    _need(x.dim() == 3, 'x must be [batch, time, channels], got', list(x.shape))
+    b, t, d = x.shape
+    _need(d > 0, 'x must have channels')
+    silu = _activation(activation)
+    _conv_parameters(d, weight, bias, x.device)
+    if initial_state is not None:
+        _like('initial_state', initial_state, (b, weight.shape[1] - 1, d), x.dtype, x.device)
+    starts = _flags('starts', starts, (b, t), x.device)
+    if _wants_grad(x, weight, bias, initial_state):
+        y, final = _ShortConv.apply(x, weight, bias, initial_state, starts, silu, bool(return_final_state))
+    else:
+        y, final = _conv_forward(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(),
+                                 None if initial_state is None else initial_state.contiguous(), starts, silu, return_final_state)
+    return (y, final) if return_final_state else y
+
+
+def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, starts=None):
+    """One row of each of ``x``'s environments: ``x [rows, channels]``, ``state [environments, taps - 1, channels]`` (x's type, contiguous) moved on in
+    place, parameters as for ``short_conv``.  ``env_ids [rows]`` says whose rows they are (``BatchedRunEnv.recv``'s ids; row i is environment i when
+    None); a negative id is padding: y = 0 and no state is touched.  An id out of range, or one that an earlier row has, gives NaN and touches no
+    state.  ``starts [rows]`` empties the window first.  Returns y [rows, channels]."""
+    kind = _leading('x', x)
+    _need(x.dim() == 2 and x.shape[1] > 0, 'x must be [rows, channels], got', list(x.shape))
+    n, d = x.shape
+    silu = _activation(activation)
+    _conv_parameters(d, weight, bias, x.device)
+    if not torch.is_tensor(state):
+        raise TypeError('state must be a torch tensor, got %s' % type(state).__name__)
+    _need(state.dim() == 3, 'state must be [environments, taps - 1, channels], got', list(state.shape))
+    _like('state', state, (state.shape[0], weight.shape[1] - 1, d), x.dtype, x.device)
+    _need(state.is_contiguous(), 'state must be contiguous')
+    if _wants_grad(x, state, weight, bias):
+        raise ValueError('short_conv_step has no gradient: call it under torch.no_grad(), or short_conv on the window')
+    starts = _flags('starts', starts, (n,), x.device)
+    env_ids = _step_ids(env_ids, n, state.shape[0], x.device)
+    x, weight = _rows(x), weight.contiguous()
+    bias, starts = (None if v is None else v.contiguous() for v in (bias, starts))
+    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, kind, silu, n, state.shape[0], d, weight.shape[1], x.data_ptr(), x.stride(0),
+                                                 weight.data_ptr(), _ptr(bias), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), x.device)
+    return y
+
+
+# ---- selective scan ------------------------------------------------------------------------------------------------------------------
+
+def _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, soft, y=None, final=None, marks=None, dy=None, dfinal=None, dx=None, ddt=None, dz=None,
+               dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dinitial=None, workspace=None):
+    b, t, d = x.shape
+    return _SCAN.pack(_SCAN.size, _TYPES[x.dtype], soft, b, t, d, B.shape[2], A.shape[1], *_at(x), *_at(dt), A.data_ptr(),
+                      B.data_ptr(), B.stride(0), B.stride(1), B.stride(2), C.data_ptr(), C.stride(0), C.stride(1), C.stride(2), _ptr(D), _ptr(dt_bias),
+                      *_at(z), *_at(starts), _ptr(initial), *_at(y), _ptr(final), _ptr(marks), *_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz),
+                      _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dinitial), _ptr(workspace), 0 if workspace is None else workspace.numel())
+
+
+def _scan_forward(inputs, want_final, train):
+    x, A = inputs[0], inputs[2]
+    lib = _load()
+    y = _window_like(x)
+    final = torch.empty((x.shape[0],) + tuple(A.shape), dtype=torch.float32, device=x.device) if want_final else None
+    probe = _scan_args(*inputs)
+    marks = None
+    if train:
+        marks = torch.empty((lib.ppn_scan_checkpoint_bytes(probe) // 4,), dtype=torch.float32, device=x.device)
+    work = _workspace(lib.ppn_scan_forward_workspace(probe), x.device)
+    _call(lib.ppn_scan_forward, _scan_args(*inputs, y=y, final=final, marks=marks, workspace=work), x.device)
+    return y, final, marks
+
+
+def _scan_layout(x, dt, A, B, C, D, z, dt_bias, initial):
+    dense = lambda v: None if v is None else v.contiguous()      # noqa: E731
+    return _rows(x), _rows(dt), A.contiguous(), _rows(B), _rows(C), dense(D), None if z is None else _rows(z), dense(dt_bias), dense(initial)
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, initial, starts, soft, want_final):
+        ctx.set_materialize_grads(False)
+        x, dt, A, B, C, D, z, dt_bias, initial = _scan_layout(x, dt, A, B, C, D, z, dt_bias, initial)
+        y, final, marks = _scan_forward((x, dt, A, B, C, D, z, dt_bias, starts, initial, soft), want_final, True)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, initial, starts, marks)
+        ctx.soft = soft
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, dt, A, B, C, D, z, dt_bias, initial, starts, marks = ctx.saved_tensors
+        if dy is None and dfinal is None:
+            return (None,) * 12
+        empty = lambda v: None if v is None else torch.empty_like(v)      # noqa: E731
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dx, ddt, dz = _window_like(x), _window_like(dt), None if z is None else _window_like(z)
+        dA, dD, dbias, dinitial = empty(A), empty(D), empty(dt_bias), empty(initial)
+        dB, dC = (torch.empty(v.shape, dtype=v.dtype, device=v.device) for v in (B, C))
+        if x.shape[0] == 0 or x.shape[1] == 0:          # no rows: the state passes through
+            for v in (dA, dD, dbias):
+                if v is not None:
+                    v.zero_()
+            if dinitial is not None:
+                dinitial.zero_() if dfinal is None else dinitial.copy_(dfinal)
+            return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
+        dy = torch.zeros_like(x) if dy is None else _rows(dy)
+        inputs = (x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft)
+        given = dict(marks=marks, dy=dy, dfinal=dfinal, dx=dx, ddt=ddt, dz=dz, dB=dB, dC=dC, dA=dA, dD=dD, ddt_bias=dbias, dinitial=dinitial)
+        lib = _load()
+        work = _workspace(lib.ppn_scan_backward_workspace(_scan_args(*inputs)), x.device)
+        _call(lib.ppn_scan_backward, _scan_args(*inputs, workspace=work, **given), x.device)
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
+
+
+def _scan_parameters(channels, A, D, dt_bias, device):
+    _need(torch.is_tensor(A) and A.dim() == 2 and 1 <= A.shape[1] <= 64, 'A must be a tensor [channels, states] with 1 to 64 states')
+    _like('A', A, (channels, A.shape[1]), torch.float32, device)
+    for name, v in (('D', D), ('dt_bias', dt_bias)):
+        if v is not None:
+            _like(name, v, (channels,), torch.float32, device)
+
+
+def _groups_of(channels, B, dims):
+    _need(torch.is_tensor(B) and B.dim() == dims, 'B must be a tensor of', dims, 'dimensions: [..., groups, states]')
+    groups = B.shape[-2]
+    _need(groups >= 1 and channels % groups == 0, channels, 'channels cannot be shared among', groups, 'groups of B and C')
+    return groups
+
+
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, starts=None, initial_state=None, return_final_state=False):
+    """Selective state space scan over ``x, dt, z [batch, time, channels]`` and ``B, C [batch, time, groups, states]`` (channel d uses group
+    ``d // (channels // groups)``) of one type, with ``A [channels, states]``, ``D, dt_bias [channels]`` in float32, 1 to 64 states:
+
+        delta = dt + dt_bias, then log(1 + e^delta) if dt_softplus
+        h[t,d,n] = exp(delta A[d,n]) h[t-1,d,n] + delta B[t,g,n] x[t,d]
+        y[t,d] = (sum_n C[t,g,n] h[t,d,n] + D[d] x[t,d]) * silu(z[t,d])           (the last factor only with z)
+
+    ``initial_state [batch, channels, states]`` float32, zeros when None; h is zero in front of a row marked in ``starts [batch, time]``.  Returns y, or
+    ``(y, final_state)``, the next window's ``initial_state`` and ``selective_scan_step``'s state.  Differentiable in every tensor but ``starts``; sums
+    run in a fixed order, so gradients repeat bit for bit.  A differentiable call keeps the states in front of every 8th row for the backward pass."""
+    _leading('x', x)
+    _need(x.dim() == 3, 'x must be [batch, time, channels], got', list(x.shape))
+    b, t, d = x.shape
+    _need(d > 0, 'x must have channels')
+    _like('dt', dt, (b, t, d), x.dtype, x.device)
+    if z is not None:
+        _like('z', z, (b, t, d), x.dtype, x.device)
+    _scan_parameters(d, A, D, dt_bias, x.device)
+    groups = _groups_of(d, B, 4)
+    for name, v in (('B', B), ('C', C)):
+        _like(name, v, (b, t, groups, A.shape[1]), x.dtype, x.device)
+    if initial_state is not None:
+        _like('initial_state', initial_state, (b, d, A.shape[1]), torch.float32, x.device)
+    starts = _flags('starts', starts, (b, t), x.device)
+    soft = 1 if dt_softplus else 0
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
+        y, final = _SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, initial_state, starts, soft, bool(return_final_state))
+    else:
+        x, dt, A, B, C, D, z, dt_bias, initial_state = _scan_layout(x, dt, A, B, C, D, z, dt_bias, initial_state)
+        y, final, _ = _scan_forward((x, dt, A, B, C, D, z, dt_bias, starts, initial_state, soft), return_final_state, False)
+    return (y, final) if return_final_state else y
+
+
+def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False, env_ids=None, starts=None):
+    """One row of each of ``x``'s environments: ``x, dt, z [rows, channels]``, ``B, C [rows, groups, states]``, ``state [environments, channels, states]``
+    (float32, contiguous) moved on in place; ``env_ids`` and ``starts`` as in ``short_conv_step``.  Returns y [rows, channels]."""
+    kind = _leading('x', x)
+    _need(x.dim() == 2 and x.shape[1] > 0, 'x must be [rows, channels], got', list(x.shape))
+    n, d = x.shape
+    _like('dt', dt, (n, d), x.dtype, x.device)
+    if z is not None:
+        _like('z', z, (n, d), x.dtype, x.device)
+    _scan_parameters(d, A, D, dt_bias, x.device)
+    states, groups = A.shape[1], _groups_of(d, B, 3)
+    for name, v in (('B', B), ('C', C)):
+        _like(name, v, (n, groups, states), x.dtype, x.device)
+    if not torch.is_tensor(state):
+        raise TypeError('state must be a torch tensor, got %s' % type(state).__name__)
+    _need(state.dim() == 3, 'state must be [environments, channels, states], got', list(state.shape))
+    _like('state', state, (state.shape[0], d, states), torch.float32, x.device)
+    _need(state.is_contiguous(), 'state must be contiguous')
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
+        raise ValueError('selective_scan_step has no gradient: call it under torch.no_grad(), or selective_scan on the window')
+    starts = _flags('starts', starts, (n,), x.device)
+    env_ids = _step_ids(env_ids, n, state.shape[0], x.device)
+    starts = None if starts is None else starts.contiguous()
+    x, dt, A, B, C, D, z, dt_bias, _ = _scan_layout(x, dt, A, B, C, D, z, dt_bias, None)
+    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    _call(_load().ppn_scan_step,
+          _SCAN_STEP.pack(_SCAN_STEP.size, kind, 1 if dt_softplus else 0, n, state.shape[0], d, groups, states, x.data_ptr(), x.stride(0), dt.data_ptr(),
+                          dt.stride(0), A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1), _ptr(D), _ptr(dt_bias),
+                          _ptr(z), 0 if z is None else z.stride(0), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), x.device)
+    return y
+
+
+# ---- cross entropy over a catalogue of actions -----------------------------------------------------------------------------------------
+
+def _loss_args(hidden, weight, target, allowed, ignore, loss=None, lse=None, dloss=None, dhidden=None, dweight=None, workspace=None):
+    return _LOSS.pack(_LOSS.size, _TYPES[hidden.dtype], hidden.shape[0], weight.shape[0], hidden.shape[1], ignore, hidden.data_ptr(), hidden.stride(0),
+                      weight.data_ptr(), weight.stride(0), target.data_ptr(), _ptr(allowed), 0 if allowed is None else allowed.stride(0), _ptr(loss),
+                      _ptr(lse), _ptr(dloss), _ptr(dhidden), _ptr(dweight), _ptr(workspace), 0 if workspace is None else workspace.numel())
+
+
+def _loss_forward(hidden, weight, target, allowed, ignore):
+    n = hidden.shape[0]
+    loss, lse = (torch.empty((n,), dtype=torch.float32, device=hidden.device) for _ in range(2))
+    lib = _load()
+    work = _workspace(lib.ppn_loss_forward_workspace(_loss_args(hidden, weight, target, allowed, ignore)), hidden.device)
+    _call(lib.ppn_loss_forward, _loss_args(hidden, weight, target, allowed, ignore, loss, lse, workspace=work), hidden.device)
+    return loss, lse
+
+
+class _ActionCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, allowed, ignore):
+        hidden, weight = _rows(hidden), _rows(weight)
+        loss, lse = _loss_forward(hidden, weight, target, allowed, ignore)
+        ctx.save_for_backward(hidden, weight, target, allowed, lse)
+        ctx.ignore = ignore
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        hidden, weight, target, allowed, lse = ctx.saved_tensors
+        dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if ctx.needs_input_grad[0] else None
+        dweight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
+        if hidden.shape[0] == 0:
+            return dhidden, None if dweight is None else dweight.zero_(), None, None, None
+        given = (hidden, weight, target, allowed, ctx.ignore)
+        lib = _load()
+        work = _workspace(lib.ppn_loss_backward_workspace(_loss_args(*given)), hidden.device)
+        _call(lib.ppn_loss_backward, _loss_args(*given, lse=lse, dloss=dloss.contiguous(), dhidden=dhidden, dweight=dweight, workspace=work), hidden.device)
+        return dhidden, dweight, None, None, None
+
+
+def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100):
+    """Cross entropy of every row over a catalogue of actions, ``[rows]`` in float32, without keeping the logits:
+
+        loss[i] = log sum_v exp(hidden[i] . weight[v]) - hidden[i] . weight[target[i]]          over the actions v that ``allowed`` has in row i
+
+    ``hidden [rows, features]`` and ``weight [actions, features]`` of one type, ``target [rows]`` int64.  ``allowed [rows, ceil(actions / 32)]``
+    int32 has one bit per action (``pack_allowed``), all actions when None.  A row whose target is ``ignore_index``, or that allows nothing, has loss 0
+    and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
+    NaN.  ``-loss`` is the log-probability of the action ``target``.  Differentiable in hidden and weight; sums run in a fixed order."""
+    _leading('hidden', hidden)
+    _need(hidden.dim() == 2 and hidden.shape[1] > 0, 'hidden must be [rows, features], got', list(hidden.shape))
+    n, f = hidden.shape
+    _need(torch.is_tensor(weight) and weight.dim() == 2 and weight.shape[0] > 0, 'weight must be a tensor [actions, features]')
+    v = weight.shape[0]
+    _like('weight', weight, (v, f), hidden.dtype, hidden.device)
+    _like('target', target, (n,), torch.int64, hidden.device)
+    if allowed is not None:
+        _like('allowed', allowed, (n, (v + 31) // 32), torch.int32, hidden.device)
+        allowed = _rows(allowed)
+    target = target.contiguous()
+    ignore_index = int(ignore_index)
+    if _wants_grad(hidden, weight):
+        return _ActionCrossEntropy.apply(hidden, weight, target, allowed, ignore_index)
+    return _loss_forward(_rows(hidden), _rows(weight), target, allowed, ignore_index)[0]
+
+
+def pack_allowed(mask):
+    """``mask [rows, actions]`` (bool) as the bits ``action_cross_entropy`` takes: int32 ``[rows, ceil(actions / 32)]``, action v in bit v % 32 of word v // 32."""
+    _need(torch.is_tensor(mask) and mask.dim() == 2, 'mask must be a tensor [rows, actions]')
+    n, v = mask.shape
+    words = (v + 31) // 32
+    bits = torch.nn.functional.pad(mask != 0, (0, words * 32 - v)).view(n, words, 4, 8)
+    place = torch.tensor([1 << i for i in range(8)], dtype=torch.uint8, device=mask.device)
+    octets = (bits * place).sum(-1, dtype=torch.int32).to(torch.uint8)           # little-endian octets of a 32-bit word
+    return octets.view(n, words * 4).contiguous().view(torch.int32) if words else octets.view(n, 0).to(torch.int32)

@@ -19,6 +19,7 @@ are not merged yet) in which an EXEC-dependent vector instruction -- anything wi
 spill pseudos and the whole-wave-mode spills (expanded with EXEC = -1 around them: prologue by design), and any COPY into a vector register -- stands in front of the block's `$exec = S_OR_B64 $exec, ...` (or, for an else-block, its `S_OR_SAVEEXEC_B64`).
 
     python tools/dev/mir_lint_exec_restore.py file.mir [...]      # exit status 1 if anything is reported
+    python tools/dev/mir_lint_exec_restore.py --policy [--keep] [flags]  # the same of the policy operators' three units
     python tools/dev/mir_lint_exec_restore.py --build [--keep] [flags]   # emits the MIR of the seven translation units first (80 s on 8 cores;
                                                                          # the files -- half a gigabyte -- are removed again unless --keep)
 """
@@ -66,17 +67,24 @@ def lint(path):
     return reports, n_restores
 
 
-def build_mir(extra_flags):
+def build_mir(extra_flags, policy=False):
     tag = 'mir' + ''.join(re.sub(r'\W+', '_', f) for f in extra_flags)
     out = os.path.join(ROOT, 'build', tag)
     os.makedirs(out, exist_ok=True)
     src = os.path.join(ROOT, 'pypownet_amd', 'csrc')
     common = [os.environ.get('HIPCC', '/opt/rocm/bin/hipcc'), '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '--cuda-device-only', '-S',
               '-mllvm', '-stop-after=' + STOP_AFTER] + list(extra_flags)
+    if policy:      # the policy operators, with the flags the product build gives them
+        return emit([(os.path.join(out, u + '.mir'), common + ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', os.path.join(src, u + '.hip')])
+                     for u in ('ppn_conv', 'ppn_scan', 'ppn_loss')])
     jobs = [(os.path.join(out, 'engine.mir'), common + ['-DPPN_SPLIT_BUILD', os.path.join(src, 'ppn_engine.hip')])]
     for w in (1, 2, 4):
         for nt in (0, 1):
             jobs.append((os.path.join(out, 'k_w%dn%d.mir' % (w, nt)), common + ['-DPPN_TU_W=%d' % w, '-DPPN_TU_NT=%d' % nt, os.path.join(src, 'ppn_kernel_tu.hip')]))
+    return emit(jobs)
+
+
+def emit(jobs):
     procs = [(o, subprocess.Popen(c + ['-o', o], stderr=subprocess.DEVNULL)) for o, c in jobs]
     for o, p in procs:
         if p.wait() != 0:
@@ -85,9 +93,9 @@ def build_mir(extra_flags):
 
 
 def main(argv):
-    built = argv[:1] == ['--build']
+    built = argv[:1] in (['--build'], ['--policy'])
     keep = '--keep' in argv
-    files = build_mir([a for a in argv[1:] if a != '--keep']) if built else argv
+    files = build_mir([a for a in argv[1:] if a != '--keep'], argv[0] == '--policy') if built else argv
     if not files:
         raise SystemExit(__doc__)
     total = seen = 0
