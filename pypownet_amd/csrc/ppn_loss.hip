@@ -43,76 +43,93 @@ struct Operands {
   int64_t K;                      // padded
 };
 
-struct StatsArgs { const int32_t* allowed; int64_t allowed_row; const int64_t* target; float2* partial; float* wanted; int64_t columns; };
+struct StatsArgs { const int32_t* allowed; int64_t allowed_row; float2* partial; int64_t columns; };
 struct GradArgs {
   const int32_t* allowed; int64_t allowed_row; const int64_t* target; const float* lse; const float* dloss; const float* scale;
   void* dl; int64_t dl_row; void* dlt; int64_t dlt_row; int64_t first, rows_padded, cols_padded;
 };
-struct SumArgs { float* sums; int64_t slots; bool add; };
+struct SumArgs { float* sums; bool add; };
 
 constexpr int LINE = 64;          // bytes of the inner dimension per step
 
-// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go through LDS, two buffers, read from memory
-// one step ahead into registers.  A line's four 16-byte parts are stored with part ^ (row / 2 % 4), so that the 16 rows a fragment read
-// touches fall into different banks.
+// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go from memory straight into LDS, into one of three
+// buffers two steps ahead of the step that is multiplied; one barrier a step.  A line's four 16-byte parts are stored with
+// part ^ (row / 2 % 4), so that the 16 rows a fragment read touches fall into different banks; the transfer writes 64 lanes' 16 bytes in
+// a row (16 lines), so the exchange is made in the addresses it reads.
 template <typename T, int MI, int NI, int WM, int WN> struct Product {
   static constexpr int BM = 16 * MI * WM, BN = 16 * NI * WN, THREADS = 64 * WM * WN;
-  static constexpr int LOADS = (BM + BN) * 4 / THREADS;
-  static constexpr int LDS_BYTES = 2 * (BM + BN) * LINE;
-  static_assert((BM + BN) * 4 % THREADS == 0, "");
+  static constexpr int GROUPS = (BM + BN) / 16, LOADS = GROUPS / (WM * WN);      // transfers of 16 lines: in all, and per wave
+  static constexpr int STAGE = (BM + BN) * LINE, LDS_BYTES = 3 * STAGE;
+  static_assert(GROUPS % (WM * WN) == 0 && BM % 16 == 0, "");
 
   f32x4 c[MI][NI];
   int wave_m, wave_n, lane;
 
   __device__ static int spot(int row, int part) { return row * LINE + ((part ^ ((row >> 1) & 3)) << 4); }
 
+  // 16 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().
+  __device__ static void transfer(unsigned to, const char* base, unsigned offset) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+  }
+
+  // The same for all lanes of the wave, and in scalar registers.
+  __device__ static const char* scalar(const char* p) {
+    const uint64_t v = (uint64_t)p;
+    return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+  }
+
   __device__ void run(const Operands& o, char* lds, int64_t m0, int64_t n0, int64_t k0, int64_t k1) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     lane = tid & 63;
-    const int wave = tid >> 6;
     wave_m = wave / WN * (16 * MI), wave_n = wave % WN * (16 * NI);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) c[i][j] = f32x4{0, 0, 0, 0};
-    const char* from[LOADS];
-    int to[LOADS];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const char* base[LOADS];
+    unsigned offset[LOADS], to[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int e = tid + i * THREADS, row = e >> 2, part = e & 3;
-      to[i] = spot(row, part);
-      if (row < BM) {
-        int64_t m = m0 + row < o.M ? m0 + row : o.M - 1;
-        from[i] = (const char*)o.A + (m * o.lda + k0) * (int64_t)sizeof(T) + part * 16;
-      } else {
-        int64_t n = n0 + row - BM < o.N ? n0 + row - BM : o.N - 1;
-        from[i] = (const char*)o.B + (n * o.ldb + k0) * (int64_t)sizeof(T) + part * 16;
-      }
+      const int group = wave * LOADS + i, row = lane >> 2, part = (lane & 3) ^ ((row >> 1) & 3);
+      const bool left = group * 16 < BM;
+      const int64_t first = left ? m0 + group * 16 : n0 + group * 16 - BM, rows = left ? o.M : o.N, ld = (left ? o.lda : o.ldb) * (int64_t)sizeof(T);
+      const int64_t top = first < rows ? first : rows - 1, spare = rows - 1 - top;             // lines past the last one read the last one again
+      base[i] = scalar((const char*)(left ? o.A : o.B) + top * ld + k0 * (int64_t)sizeof(T));
+      offset[i] = (unsigned)((row < spare ? row : spare) * ld) + part * 16;
+      to[i] = lds0 + group * 16 * LINE;
     }
     const int steps = (int)((k1 - k0) * (int64_t)sizeof(T) / LINE);
-    u32x4 held[LOADS];
+    int filled = 0;                                                    // buffer the next transfers go to
+    auto fetch = [&]() {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4*)from[i];
-    for (int s = 0; s < steps; ++s) {
-      char* buf = lds + (s & 1) * (BM + BN) * LINE;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) *(u32x4*)(buf + to[i]) = held[i];
-      if (s + 1 < steps) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4*)(from[i] + (int64_t)(s + 1) * LINE);
+      for (int i = 0; i < LOADS; ++i) {
+        transfer(to[i] + filled * STAGE, base[i], offset[i]);
+        base[i] += LINE;
       }
-      __syncthreads();
+      filled = filled == 2 ? 0 : filled + 1;
+    };
+    fetch();
+    if (steps > 1) fetch();
+    int turn = 0;
+    for (int s = 0; s < steps; ++s) {
+      // This step's lines are in (the next step's LOADS transfers may be under way), for every wave once all have passed the barrier; and
+      // every wave is done reading the buffer of the step before, which the transfers below fill.
+      if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 2 < steps) fetch();
+      const char* buf = lds + turn * STAGE;
+      turn = turn == 2 ? 0 : turn + 1;
       u32x4 a[MI], b[NI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = *(const u32x4*)(buf + spot(wave_m + i * 16 + (lane & 15), lane >> 4));
-#pragma unroll
       for (int j = 0; j < NI; ++j) b[j] = *(const u32x4*)(buf + spot(BM + wave_n + j * 16 + (lane & 15), lane >> 4));
+#pragma unroll
+      for (int i = 0; i < MI; ++i) a[i] = *(const u32x4*)(buf + spot(wave_m + i * 16 + (lane & 15), lane >> 4));
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) multiply(c[i][j], a[i], b[j], T());
     }
-    // (the buffer written two steps on is the one read now: the barrier between them is the next step's)
   }
   // Sum (i, j, r) of this lane: row wave_m + 16 i + 4 (lane / 16) + r, column wave_n + 16 j + lane % 16 of the tile.
   __device__ int row_of(int i, int r) const { return wave_m + i * 16 + (lane >> 4) * 4 + r; }
@@ -121,12 +138,10 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
 
 // Tiles are handed to the eight dies in turn, each with its own L2: neighbours in the list below go to one die, all row tiles of a
 // column tile one after the other, so that a die reads its share of the larger operand once.
-__device__ inline int64_t tile_of(int64_t id, int64_t count) {
-  const int64_t per = count / 8, whole = per * 8;
+__device__ inline unsigned tile_of(unsigned id, unsigned count) {
+  const unsigned per = count / 8, whole = per * 8;
   return id < whole ? (id % 8) * per + id / 8 : id;
 }
-
-__device__ inline bool is_allowed(const int32_t* allowed, int64_t at, int64_t col) { return !allowed || ((allowed[at + (col >> 5)] >> (col & 31)) & 1); }
 
 template <int PATTERN> __device__ inline float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
@@ -138,51 +153,74 @@ template <typename F> __device__ inline float over_16(float v, F f) {      // ov
   return f(v, dpp<0xb1>(v));    // quad_perm 1,0,3,2
 }
 
-// Forward: of every row and every 16 NI columns the maximum and the sum of exp(l - maximum); the target's logit as it goes by.
+// The bits of BN columns from n0 (of N, whose word 0 is `word` words into a row of allowed) that row `row` may count: nothing past the last
+// column.  Called before the product, so that the loads' way is covered by it; read after it.
+template <int BN> __device__ inline void stage_mask(unsigned (*mask)[BN / 32], int at, const int32_t* allowed, int64_t allowed_row, int64_t row, int64_t word, int64_t n0, int64_t N,
+                                                    bool live) {
+#pragma unroll
+  for (int w = 0; w < BN / 32; ++w) {
+    const int64_t left = N - n0 - 32 * w;
+    unsigned bits = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
+    if (!live) bits = 0;
+    if (allowed && bits) bits &= (unsigned)allowed[row * allowed_row + word + n0 / 32 + w];
+    mask[at][w] = bits;
+  }
+}
+
+// Forward: of every row and every 16 NI columns the maximum and the sum of exp(l - maximum).
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) loss_stats(Operands o, StatsArgs s, int64_t tiles_m, int64_t tiles_n) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsArgs s, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
   __shared__ __align__(16) char lds[P::LDS_BYTES];
-  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), m0 = tile % tiles_m * P::BM, n0 = tile / tiles_m * P::BN;
+  __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
+  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
+  const int64_t m0 = (int64_t)(tile % tiles_m) * P::BM, n0 = (int64_t)(tile / tiles_m) * P::BN;
+  for (int r = threadIdx.x; r < P::BM; r += P::THREADS)
+    stage_mask<P::BN>(mask, r, s.allowed, s.allowed_row, m0 + r < o.M ? m0 + r : o.M - 1, 0, n0, o.N, true);
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
+  const unsigned bit = 1u << (p.lane & 15);
+  float2* out = s.partial + m0 * s.columns + (n0 + p.wave_n) / (16 * NI);
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t row = m0 + p.row_of(i, r);
-      const bool in = row < o.M;
-      const int64_t at = (in ? row : o.M - 1) * s.allowed_row, target = s.target[in ? row : o.M - 1];
-      float top = -INFINITY, sum = 0.0f;
-      bool live[NI];
+      const int row = p.row_of(i, r);
+      float l[NI], top = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int64_t col = n0 + p.col_of(j);
-        live[j] = col < o.N && is_allowed(s.allowed, at, col);
-        const float l = p.c[i][j][r];
-        if (live[j] && in && col == target) s.wanted[row] = l;
-        top = live[j] ? (l != l ? l : (top > l ? top : l)) : top;      // (a NaN stays the maximum, and the sum becomes NaN with it)
+        const unsigned word = mask[row][p.wave_n / 32 + j / 2];
+        l[j] = word & (j & 1 ? bit << 16 : bit) ? p.c[i][j][r] : -INFINITY;
+        top = fmaxf(top, l[j]);      // (drops a NaN; the sum below does not)
       }
-      top = over_16(top, [](float a, float b) { return a != a ? a : b != b ? b : a > b ? a : b; });
-      const float ref = top == -INFINITY ? 0.0f : top;
+      top = over_16(top, [](float a, float b) { return fmaxf(a, b); });
+      const float ref = top == -INFINITY ? 0.0f : top * LOG2E;
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sum += live[j] ? exp_fast(p.c[i][j][r] - ref) : 0.0f;
+      for (int j = 0; j < NI; ++j) sum += __builtin_amdgcn_exp2f(l[j] * LOG2E - ref);
       sum = over_16(sum, [](float a, float b) { return a + b; });
-      if (in && (p.lane & 15) == 0) s.partial[row * s.columns + (n0 + p.wave_n) / (16 * NI)] = make_float2(top, sum);
+      if ((p.lane & 15) == 0 && m0 + row < o.M) out[(unsigned)(row * (unsigned)s.columns)] = make_float2(top, sum);
     }
 }
 
-// One wave a row: joins the tiles' maxima and sums.
-__global__ void __launch_bounds__(256) loss_join(const float2* partial, int64_t columns, const float* wanted, const int64_t* target, const int32_t* allowed,
-                                                 int64_t allowed_row, int64_t rows, int64_t actions, int64_t ignore, float* loss, float* lse) {
+// One wave a row: joins the tiles' maxima and sums, and takes the target's logit as a product of its own.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* partial, int64_t columns) {
   const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int lane = threadIdx.x & 63;
-  if (row >= rows) return;
+  if (row >= a.rows) return;
+  const int64_t at = a.target[row];
+  const bool inside = at >= 0 && at < a.actions;
+  float wanted = 0.0f;
+  if (inside) {
+    const T* h = (const T*)a.hidden + row * a.hidden_row;
+    const T* w = (const T*)a.weight + at * a.weight_row;
+    for (int64_t f = lane; f < a.features; f += 64) wanted += to_float(h[f]) * to_float(w[f]);
+  }
   float top = -INFINITY, sum = 0.0f;
+  // (a tile without an allowed action has the sum 0 and the maximum -infinity; one with a NaN has the sum NaN whatever its maximum)
   auto join = [&](float t, float s) {
-    if (t == -INFINITY) return;
-    const float high = t != t || top != top ? NAN : t > top ? t : top;
-    sum = (top == -INFINITY ? 0.0f : sum * exp_fast(top - high)) + s * exp_fast(t - high);
+    const float high = fmaxf(top, t), ref = high == -INFINITY ? 0.0f : high;
+    sum = sum * exp_fast(top - ref) + s * exp_fast(t - ref);
     top = high;
   };
   for (int64_t c = lane; c < columns; c += 64) {
@@ -190,21 +228,21 @@ __global__ void __launch_bounds__(256) loss_join(const float2* partial, int64_t 
     join(v.x, v.y);
   }
   for (int d = 32; d; d >>= 1) {
+    wanted += __shfl_xor(wanted, d);
     const float t = __shfl_xor(top, d), s = __shfl_xor(sum, d);
     join(t, s);
   }
   if (lane) return;
-  const int64_t at = target[row];
-  const bool nothing = top == -INFINITY, inside = at >= 0 && at < actions;
+  const bool nothing = top == -INFINITY && sum == 0.0f;
   const float whole = top + 0.693147180559945309f * __builtin_amdgcn_logf(sum);
-  if (at == ignore || nothing) {
-    loss[row] = 0.0f, lse[row] = INFINITY;
-  } else if (!inside) {
-    loss[row] = NAN, lse[row] = NAN;
-  } else {
-    loss[row] = is_allowed(allowed, row * allowed_row, at) ? whole - wanted[row] : INFINITY;
-    lse[row] = whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
+  float loss = 0.0f, lse = INFINITY;
+  if (at != a.ignore_index && !nothing) {
+    const bool legal = inside && (!a.allowed || ((a.allowed[row * a.allowed_row + (at >> 5)] >> (at & 31)) & 1));
+    loss = !inside ? NAN : legal ? whole - wanted : INFINITY;
+    lse = !inside || whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
   }
+  a.loss[row] = loss;
+  a.lse[row] = lse;
 }
 
 // scale[0] = the power of two dl is multiplied by, scale[1] = 1 / it.
@@ -230,69 +268,83 @@ __global__ void __launch_bounds__(256) loss_scale(const float* dloss, const floa
 
 // Backward, first product: dl of the columns first .. first + N of the catalogue, [rows x cols_padded] and [N x rows_padded], zeros in the padding.
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) loss_grad(Operands o, GradArgs g, int64_t tiles_m, int64_t tiles_n) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArgs g, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
+  struct Row { float lse2, up; int target, unused; };
   __shared__ __align__(16) char lds[P::LDS_BYTES];
-  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), m0 = tile % tiles_m * P::BM, n0 = tile / tiles_m * P::BN;
+  __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
+  __shared__ __align__(16) Row rows[P::BM];
+  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
+  const int64_t m0 = (int64_t)(tile % tiles_m) * P::BM, n0 = (int64_t)(tile / tiles_m) * P::BN;
+  for (int r = threadIdx.x; r < P::BM; r += P::THREADS) {
+    const int64_t row = m0 + r < o.M ? m0 + r : o.M - 1, target = g.target[row] - g.first - n0;
+    const float lse = g.lse[row];
+    const bool live = m0 + r < o.M && lse != INFINITY;                   // a row without a gradient, or past the last one: zeros
+    stage_mask<P::BN>(mask, r, g.allowed, g.allowed_row, row, g.first / 32, n0, o.N, live);
+    rows[r] = Row{lse * LOG2E, live ? g.dloss[row] * g.scale[0] : 0.0f, target >= 0 && target < P::BN ? (int)target : -1, 0};
+  }
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
-  const float scale = g.scale[0];
+  const unsigned bit = 1u << (p.lane & 15);
+  const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
+  T* dl = (T*)g.dl + m0 * g.dl_row + n0;
+  T* dlt = (T*)g.dlt + n0 * g.dlt_row + m0;
+  const unsigned dl_row = (unsigned)g.dl_row, dlt_row = (unsigned)g.dlt_row;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     T out[NI][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t row = m0 + p.row_of(i, r), safe = row < o.M ? row : o.M - 1;
-      const float lse = row < o.M ? g.lse[safe] : INFINITY, up = lse == INFINITY ? 0.0f : g.dloss[safe] * scale;
-      const int64_t target = lse == INFINITY ? -1 : g.target[safe] - g.first;
+      const int row = p.row_of(i, r);
+      const Row q = rows[row];
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int64_t col = n0 + p.col_of(j);
-        float v = 0.0f;
-        if (lse != INFINITY && col < o.N) {
-          const bool live = is_allowed(g.allowed, safe * g.allowed_row, col + g.first);
-          v = live ? (exp_fast(p.c[i][j][r] - lse) - (col == target ? 1.0f : 0.0f)) * up : lse != lse ? lse : 0.0f;
-        }
-        out[j][r] = (T)v;
-        if (row < o.M && col < g.cols_padded) ((T*)g.dl)[row * g.dl_row + col] = out[j][r];
+        const unsigned word = mask[row][p.wave_n / 32 + j / 2];
+        const float e = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2);
+        const float v = (e - (p.col_of(j) == q.target ? 1.0f : 0.0f)) * q.up;
+        out[j][r] = (T)(word & (j & 1 ? bit << 16 : bit) ? v : 0.0f);
+        if (whole || (m0 + row < o.M && n0 + p.col_of(j) < g.cols_padded)) dl[row * dl_row + p.col_of(j)] = out[j][r];
       }
     }
-    const int64_t row = m0 + p.row_of(i, 0);
+    const int row = p.row_of(i, 0);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int64_t col = n0 + p.col_of(j);
-      if (col < o.N && row < g.rows_padded) {      // rows_padded is a multiple of 16: the four rows are in or out together
+    for (int j = 0; j < NI; ++j)
+      if (whole || (n0 + p.col_of(j) < o.N && m0 + row < g.rows_padded)) {      // rows_padded is a multiple of 16: the four rows are in or out together
         struct alignas(4 * sizeof(T)) Four { T v[4]; } f = {{out[j][0], out[j][1], out[j][2], out[j][3]}};
-        *(Four*)((T*)g.dlt + col * g.dlt_row + row) = f;
+        *(Four*)(dlt + p.col_of(j) * dlt_row + row) = f;
       }
-    }
   }
 }
 
 // Backward, second products: 32-bit sums of one share of the inner dimension (grid.y shares, a slot of [M x N] floats each).
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) loss_sums(Operands o, SumArgs s, int64_t share, int64_t tiles_m, int64_t tiles_n) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(Operands o, SumArgs s, int64_t share, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
   __shared__ __align__(16) char lds[P::LDS_BYTES];
-  const int64_t tile = tile_of(blockIdx.x, tiles_m * tiles_n), n0 = tile % tiles_n * P::BN, m0 = tile / tiles_n * P::BM;
+  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
+  const int64_t n0 = (int64_t)(tile % tiles_n) * P::BN, m0 = (int64_t)(tile / tiles_n) * P::BM;
   const int64_t k0 = blockIdx.y * share, k1 = k0 + share < o.K ? k0 + share : o.K;
   P p;
   p.run(o, lds, m0, n0, k0, k1);
-  float* sums = s.sums + blockIdx.y * o.M * o.N;
+  float* sums = s.sums + blockIdx.y * o.M * o.N + m0 * o.N + n0;
+  const unsigned ld = (unsigned)o.N;
+  const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < MI; ++i) {
+    float old[4][NI];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t row = m0 + p.row_of(i, r);
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int64_t col = n0 + p.col_of(j);
-        if (row < o.M && col < o.N) {
-          float* at = sums + row * o.N + col;
-          *at = s.add ? *at + p.c[i][j][r] : p.c[i][j][r];
-        }
+        old[r][j] = 0.0f;
+        if (s.add && (whole || (m0 + p.row_of(i, r) < o.M && n0 + p.col_of(j) < o.N))) old[r][j] = sums[p.row_of(i, r) * ld + p.col_of(j)];
       }
-    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        if (whole || (m0 + p.row_of(i, r) < o.M && n0 + p.col_of(j) < o.N)) sums[p.row_of(i, r) * ld + p.col_of(j)] = old[r][j] + p.c[i][j][r];
+  }
 }
 
 template <typename T>
@@ -313,16 +365,17 @@ __global__ void __launch_bounds__(256) loss_pad(const T* in, int64_t in_row, int
   out[i] = c < cols ? in[r * in_row + c] : (T)0.0f;
 }
 
-// [rows x cols] with any row stride -> [cols x rows_padded], zeros in the padding.  64 x 64 tiles through LDS.
+// [rows x cols] with any row stride -> [cols x rows_padded], zeros in the padding.  64 x 64 tiles through LDS.  A row without a gradient (lse
+// +infinity) becomes zeros: whatever stands in it, its product with dl's zeros is zero.
 template <typename T>
-__global__ void __launch_bounds__(256) loss_transpose(const T* in, int64_t in_row, int64_t rows, int64_t cols, T* out, int64_t rows_padded) {
+__global__ void __launch_bounds__(256) loss_transpose(const T* in, int64_t in_row, int64_t rows, int64_t cols, T* out, int64_t rows_padded, const float* lse) {
   __shared__ T tile[64][64 + 4 / sizeof(T)];
   const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
   const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
     const int64_t r = r0 + y + i, c = c0 + x;
-    tile[y + i][x] = r < rows && c < cols ? in[r * in_row + c] : (T)0.0f;
+    tile[y + i][x] = r < rows && c < cols && !(lse && lse[r] == INFINITY) ? in[r * in_row + c] : (T)0.0f;
   }
   __syncthreads();
 #pragma unroll
@@ -349,7 +402,7 @@ Config config_for(int64_t m, int64_t n, int64_t times) {
 
 struct Layout { int64_t bytes = 0; int64_t take(int64_t n) { int64_t at = bytes; bytes += padded(n, 256); return at; } };
 
-struct ForwardPlan { Config config; int64_t columns, features_padded, hidden, weight, partial, wanted, bytes; };
+struct ForwardPlan { Config config; int64_t columns, features_padded, hidden, weight, partial, bytes; };
 ForwardPlan plan_forward(const ppn_loss_args* a) {
   ForwardPlan p;
   Layout l;
@@ -360,7 +413,6 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
   p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
   p.partial = l.take(a->rows * p.columns * 8);
-  p.wanted = l.take(a->rows * 4);
   p.bytes = l.bytes;
   return p;
 }
@@ -455,13 +507,12 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
       if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
       o.B = w + p.weight, o.ldb = p.features_padded;
     }
-    const StatsArgs st = {a->allowed, a->allowed_row, a->target, (float2*)(w + p.partial), (float*)(w + p.wanted), p.columns};
+    const StatsArgs st = {a->allowed, a->allowed_row, (float2*)(w + p.partial), p.columns};
     const int64_t tm = ceil_div(a->rows, p.config.bm), tn = ceil_div(a->actions, p.config.bn);
     if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
     if (p.config.large) loss_stats<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
     else loss_stats<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
-    loss_join<<<dim3(ceil_div(a->rows, 4)), dim3(256), 0, s>>>(st.partial, p.columns, st.wanted, a->target, a->allowed, a->allowed_row, a->rows, a->actions,
-                                                               a->ignore_index, a->loss, a->lse);
+    loss_join<T><<<dim3(ceil_div(a->rows, 4)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
     return launched("ppn_loss_forward");
   });
 }
@@ -496,10 +547,10 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
     }
     if (a->dweight)
       loss_transpose<T><<<dim3(ceil_div(p.rows_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->hidden, a->hidden_row, a->rows, a->features,
-                                                                                                          (T*)(w + p.hidden_t), p.rows_padded);
+                                                                                                          (T*)(w + p.hidden_t), p.rows_padded, a->lse);
     if (a->dhidden)
       loss_transpose<T><<<dim3(ceil_div(p.actions_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->weight, a->weight_row, a->actions,
-                                                                                                             a->features, (T*)(w + p.weight_t), p.actions_padded);
+                                                                                                             a->features, (T*)(w + p.weight_t), p.actions_padded, nullptr);
     loss_scale<<<dim3(1), dim3(256), 0, s>>>(a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale);
     for (int64_t first = 0; first < a->actions; first += p.piece) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 32);
@@ -512,7 +563,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
         const Operands q = {w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np};
         const int64_t um = ceil_div(a->rows, p.dh_config.bm), un = ceil_div(a->features, p.dh_config.bn);
         // (the last piece is shorter: a share that begins past its end adds nothing, so every slot is written by the first piece)
-        const SumArgs sums = {(float*)(w + p.dh), p.dh_slots, first > 0};
+        const SumArgs sums = {(float*)(w + p.dh), first > 0};
         const dim3 grid(um * un, first > 0 ? ceil_div(np, p.dh_share) : p.dh_slots);
         if (p.dh_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
         else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
@@ -520,7 +571,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
       if (a->dweight) {
         const Operands q = {w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded};
         const int64_t um = ceil_div(n, p.dw_config.bm), un = ceil_div(a->features, p.dw_config.bn);
-        const SumArgs sums = {(float*)(w + p.dw), p.dw_slots, false};
+        const SumArgs sums = {(float*)(w + p.dw), false};
         const dim3 grid(um * un, p.dw_slots);
         if (p.dw_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
         else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
