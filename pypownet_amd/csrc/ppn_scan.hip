@@ -13,7 +13,7 @@
 namespace ppn_policy {
 namespace {
 
-constexpr int ROWS = 8;          // rows staged together; also the distance of the checkpoints the backward pass restarts from
+constexpr int ROWS = 8;          // rows of a block; also the distance of the checkpoints the backward pass restarts from
 
 // ---- lanes -------------------------------------------------------------------------------------------------------------------------
 // NS states per lane, LPC lanes per channel, 64 / LPC channels per wave: lane = part * (64 / LPC) + channel, part p has states p NS ..
@@ -97,24 +97,41 @@ template <int V, int LPC> struct Kept {
   static constexpr int LEVELS = LPC == 1 ? 6 : LPC == 2 ? 5 : 4;
   static constexpr int COUNT = (V >> LEVELS) > 1 ? (V >> LEVELS) : 1;
   static constexpr int SPARE = V >= (1 << LEVELS) ? 0 : LPC == 1 ? (V == 32 ? 1 : 2) : (V == 16 ? 1 : 0);      // low lane bits that hold copies
-  __device__ static bool writes(int lane) { return (lane & ((1 << SPARE) - 1)) == 0; }
   __device__ static int first(int lane) { return ((lane & ((1 << LEVELS) - 1)) >> SPARE) * COUNT; }
 };
 
 // ---- staging -----------------------------------------------------------------------------------------------------------------------
-// ROWS rows of B (and C) of one environment and group, as 32-bit floats in LDS, zero beyond the last state and the last row.
-template <typename T, int STATES, bool WITH_C>
-__device__ inline void stage(const ppn_scan_args& a, int64_t b, int64_t g, int64_t t0, int64_t t1, float* sb, float* sc) {
-  const T* B = (const T*)a.B + b * a.B_batch + g * a.B_group;
-  const T* C = (const T*)a.C + b * a.C_batch + g * a.C_group;
+// The rows are taken in blocks of ROWS without a branch that a memory operation hangs on: the wait for a block's loads would otherwise be a
+// wait for every store before them too.  A block past the end of the time axis (or of the chunk) repeats its last row with a step
+// size of zero, which leaves the state as it is and writes the last row's values again; a lane past the last channel, and the second and
+// later lanes of a channel, write what the channel's own lane writes.
+
+// Addresses are a pointer that is the same for the wave, in scalar registers, and an unsigned 32-bit byte offset.  A block's rows lie within such
+// an offset: strides of time are at most 2^27 elements, as the entry points check.
+template <typename V> __device__ inline V& at(const void* base, unsigned bytes) { return *(V*)((char*)base + bytes); }
+
+// ROWS rows of B and C of one environment and group, as 32-bit floats in LDS, zero beyond the last state: fetched into registers while the
+// rows before are worked on, put into LDS when their turn comes.
+template <typename T, int STATES, bool WITH_B, bool WITH_C> struct Staged {
+  static constexpr int COUNT = ROWS * STATES / 64;
+  T b[COUNT], c[COUNT];
+  __device__ void fetch(const ppn_scan_args& a, const T* B, const T* C, int rows) {      // B, C: at the block's first row
 #pragma unroll
-  for (int i = 0; i < ROWS * STATES / 64; ++i) {
-    const int e = threadIdx.x + 64 * i, j = e / STATES, n = e % STATES;
-    const bool in = n < a.states && t0 + j < t1;
-    sb[e] = in ? to_float(B[(t0 + j) * a.B_time + n]) : 0.0f;
-    if constexpr (WITH_C) sc[e] = in ? to_float(C[(t0 + j) * a.C_time + n]) : 0.0f;
+    for (int i = 0; i < COUNT; ++i) {
+      const int e = threadIdx.x + 64 * i, j = min(e / STATES, rows - 1), n = min(e % STATES, (int)a.states - 1);
+      if constexpr (WITH_B) b[i] = at<const T>(B, ((unsigned)j * (unsigned)a.B_time + (unsigned)n) * (unsigned)sizeof(T));
+      if constexpr (WITH_C) c[i] = at<const T>(C, ((unsigned)j * (unsigned)a.C_time + (unsigned)n) * (unsigned)sizeof(T));
+    }
   }
-}
+  __device__ void put(int states, float* sb, float* sc) const {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int e = threadIdx.x + 64 * i;
+      if constexpr (WITH_B) sb[e] = e % STATES < states ? to_float(b[i]) : 0.0f;
+      if constexpr (WITH_C) sc[e] = e % STATES < states ? to_float(c[i]) : 0.0f;
+    }
+  }
+};
 
 template <int NS> __device__ inline void read_states(const float* p, float (&v)[NS]) {
 #pragma unroll
@@ -124,27 +141,55 @@ template <int NS> __device__ inline void read_states(const float* p, float (&v)[
   }
 }
 
-// Bit j: row t0 + j begins an episode.  Wave-uniform.
-__device__ inline unsigned starts_of(const ppn_scan_args& a, int64_t b, int64_t t0, int64_t t1) {
-  if (!a.starts) return 0;
-  const int lane = threadIdx.x;
-  const bool s = lane < ROWS && t0 + lane < t1 && a.starts[b * a.starts_batch + (t0 + lane) * a.starts_time] != 0;
-  return (unsigned)__ballot(s);
+// One block's rows of a [.. x channels] tensor, this lane's channel: ROWS loads in flight.
+template <typename T> struct Column {
+  T v[ROWS];
+  __device__ void fetch(const T* p, int64_t stride, unsigned d, int rows) {
+    const unsigned step = (unsigned)stride * (unsigned)sizeof(T);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) v[j] = at<const T>(p, (unsigned)min(j, rows - 1) * step + d * (unsigned)sizeof(T));
+  }
+};
+
+// A value the compiler knows nothing about: what follows is computed from it here, not moved in front of earlier rows or kept from them (eight rows'
+// exponentials, B and C do not fit the registers next to the states).
+__device__ inline float anew(float v) {
+  asm volatile("" : "+v"(v)::"memory");
+  __builtin_amdgcn_sched_barrier(0);
+  return v;
+}
+template <typename T> __device__ inline float widened(T v) {      // to_float, here and not in front of earlier rows
+  float f = to_float(v);
+  asm volatile("" : "+v"(f));
+  return f;
 }
 
-struct Place { int64_t b, g, d; bool live; int part; };
+// Bit j: row t0 + j begins an episode.  Wave-uniform.
+__device__ inline unsigned starts_of(const ppn_scan_args& a, int64_t b, int64_t t0, int rows) {
+  if (!a.starts) return 0;
+  const int lane = threadIdx.x, j = min(lane, rows - 1);
+  const bool s = a.starts[b * a.starts_batch + (t0 + j) * a.starts_time] != 0;
+  return (unsigned)__ballot(s && lane < rows);
+}
 
-// Workgroup x: (environment, group, tile of channels), the tile fastest.  A lane past the last channel works on the last one and writes nothing.
-template <int NS, int LPC> __device__ inline Place place(const ppn_scan_args& a, int64_t x) {
-  constexpr int CHANNELS = Shape<NS, LPC>::CHANNELS;
-  const int64_t wide = a.channels / a.groups, tiles = (wide + CHANNELS - 1) / CHANNELS;
+// d: this lane's channel, as an unsigned offset from a row's address, which is the same for the wave and kept in scalar registers.
+struct Place { int64_t b, g, tile; unsigned d; bool live; int part; };
+
+// Workgroup x: (environment, group, tile of channels), the tile fastest.  The eight dies take workgroups in turn, each with its own L2: neighbours
+// in that order (which share rows of B and C, and cache lines where a tile's rows end inside one) are given to one die.  A lane past the last
+// channel works on the last one.
+template <int NS, int LPC> __device__ inline Place place(const ppn_scan_args& a) {
+  constexpr unsigned CHANNELS = Shape<NS, LPC>::CHANNELS;
+  const unsigned per = gridDim.x / 8, x = blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+  const unsigned groups = (unsigned)a.groups, wide = (unsigned)a.channels / groups, tiles = (wide + CHANNELS - 1) / CHANNELS;
+  const unsigned b = x / (groups * tiles), gt = x - b * (groups * tiles), g = gt / tiles, tile = gt - g * tiles;
   Place p;
-  const int64_t gt = x % (a.groups * tiles);
-  p.b = x / (a.groups * tiles);
-  p.g = gt / tiles;
-  const int64_t c = (gt - p.g * tiles) * CHANNELS + threadIdx.x % CHANNELS;
+  p.b = __builtin_amdgcn_readfirstlane((int)b);
+  p.g = __builtin_amdgcn_readfirstlane((int)g);
+  p.tile = __builtin_amdgcn_readfirstlane((int)tile);
+  const unsigned c = tile * CHANNELS + threadIdx.x % CHANNELS;
   p.live = c < wide;
-  p.d = p.g * wide + (p.live ? c : wide - 1);
+  p.d = g * wide + (p.live ? c : wide - 1);
   p.part = threadIdx.x / CHANNELS;
   return p;
 }
@@ -159,104 +204,127 @@ template <int NS> __device__ inline void store_states(float* p, int64_t states, 
   for (int n = 0; n < NS; ++n)
     if (part * NS + n < states) p[part * NS + n] = v[n];
 }
-// Workspace states: [.. x states x channels], so that a wave's lanes write next to each other.
-template <int NS> __device__ inline void load_plane(const float* p, int64_t states, int64_t channels, int64_t d, int part, float (&v)[NS]) {
+// Workspace states: [.. x states x channels], so that a wave's lanes write next to each other.  Places past the last state are read as the last one
+// (and do not matter: B and C are zero there).
+template <int NS> __device__ inline void load_plane(const float* p, int64_t states, int64_t channels, unsigned d, int part, float (&v)[NS]) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) v[n] = part * NS + n < states ? p[(part * NS + n) * channels + d] : 0.0f;
+  for (int n = 0; n < NS; ++n) v[n] = at<const float>(p, ((unsigned)min(part * NS + n, (int)states - 1) * (unsigned)channels + d) * 4u);
 }
-template <int NS> __device__ inline void store_plane(float* p, int64_t states, int64_t channels, int64_t d, int part, const float (&v)[NS]) {
+template <int NS> __device__ inline void store_plane(float* p, int64_t states, int64_t channels, unsigned d, int part, const float (&v)[NS]) {
 #pragma unroll
   for (int n = 0; n < NS; ++n)
-    if (part * NS + n < states) p[(part * NS + n) * channels + d] = v[n];
+    if (part * NS + n < (int)states) at<float>(p, ((unsigned)(part * NS + n) * (unsigned)channels + d) * 4u) = v[n];
 }
 
-__device__ inline float step_size(float dt, float bias, bool soft) {
-  const float v = dt + bias;
-  return soft ? softplus(v) : v;
+// softplus of a block's step sizes at once (one branch); rows past the block's last one: 0.
+template <typename T> __device__ inline void step_sizes(const Column<T>& dt, float bias, bool soft, int rows, float (&delta)[ROWS]) {
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) delta[j] = to_float(dt.v[j]) + bias;
+  if (soft) {
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) delta[j] = softplus(delta[j]);
+  }
+#pragma unroll
+  for (int j = 1; j < ROWS; ++j) delta[j] = j < rows ? delta[j] : 0.0f;
+}
+
+// The state behind a row; a row that begins an episode drops the state before, whatever is in it (a branch the whole wave takes).
+template <int NS> __device__ inline void advance(const float (&before)[NS], float (&h)[NS], float delta, float w, const float (&A2)[NS], const float (&bv)[NS], bool begin) {
+  if (begin) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[n] = w * bv[n];
+  } else {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[n] = __builtin_amdgcn_exp2f(delta * A2[n]) * before[n] + w * bv[n];
+  }
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // One wave: 64 / LPC channels of one environment over the rows of one chunk (grid.y chunks of `chunk` rows, a multiple of ROWS).
-// SUMMARY: no outputs, only what the chunk does to a state that enters it: its own end state from zero, and the sum of delta (the decay of
-// the whole chunk is exp(A sum delta)); -1 stands for a chunk that an episode's start cuts, through which nothing passes.
-template <typename T, int NS, int LPC, bool SUMMARY>
-__global__ void __launch_bounds__(64) scan_forward(ppn_scan_args a, int64_t chunk, int64_t chunks, const float* entering, float* ends, float* sums) {
+// OUTPUT: y.  TRAIN: the states in front of every block as well.  SUMMARY: neither, only what the chunk does to a state that enters it: its
+// own end state from zero, the sum of delta (the decay of the whole chunk is exp(A sum delta)), and whether an episode's start cuts it.
+enum { OUTPUT, TRAIN, SUMMARY };
+template <typename T, int NS, int LPC, int MODE>
+__global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t chunk, int64_t chunks, const float* entering, float* ends, float* sums) {
   constexpr int STATES = Shape<NS, LPC>::STATES;
-  __shared__ __align__(16) float sb[2][ROWS * STATES], sc[2][SUMMARY ? 4 : ROWS * STATES];
-  const Place p = place<NS, LPC>(a, blockIdx.x);
-  const int64_t k = blockIdx.y, t0 = k * chunk, t1 = t0 + chunk < a.time ? t0 + chunk : a.time;
-  const bool writes = p.live && p.part == 0;
+  __shared__ __align__(16) float sb[ROWS * STATES], sc[ROWS * STATES];
+  const Place p = place<NS, LPC>(a);
+  const int64_t k = blockIdx.y, t0 = k * chunk, t1 = t0 + chunk < a.time ? t0 + chunk : a.time, plane = a.states * a.channels;
   float A2[NS], h[NS];
-  load_states<NS>(a.A + p.d * a.states, a.states, p.part, A2);
+  load_states<NS>(a.A + (int64_t)p.d * a.states, a.states, p.part, A2);
 #pragma unroll
   for (int n = 0; n < NS; ++n) A2[n] *= LOG2E, h[n] = 0.0f;
-  if constexpr (!SUMMARY) {
-    if (entering) load_plane<NS>(entering + (p.b * chunks + k) * a.states * a.channels, a.states, a.channels, p.d, p.part, h);
+  if constexpr (MODE != SUMMARY) {
+    if (entering) load_plane<NS>(entering + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
     else if (a.initial) load_states<NS>(a.initial + (p.b * a.channels + p.d) * a.states, a.states, p.part, h);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
-  const bool soft = a.softplus;
-  const T* x = (const T*)a.x + p.b * a.x_batch + p.d;
-  const T* dt = (const T*)a.dt + p.b * a.dt_batch + p.d;
-  const T* z = a.z && !SUMMARY ? (const T*)a.z + p.b * a.z_batch + p.d : nullptr;
-  T* y = (T*)a.y + p.b * a.y_batch + p.d;
+  const bool soft = a.softplus, gated = a.z != nullptr;
+  // (without a gate, x is read in its place)
+  const void* zz = gated ? a.z : a.x;
+  const int64_t z_batch = gated ? a.z_batch : a.x_batch, z_time = gated ? a.z_time : a.x_time;
+  const T* px = (const T*)a.x + p.b * a.x_batch + t0 * a.x_time;
+  const T* pdt = (const T*)a.dt + p.b * a.dt_batch + t0 * a.dt_time;
+  const T* pz = (const T*)zz + p.b * z_batch + t0 * z_time;
+  const T* pB = (const T*)a.B + p.b * a.B_batch + p.g * a.B_group + t0 * a.B_time;
+  const T* pC = (const T*)a.C + p.b * a.C_batch + p.g * a.C_group + t0 * a.C_time;
+  T* py = (T*)a.y + p.b * a.y_batch + t0 * a.y_time;
+  float* pmark = MODE == TRAIN ? a.checkpoints + (p.b * ((a.time + ROWS - 1) / ROWS) + t0 / ROWS) * plane : nullptr;
+  const unsigned y_step = (unsigned)a.y_time * (unsigned)sizeof(T);
   float total = 0.0f;
   bool cut = false;
-  int turn = 0;
-  for (int64_t t = t0; t < t1; t += ROWS, turn ^= 1) {
-    T rx[ROWS], rdt[ROWS], rz[ROWS];
+  for (int64_t t = t0; t < t1; t += ROWS) {
+    const int rows = (int)min(t1 - t, (int64_t)ROWS);
+    Column<T> x, dt, z;
+    Staged<T, STATES, true, MODE != SUMMARY> bc;
+    dt.fetch(pdt, a.dt_time, p.d, rows);
+    x.fetch(px, a.x_time, p.d, rows);
+    bc.fetch(a, pB, pC, rows);
+    if constexpr (MODE != SUMMARY) z.fetch(pz, z_time, p.d, rows);
+    const unsigned now = starts_of(a, p.b, t, rows);
+    px += ROWS * a.x_time, pdt += ROWS * a.dt_time, pz += ROWS * z_time, pB += ROWS * a.B_time, pC += ROWS * a.C_time;
+    cut |= now != 0;
+    float delta[ROWS], w[ROWS], gate[ROWS], over[ROWS];
+    step_sizes(dt, bias, soft, rows, delta);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      const int64_t at = t + j < t1 ? t + j : t1 - 1;
-      rx[j] = x[at * a.x_time];
-      rdt[j] = dt[at * a.dt_time];
-      if (z) rz[j] = z[at * a.z_time];
+      const float xv = to_float(x.v[j]);
+      w[j] = delta[j] * xv;
+      over[j] = skip * xv;
+      total += delta[j];
+      if constexpr (MODE != SUMMARY) {
+        const float zv = to_float(z.v[j]);
+        gate[j] = gated ? zv * sigmoid(zv) : 1.0f;
+      }
     }
-    const unsigned begins = starts_of(a, p.b, t, t1);
-    stage<T, STATES, !SUMMARY>(a, p.b, p.g, t, t1, sb[turn], sc[turn]);
     __syncthreads();
-    if constexpr (!SUMMARY) {
-      if (a.checkpoints && p.live) {
-        const int64_t marks = (a.time + ROWS - 1) / ROWS;
-        store_plane<NS>(a.checkpoints + (p.b * marks + t / ROWS) * a.states * a.channels, a.states, a.channels, p.d, p.part, h);
-      }
+    bc.put((int)a.states, sb, sc);
+    __syncthreads();
+    if constexpr (MODE == TRAIN) {
+      store_plane<NS>(pmark, a.states, a.channels, p.d, p.part, h);
+      pmark += plane;
     }
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      if (t + j >= t1) break;
-      const float xv = to_float(rx[j]), delta = step_size(to_float(rdt[j]), bias, soft), dx = delta * xv;
       float bv[NS];
-      read_states<NS>(sb[turn] + j * STATES + p.part * NS, bv);
-      if ((begins >> j) & 1) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = dx * bv[n];
-        cut = true;
-      } else {
-#pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = __builtin_amdgcn_exp2f(delta * A2[n]) * h[n] + dx * bv[n];
-      }
-      total += delta;
-      if constexpr (!SUMMARY) {
+      const float step = anew(delta[j]);
+      read_states<NS>(sb + j * STATES + p.part * NS, bv);
+      advance<NS>(h, h, step, w[j], A2, bv, (now >> j) & 1);
+      if constexpr (MODE != SUMMARY) {
         float cv[NS], s = 0.0f;
-        read_states<NS>(sc[turn] + j * STATES + p.part * NS, cv);
+        read_states<NS>(sc + j * STATES + p.part * NS, cv);
 #pragma unroll
         for (int n = 0; n < NS; ++n) s += cv[n] * h[n];
-        s = sum_parts<LPC>(s) + skip * xv;
-        if (z) {
-          const float zv = to_float(rz[j]);
-          s *= zv * sigmoid(zv);
-        }
-        if (writes) y[(t + j) * a.y_time] = (T)s;
+        at<T>(py, (unsigned)min(j, rows - 1) * y_step + p.d * (unsigned)sizeof(T)) = (T)((sum_parts<LPC>(s) + over[j]) * gate[j]);
       }
     }
+    py += ROWS * a.y_time;
   }
-  if constexpr (SUMMARY) {
-    if (p.live) store_plane<NS>(ends + (p.b * chunks + k) * a.states * a.channels, a.states, a.channels, p.d, p.part, h);
-    if (writes) {
-      sums[((p.b * chunks + k) * 2 + 0) * a.channels + p.d] = total;
-      sums[((p.b * chunks + k) * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
-    }
-  } else if (p.live && a.final_state && t1 == a.time) {
+  if constexpr (MODE == SUMMARY) {
+    store_plane<NS>(ends + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
+    sums[((p.b * chunks + k) * 2 + 0) * a.channels + p.d] = total;
+    sums[((p.b * chunks + k) * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
+  } else if (a.final_state && t1 == a.time) {
     store_states<NS>(a.final_state + (p.b * a.channels + p.d) * a.states, a.states, p.part, h);
   }
 }
@@ -272,7 +340,7 @@ __global__ void __launch_bounds__(256) scan_join(ppn_scan_args a, int64_t chunks
   float h = outside ? outside[(b * a.channels + d) * a.states + n] : 0.0f;
   float* p = ends + b * chunks * per + rest;
   const float* s = sums + b * chunks * 2 * a.channels + d;
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 32;
   for (int64_t i0 = 0; i0 < chunks; i0 += AHEAD) {
     float own[AHEAD], total[AHEAD], cut[AHEAD];
 #pragma unroll
@@ -296,174 +364,176 @@ __global__ void __launch_bounds__(256) scan_join(ppn_scan_args a, int64_t chunks
 // With u[t] = dy[t] silu(z[t]) and the adjoint e[t] = u[t] C[t] + exp(delta[t+1] A) e[t+1]  (0 across an episode's start):
 //   dC[t] = sum_d u[t] h[t]       dB[t] = sum_d e[t] delta[t] x[t]       dx[t] = delta[t] sum_n e[t] B[t] + D u[t]
 //   q[t] = e[t] exp(delta[t] A) h[t-1];   ddelta[t] = sum_n q[t] A + x[t] sum_n e[t] B[t];   dA = sum_t q[t] delta[t]
-// The rows are taken in blocks of 8 from the last to the first: the states of a block are recomputed from its checkpoint and kept in
-// registers (8 x NS), then the block is walked backwards.  The sums over channels (dB, dC) are the wave's part of them, one row of partial
-// sums per tile of channels, added up by scan_reduce_rows; dA, dD and ddt_bias stay in registers over all rows and environments of the
-// workgroup and leave one row of partial sums each.  Both reductions run in a fixed order.
+// The rows are taken in blocks of 8 from the last to the first.  A block's states are recomputed from its checkpoint, four rows' worth kept in
+// registers at a time with 16 states a lane (5 x 16; the first four rows are walked twice for that: 8 % more work, and two waves fit a SIMD
+// where all eight rows' states left room for one), eight with 8 states.  The sums over channels (dB, dC) are the wave's part of them, one row of
+// partial sums per tile of channels, added up by scan_reduce_rows; dA, dD and ddt_bias stay in registers over the wave's rows and leave one
+// row of partial sums for each environment and chunk.  Both reductions run in a fixed order.
 //
-// SUMMARY: only what a chunk adds to the adjoint in front of it, and its sum of delta, for chunks that are worked on at once.
-template <typename T, int NS, int LPC, bool SUMMARY>
-__global__ void __launch_bounds__(64) scan_backward(ppn_scan_args a, int64_t chunk, int64_t chunks, int64_t share, const float* entering, float* ends, float* sums,
-                                                    float* rows_out, float* params_out) {
-  constexpr int STATES = Shape<NS, LPC>::STATES, CHANNELS = Shape<NS, LPC>::CHANNELS;
-  __shared__ __align__(16) float sb[ROWS * STATES], sc[ROWS * STATES];
-  const int64_t wide = a.channels / a.groups, tiles = (wide + CHANNELS - 1) / CHANNELS;
-  const int64_t k = blockIdx.y, first = k * chunk, last = first + chunk < a.time ? first + chunk : a.time, marks = (a.time + ROWS - 1) / ROWS;
-  const bool soft = a.softplus;
-  Place p = place<NS, LPC>(a, blockIdx.x);
-  const bool writes = p.live && p.part == 0;
+// ADJOINT: only what a chunk adds to the adjoint in front of it, and its sum of delta, for chunks that are worked on at once.
+template <typename T, int NS, int LPC, bool ADJOINT>
+__global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t chunk, int64_t chunks, const float* entering, float* ends, float* sums, float* rows_out,
+                                                                    float* params_out) {
+  constexpr int STATES = Shape<NS, LPC>::STATES, KEPT = NS == 8 ? ROWS : ROWS / 2;
+  __shared__ __align__(16) float sb[ADJOINT ? 4 : ROWS * STATES], sc[ROWS * STATES];
+  const Place p = place<NS, LPC>(a);
+  const int64_t k = blockIdx.y, first = k * chunk, last = first + chunk < a.time ? first + chunk : a.time;
+  const int64_t plane = a.states * a.channels, pair = a.groups * 2 * STATES, cell = p.b * chunks + k;
+  const bool soft = a.softplus, gated = a.z != nullptr;
   const float alive = p.live ? 1.0f : 0.0f;
-  const int64_t b0 = p.b * share, b1 = b0 + share < a.batch ? b0 + share : a.batch;
+  int64_t t = (last - 1) / ROWS * ROWS;
+  // without a gate: x in z's place, and dz goes where dx is written over it
+  const bool dgate = a.dz != nullptr;
+  const int64_t x_time = a.x_time, dt_time = a.dt_time, dy_time = a.dy_time, dx_time = a.dx_time, ddt_time = a.ddt_time;
+  const int64_t z_time = gated ? a.z_time : x_time, dz_time = dgate ? a.dz_time : dx_time;
+  const T* px = (const T*)a.x + p.b * a.x_batch + t * x_time;
+  const T* pdt = (const T*)a.dt + p.b * a.dt_batch + t * dt_time;
+  const T* pdy = (const T*)a.dy + p.b * a.dy_batch + t * dy_time;
+  const T* pz = gated ? (const T*)a.z + p.b * a.z_batch + t * z_time : px;
+  const T* pB = (const T*)a.B + p.b * a.B_batch + p.g * a.B_group + t * a.B_time;
+  const T* pC = (const T*)a.C + p.b * a.C_batch + p.g * a.C_group + t * a.C_time;
+  T* pdx = ADJOINT ? nullptr : (T*)a.dx + p.b * a.dx_batch + t * dx_time;
+  T* pddt = ADJOINT ? nullptr : (T*)a.ddt + p.b * a.ddt_batch + t * ddt_time;
+  T* pdz = ADJOINT ? nullptr : dgate ? (T*)a.dz + p.b * a.dz_batch + t * dz_time : pdx;
+  const float* pmark = ADJOINT ? nullptr : a.checkpoints + (p.b * ((a.time + ROWS - 1) / ROWS) + t / ROWS) * plane;
+  float* pout = ADJOINT ? nullptr : rows_out + ((p.tile * a.batch + p.b) * a.time + t) * pair + p.g * 2 * STATES;
   float A2[NS], dA[NS], e[NS];
-  load_states<NS>(a.A + p.d * a.states, a.states, p.part, A2);
+  load_states<NS>(a.A + (int64_t)p.d * a.states, a.states, p.part, A2);
 #pragma unroll
-  for (int n = 0; n < NS; ++n) A2[n] *= LOG2E, dA[n] = 0.0f;
+  for (int n = 0; n < NS; ++n) A2[n] *= LOG2E, dA[n] = 0.0f, e[n] = 0.0f;
+  if constexpr (!ADJOINT) {
+    if (entering) load_plane<NS>(entering + cell * plane, a.states, a.channels, p.d, p.part, e);
+    else if (a.dfinal) load_states<NS>(a.dfinal + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
+  }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
-  float dskip = 0.0f, dbias = 0.0f;
-  for (int64_t b = b0; b < b1; ++b) {
-    const T* x = (const T*)a.x + b * a.x_batch + p.d;
-    const T* dt = (const T*)a.dt + b * a.dt_batch + p.d;
-    const T* z = a.z ? (const T*)a.z + b * a.z_batch + p.d : nullptr;
-    const T* dy = (const T*)a.dy + b * a.dy_batch + p.d;
-    T* dx = (T*)a.dx + b * a.dx_batch + p.d;
-    T* ddt = (T*)a.ddt + b * a.ddt_batch + p.d;
-    T* dz = a.dz ? (T*)a.dz + b * a.dz_batch + p.d : nullptr;
+  const unsigned mine = p.d * (unsigned)sizeof(T);
+  float dskip = 0.0f, dbias = 0.0f, total = 0.0f;
+  bool cut = false;
+  for (; t >= first; t -= ROWS) {
+    const int rows = (int)min(last - t, (int64_t)ROWS);
+    Column<T> x, dt, z, dy;
+    Staged<T, STATES, !ADJOINT, true> bc;
+    float mark[NS], h[ADJOINT ? 1 : KEPT + 1][NS], delta[ROWS];
+    dt.fetch(pdt, dt_time, p.d, rows);
+    bc.fetch(a, pB, pC, rows);
+    if constexpr (!ADJOINT) load_plane<NS>(pmark, a.states, a.channels, p.d, p.part, mark);
+    if constexpr (!ADJOINT) x.fetch(px, x_time, p.d, rows);
+    dy.fetch(pdy, dy_time, p.d, rows);
+    z.fetch(pz, z_time, p.d, rows);
+    const unsigned now = starts_of(a, p.b, t, rows);
+    px -= ROWS * x_time, pdt -= ROWS * dt_time, pdy -= ROWS * dy_time, pz -= ROWS * z_time, pB -= ROWS * a.B_time, pC -= ROWS * a.C_time;
+    if constexpr (!ADJOINT) pmark -= plane;
+    cut |= now != 0;
+    step_sizes(dt, bias, soft, rows, delta);
+    if constexpr (ADJOINT) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) e[n] = 0.0f;
-    if constexpr (!SUMMARY) {
-      if (entering) load_plane<NS>(entering + (b * chunks + k) * a.states * a.channels, a.states, a.channels, p.d, p.part, e);
-      else if (a.dfinal) load_states<NS>(a.dfinal + (b * a.channels + p.d) * a.states, a.states, p.part, e);
+      for (int j = 0; j < ROWS; ++j) total += delta[j];
     }
-    float total = 0.0f;
-    bool cut = false;
-    for (int64_t t = (last - 1) / ROWS * ROWS; t >= first && last > first; t -= ROWS) {
-      T rx[ROWS], rdt[ROWS], rz[ROWS], rdy[ROWS];
-      float h[SUMMARY ? 1 : ROWS + 1][NS];
+    __syncthreads();
+    bc.put((int)a.states, sb, sc);
+    __syncthreads();
+    auto forward = [&](int j, const float (&before)[NS], float (&after)[NS]) {
+      float bv[NS];
+      const float step = anew(delta[j]);
+      read_states<NS>(sb + j * STATES + p.part * NS, bv);
+      advance<NS>(before, after, step, step * widened(x.v[j]), A2, bv, (now >> j) & 1);
+    };
 #pragma unroll
-      for (int j = 0; j < ROWS; ++j) {
-        const int64_t at = t + j < last ? t + j : last - 1;
-        if constexpr (!SUMMARY) rx[j] = x[at * a.x_time];
-        rdt[j] = dt[at * a.dt_time];
-        rdy[j] = dy[at * a.dy_time];
-        if (z) rz[j] = z[at * a.z_time];
-      }
-      if constexpr (!SUMMARY) load_plane<NS>(a.checkpoints + (b * marks + t / ROWS) * a.states * a.channels, a.states, a.channels, p.d, p.part, h[0]);
-      const unsigned begins = starts_of(a, b, t, last);
-      __syncthreads();
-      stage<T, STATES, true>(a, b, p.g, t, last, sb, sc);
-      __syncthreads();
-      if constexpr (!SUMMARY) {
+    for (int j = ROWS - 1; j >= 0; --j) {
+      if constexpr (!ADJOINT) {
+        if (j % KEPT == KEPT - 1) {          // the states in front of and behind rows j - KEPT + 1 .. j, from the checkpoint
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-          const float delta = step_size(to_float(rdt[j]), bias, soft), w = delta * to_float(rx[j]);
-          float bv[NS];
-          read_states<NS>(sb + j * STATES + p.part * NS, bv);
-          if ((begins >> j) & 1) {
+          for (int n = 0; n < NS; ++n) h[0][n] = mark[n];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) h[j + 1][n] = w * bv[n];
-          } else {
+          for (int i = 0; i < j - KEPT + 1; ++i) forward(i, h[0], h[0]);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) h[j + 1][n] = __builtin_amdgcn_exp2f(delta * A2[n]) * h[j][n] + w * bv[n];
-          }
+          for (int i = 0; i < KEPT; ++i) forward(j - KEPT + 1 + i, h[i], h[i + 1]);
         }
       }
+      const bool begin = (now >> j) & 1;
+      const float step = anew(delta[j]);
+      unsigned place = (unsigned)min(j, rows - 1);
+      asm volatile("" : "+s"(place));
+      const float real = __builtin_bit_cast(float, (int)place == j ? 0x3f800000 : 0);      // (a repeated last row adds nothing, and is written over by itself)
+      const float up = widened(dy.v[j]) * real, zv = widened(z.v[j]), sg = gated ? sigmoid(zv) : 1.0f, u = gated ? up * zv * sg : up;
+      float cv[NS];
+      read_states<NS>(sc + j * STATES + p.part * NS, cv);
+      if constexpr (ADJOINT) {
+        if (begin) {
 #pragma unroll
-      for (int j = ROWS - 1; j >= 0; --j) {
-        if (t + j >= last) continue;
-        const float raw = to_float(rdt[j]) + bias, delta = soft ? softplus(raw) : raw;
-        const float up = to_float(rdy[j]);
-        float u = up, sg = 0.0f, zv = 0.0f;
-        if (z) {
-          zv = to_float(rz[j]);
-          sg = sigmoid(zv);
-          u = up * zv * sg;
-        }
-        float cv[NS];
-        read_states<NS>(sc + j * STATES + p.part * NS, cv);
-        const bool begin = (begins >> j) & 1;
-        if constexpr (SUMMARY) {
-#pragma unroll
-          for (int n = 0; n < NS; ++n) e[n] = begin ? 0.0f : __builtin_amdgcn_exp2f(delta * A2[n]) * (e[n] + u * cv[n]);
-          total += delta;
-          cut |= begin;
+          for (int n = 0; n < NS; ++n) e[n] = 0.0f;
         } else {
-          const float xv = to_float(rx[j]), w = delta * xv;
-          float bv[NS], sums2[2 * NS], s = 0.0f, through = 0.0f, decay = 0.0f;
-          read_states<NS>(sb + j * STATES + p.part * NS, bv);
-          const float ul = u * alive, wl = w * alive;        // (a lane past the last channel adds nothing to the sums over channels)
+#pragma unroll
+          for (int n = 0; n < NS; ++n) e[n] = __builtin_amdgcn_exp2f(step * A2[n]) * (e[n] + u * cv[n]);
+        }
+      } else {
+        float bv[NS], part[2 * NS], s = 0.0f, through = 0.0f, decay = 0.0f;
+        read_states<NS>(sb + j * STATES + p.part * NS, bv);
+        const float xv = widened(x.v[j]), ul = u * alive, wl = step * xv * alive;        // (a lane past the last channel adds nothing to the sums over channels)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          s += cv[n] * h[j % KEPT + 1][n];
+          e[n] += u * cv[n];
+          part[NS + n] = ul * h[j % KEPT + 1][n];
+          part[n] = wl * e[n];
+          through += e[n] * bv[n];
+        }
+        if (begin) {
+#pragma unroll
+          for (int n = 0; n < NS; ++n) e[n] = 0.0f;
+        } else {
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            s += cv[n] * h[j + 1][n];
-            e[n] += u * cv[n];
-            sums2[NS + n] = ul * h[j + 1][n];
-            sums2[n] = wl * e[n];
-            through += e[n] * bv[n];
-            if (begin) {
-              e[n] = 0.0f;
-            } else {
-              e[n] *= __builtin_amdgcn_exp2f(delta * A2[n]);
-              const float q = e[n] * h[j][n];
-              dA[n] += q * delta;
-              decay += q * A2[n];
-            }
-          }
-          sum_channels<2 * NS, LPC>(sums2);
-          typedef Kept<2 * NS, LPC> K;
-          const int lane = threadIdx.x;
-          if (K::writes(lane)) {
-            const int64_t tile = blockIdx.x % (a.groups * tiles) % tiles;
-            float* out = rows_out + (((tile * a.batch + b) * a.time + t + j) * a.groups + p.g) * 2 * a.states;
-#pragma unroll
-            for (int i = 0; i < K::COUNT; ++i) {
-              const int v = K::first(lane) + i, n = p.part * NS + v % NS;
-              if (n < a.states) out[(v / NS) * a.states + n] = sums2[i];
-            }
-          }
-          s = sum_parts<LPC>(s) + skip * xv;
-          through = sum_parts<LPC>(through);
-          decay = sum_parts<LPC>(decay) * (1.0f / LOG2E);
-          float dd = decay + through * xv;
-          if (soft) dd *= raw > 20.0f ? 1.0f : sigmoid(raw);
-          dbias += dd;
-          dskip += u * xv;
-          if (writes) {
-            dx[(t + j) * a.dx_time] = (T)(through * delta + skip * u);
-            ddt[(t + j) * a.ddt_time] = (T)dd;
-            if (dz) dz[(t + j) * a.dz_time] = (T)(up * s * sg * (1.0f + zv * (1.0f - sg)));
+            e[n] *= __builtin_amdgcn_exp2f(step * A2[n]);
+            const float q = e[n] * h[j % KEPT][n];
+            dA[n] += q * step;
+            decay += q * A2[n];
           }
         }
+        sum_channels<2 * NS, LPC>(part);
+        typedef Kept<2 * NS, LPC> K;
+#pragma unroll
+        for (int i = 0; i < K::COUNT; ++i) {            // (lanes that hold copies write the same values)
+          const int v = K::first(threadIdx.x) + i, n = p.part * NS + v % NS;
+          at<float>(pout, (place * (unsigned)pair + (unsigned)((v / NS) * STATES + n)) * 4u) = part[i];
+        }
+        s = sum_parts<LPC>(s) + skip * xv;
+        through = sum_parts<LPC>(through);
+        decay = sum_parts<LPC>(decay) * (1.0f / LOG2E);
+        const float v = widened(dt.v[j]) + bias;
+        float dd = decay + through * xv;
+        dd *= !soft || v > 20.0f ? 1.0f : sigmoid(v);
+        dbias += dd * real;
+        dskip += u * xv;
+        at<T>(pdz, place * ((unsigned)dz_time * (unsigned)sizeof(T)) + mine) = (T)(up * s * sg * (1.0f + zv * (1.0f - sg)));
+        at<T>(pdx, place * ((unsigned)dx_time * (unsigned)sizeof(T)) + mine) = (T)(through * step + skip * u);
+        at<T>(pddt, place * ((unsigned)ddt_time * (unsigned)sizeof(T)) + mine) = (T)dd;
       }
     }
-    if constexpr (SUMMARY) {
-      if (p.live) store_plane<NS>(ends + (b * chunks + k) * a.states * a.channels, a.states, a.channels, p.d, p.part, e);
-      if (writes) {
-        sums[((b * chunks + k) * 2 + 0) * a.channels + p.d] = total;
-        sums[((b * chunks + k) * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
-      }
-    } else if (p.live && a.dinitial && first == 0) {
-      store_states<NS>(a.dinitial + (b * a.channels + p.d) * a.states, a.states, p.part, e);
-    }
+    if constexpr (!ADJOINT) pdx -= ROWS * dx_time, pddt -= ROWS * ddt_time, pdz -= ROWS * dz_time, pout -= ROWS * pair;
   }
-  if constexpr (!SUMMARY) {
-    float* out = params_out + (p.b * chunks + k) * (a.states + 2) * a.channels;
-    if (p.live) store_plane<NS>(out, a.states, a.channels, p.d, p.part, dA);
-    if (writes) {
-      out[a.states * a.channels + p.d] = dskip;
-      out[(a.states + 1) * a.channels + p.d] = dbias;
-    }
+  if constexpr (ADJOINT) {
+    store_plane<NS>(ends + cell * plane, a.states, a.channels, p.d, p.part, e);
+    sums[(cell * 2 + 0) * a.channels + p.d] = total;
+    sums[(cell * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
+  } else {
+    if (a.dinitial && first == 0) store_states<NS>(a.dinitial + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
+    float* out = params_out + cell * (a.states + 2) * a.channels;
+    store_plane<NS>(out, a.states, a.channels, p.d, p.part, dA);
+    out[a.states * a.channels + p.d] = dskip;
+    out[(a.states + 1) * a.channels + p.d] = dbias;
   }
 }
 
-// dB and dC out of the tiles' partial rows [tiles x rows x 2 states].
-template <typename T>
+// dB and dC out of the tiles' partial rows [tiles x rows x 2 STATES], padded to the states of whole lanes.
+template <typename T, int STATES>
 __global__ void __launch_bounds__(256) scan_reduce_rows(const float* in, int64_t tiles, int64_t rows, int64_t states, T* dB, T* dC) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, count = rows * 2 * states;
-  if (id >= count) return;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, count = rows * 2 * STATES, row = id / (2 * STATES);
+  const int v = (int)(id % (2 * STATES)), n = v % STATES;
+  if (id >= count || n >= states) return;
   float s = 0.0f;
   for (int64_t t = 0; t < tiles; ++t) s += in[t * count + id];
-  const int64_t row = id / (2 * states), v = id - row * 2 * states;
-  if (v < states) dB[row * states + v] = (T)s;
-  else dC[row * states + v - states] = (T)s;
+  (v < STATES ? dB : dC)[row * states + n] = (T)s;
 }
 
 // dA, dD, ddt_bias out of the workgroups' partial rows [shares x (states + 2) x channels].
@@ -472,7 +542,13 @@ __global__ void __launch_bounds__(256) scan_reduce_params(const float* in, int64
   const int part = threadIdx.x / 32;
   float s = 0.0f;
   if (col < columns)
-    for (int64_t r = part; r < shares; r += 8) s += in[r * columns + col];
+    for (int64_t r = part; r < shares; r += 64) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = r + 8 * i < shares ? in[(r + 8 * i) * columns + col] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
   __shared__ float sums[8][33];
   sums[part][threadIdx.x % 32] = s;
   __syncthreads();
@@ -538,7 +614,7 @@ __global__ void __launch_bounds__(256) scan_step(ppn_scan_step_args a) {
         cv[i] = in ? to_float(cp[i]) : 0.0f;
       }
       xv = to_float(((const T*)a.x)[row * a.x_row + d]);
-      const float delta = step_size(to_float(((const T*)a.dt)[row * a.dt_row + d]), a.dt_bias ? a.dt_bias[d] : 0.0f, a.softplus);
+      const float raw = to_float(((const T*)a.dt)[row * a.dt_row + d]) + (a.dt_bias ? a.dt_bias[d] : 0.0f), delta = a.softplus ? softplus(raw) : raw;
       if (a.z) zv = to_float(((const T*)a.z)[row * a.z_row + d]);
       const float w = delta * xv;
 #pragma unroll
@@ -564,6 +640,7 @@ __global__ void __launch_bounds__(256) scan_step(ppn_scan_step_args a) {
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------------------------
+// States per lane and lanes per channel.
 template <typename F> int by_states(int64_t states, F f) {
   if (states <= 8) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
   if (states <= 16) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
@@ -572,8 +649,15 @@ template <typename F> int by_states(int64_t states, F f) {
 }
 
 int64_t tiles_of(const ppn_scan_args* a) {
-  const int64_t channels = a->states <= 16 ? 64 : a->states <= 32 ? 32 : 16;
-  return ceil_div(a->channels / a->groups, channels);
+  int64_t lanes = 1;
+  by_states(a->states, [&](auto, auto lpc) { return (int)(lanes = decltype(lpc)::value); });
+  return ceil_div(a->channels / a->groups, 64 / lanes);
+}
+
+int64_t states_of(const ppn_scan_args* a) {
+  int64_t states = 0;
+  by_states(a->states, [&](auto ns, auto lpc) { return (int)(states = decltype(ns)::value * decltype(lpc)::value); });
+  return states;
 }
 
 // Chunks of time that are worked on at once: one while the waves of (environment, tile) alone fill the chip, since splitting walks the rows
@@ -589,20 +673,16 @@ Split split_time(const ppn_scan_args* a, int64_t waves, int64_t wanted) {
 }
 Split forward_split(const ppn_scan_args* a) { return split_time(a, a->batch * a->groups * tiles_of(a), 4096); }
 
-struct BackwardPlan { Split split; int64_t share, shares, rows_bytes, params_bytes, ends_bytes, sums_bytes; };
+struct BackwardPlan { Split split; int64_t rows_bytes, params_bytes, ends_bytes, sums_bytes; };
 BackwardPlan plan_backward(const ppn_scan_args* a) {
   BackwardPlan p;
-  const int64_t tiles = a->groups * tiles_of(a);
-  p.split = split_time(a, a->batch * tiles, 2048);
-  // environments per wave: one row of partial parameter gradients each, so as few as keep 2048 waves (two for each SIMD)
-  p.share = p.split.chunks > 1 ? 1 : a->batch * tiles / 2048;
-  if (p.share < 1) p.share = 1;
-  p.shares = ceil_div(a->batch, p.share);
+  p.split = split_time(a, a->batch * a->groups * tiles_of(a), 2048);
   auto round = [](int64_t v) { return (v + 255) / 256 * 256; };
-  p.rows_bytes = round(tiles_of(a) * a->batch * a->time * a->groups * 2 * a->states * 4);
-  p.params_bytes = round(p.shares * p.split.chunks * (a->states + 2) * a->channels * 4);
-  p.ends_bytes = p.split.chunks > 1 ? round(a->batch * p.split.chunks * a->states * a->channels * 4) : 0;
-  p.sums_bytes = p.split.chunks > 1 ? round(a->batch * p.split.chunks * 2 * a->channels * 4) : 0;
+  const int64_t cells = a->batch * p.split.chunks;
+  p.rows_bytes = round(tiles_of(a) * a->batch * a->time * a->groups * 2 * states_of(a) * 4);
+  p.params_bytes = round(cells * (a->states + 2) * a->channels * 4);
+  p.ends_bytes = p.split.chunks > 1 ? round(cells * a->states * a->channels * 4) : 0;
+  p.sums_bytes = p.split.chunks > 1 ? round(cells * 2 * a->channels * 4) : 0;
   return p;
 }
 
@@ -611,7 +691,10 @@ int check(const ppn_scan_args* a) {
   if (a->type < 0 || a->type > PPN_T_F16) return fail(PPN_E_INVALID, "element type %lld is unknown", (long long)a->type);
   if (a->batch < 0 || a->time < 0 || a->channels < 1 || a->groups < 1 || a->channels % a->groups)
     return fail(PPN_E_INVALID, "scan: batch, time >= 0 and channels a multiple of groups >= 1 are needed");
-  if (a->batch > 0x7fffffff || a->time > 0x7fffffff || a->channels > (1 << 24)) return fail(PPN_E_INVALID, "scan: a size is out of range");
+  if (a->batch > 0x7fffffff || a->time > 0x7fffffff || a->channels > (1 << 22)) return fail(PPN_E_INVALID, "scan: a size is out of range");
+  const int64_t strides[] = {a->x_time, a->dt_time, a->B_time, a->C_time, a->z_time, a->y_time, a->dy_time, a->dx_time, a->ddt_time, a->dz_time, a->groups * 128};
+  for (int64_t v : strides)
+    if (v < 0 || v > (1 << 27)) return fail(PPN_E_INVALID, "scan: rows of time may be at most 2^27 elements apart, got %lld", (long long)v);
   if (a->states < 1 || a->states > 64) return fail(PPN_E_INVALID, "states must be 1..64, got %lld", (long long)a->states);
   return PPN_OK;
 }
@@ -648,10 +731,12 @@ extern "C" int ppn_scan_forward(const ppn_scan_args* a, void* stream) {
     return by_states(a->states, [&](auto ns, auto lpc) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
       if (s.chunks > 1) {
-        scan_forward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, nullptr, ends, sums);
+        scan_forward<T, NS, LPC, SUMMARY><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, nullptr, ends, sums);
         scan_join<false><<<dim3(ceil_div(cells, 256)), dim3(256), 0, (hipStream_t)stream>>>(*a, s.chunks, ends, sums);
       }
-      scan_forward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, s.chunks > 1 ? ends : nullptr, nullptr, nullptr);
+      const float* entering = s.chunks > 1 ? ends : nullptr;
+      if (a->checkpoints) scan_forward<T, NS, LPC, TRAIN><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, entering, nullptr, nullptr);
+      else scan_forward<T, NS, LPC, OUTPUT><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, entering, nullptr, nullptr);
       return launched("ppn_scan_forward");
     });
   });
@@ -676,21 +761,21 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
   float* params = (float*)(w + p.rows_bytes);
   float* ends = (float*)(w + p.rows_bytes + p.params_bytes);
   float* sums = (float*)(w + p.rows_bytes + p.params_bytes + p.ends_bytes);
-  const int64_t tiles = a->groups * tiles_of(a), cells = a->batch * a->states * a->channels, count = a->batch * a->time * a->groups * 2 * a->states;
-  if (p.shares * tiles > 0x7fffffff || ceil_div(cells, 256) > 0x7fffffff || ceil_div(count, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many rows");
-  const dim3 grid(p.shares * tiles, p.split.chunks);
+  const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels, count = a->batch * a->time * a->groups * 2 * states_of(a);
+  if (waves > 0x7fffffff || ceil_div(cells, 256) > 0x7fffffff || ceil_div(count, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many rows");
+  const dim3 grid(waves, p.split.chunks);
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     return by_states(a->states, [&](auto ns, auto lpc) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
       const bool split = p.split.chunks > 1;
       if (split) {
-        scan_backward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, p.share, nullptr, ends, sums, nullptr, nullptr);
+        scan_backward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, nullptr, nullptr);
         scan_join<true><<<dim3(ceil_div(cells, 256)), dim3(256), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
       }
-      scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, p.share, split ? ends : nullptr, nullptr, nullptr, rows, params);
-      scan_reduce_rows<T><<<dim3(ceil_div(count, 256)), dim3(256), 0, (hipStream_t)stream>>>(rows, tiles_of(a), a->batch * a->time * a->groups, a->states, (T*)a->dB, (T*)a->dC);
-      scan_reduce_params<<<dim3(ceil_div((a->states + 2) * a->channels, 32)), dim3(256), 0, (hipStream_t)stream>>>(params, p.shares * p.split.chunks, a->states,
+      scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, split ? ends : nullptr, nullptr, nullptr, rows, params);
+      scan_reduce_rows<T, NS * LPC><<<dim3(ceil_div(count, 256)), dim3(256), 0, (hipStream_t)stream>>>(rows, tiles_of(a), a->batch * a->time * a->groups, a->states, (T*)a->dB, (T*)a->dC);
+      scan_reduce_params<<<dim3(ceil_div((a->states + 2) * a->channels, 32)), dim3(256), 0, (hipStream_t)stream>>>(params, a->batch * p.split.chunks, a->states,
                                                                                                                    a->channels, a->dA, a->dD, a->ddt_bias);
       return launched("ppn_scan_backward");
     });
