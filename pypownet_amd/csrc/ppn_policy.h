@@ -13,8 +13,6 @@ namespace ppn_policy {
 int fail(int code, const char* format, ...);
 int launched(const char* what);
 
-template <typename T> struct alignas(16) Pack { T v[16 / sizeof(T)]; };
-
 __device__ inline float to_float(float x) { return x; }
 __device__ inline float to_float(__bf16 x) { return (float)x; }
 __device__ inline float to_float(_Float16 x) { return (float)x; }

@@ -284,15 +284,13 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
     const unsigned now = starts_of(a, p.b, t, rows);
     px += ROWS * a.x_time, pdt += ROWS * a.dt_time, pz += ROWS * z_time, pB += ROWS * a.B_time, pC += ROWS * a.C_time;
     cut |= now != 0;
-    float delta[ROWS], w[ROWS], gate[ROWS], over[ROWS];
+    float delta[ROWS], gate[ROWS];
     step_sizes(dt, bias, soft, rows, delta);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      const float xv = to_float(x.v[j]);
-      w[j] = delta[j] * xv;
-      over[j] = skip * xv;
-      total += delta[j];
-      if constexpr (MODE != SUMMARY) {
+      if constexpr (MODE == SUMMARY) {
+        total += delta[j];
+      } else {
         const float zv = to_float(z.v[j]);
         gate[j] = gated ? zv * sigmoid(zv) : 1.0f;
       }
@@ -309,13 +307,14 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
       float bv[NS];
       const float step = anew(delta[j]);
       read_states<NS>(sb + j * STATES + p.part * NS, bv);
-      advance<NS>(h, h, step, w[j], A2, bv, (now >> j) & 1);
+      const float xv = widened(x.v[j]);
+      advance<NS>(h, h, step, step * xv, A2, bv, (now >> j) & 1);
       if constexpr (MODE != SUMMARY) {
         float cv[NS], s = 0.0f;
         read_states<NS>(sc + j * STATES + p.part * NS, cv);
 #pragma unroll
         for (int n = 0; n < NS; ++n) s += cv[n] * h[n];
-        at<T>(py, (unsigned)min(j, rows - 1) * y_step + p.d * (unsigned)sizeof(T)) = (T)((sum_parts<LPC>(s) + over[j]) * gate[j]);
+        at<T>(py, (unsigned)min(j, rows - 1) * y_step + p.d * (unsigned)sizeof(T)) = (T)((sum_parts<LPC>(s) + skip * xv) * gate[j]);
       }
     }
     py += ROWS * a.y_time;
@@ -331,8 +330,8 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
 
 // What enters each chunk, in place of what leaves it (forward: chunk k from k - 1; BACKWARD: adjoints, chunk k from k + 1).
 template <bool BACKWARD>
-__global__ void __launch_bounds__(256) scan_join(ppn_scan_args a, int64_t chunks, float* ends, const float* sums) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, per = a.states * a.channels;
+__global__ void __launch_bounds__(64) scan_join(ppn_scan_args a, int64_t chunks, float* ends, const float* sums) {
+  const int64_t id = (int64_t)blockIdx.x * 64 + threadIdx.x, per = a.states * a.channels;
   if (id >= a.batch * per) return;
   const int64_t b = id / per, rest = id - b * per, n = rest / a.channels, d = rest - n * a.channels;
   const float A2 = a.A[d * a.states + n] * LOG2E;
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(256) scan_join(ppn_scan_args a, int64_t chunks
   float h = outside ? outside[(b * a.channels + d) * a.states + n] : 0.0f;
   float* p = ends + b * chunks * per + rest;
   const float* s = sums + b * chunks * 2 * a.channels + d;
-  constexpr int AHEAD = 32;
+  constexpr int AHEAD = 16;
   for (int64_t i0 = 0; i0 < chunks; i0 += AHEAD) {
     float own[AHEAD], total[AHEAD], cut[AHEAD];
 #pragma unroll
@@ -722,7 +721,7 @@ extern "C" int ppn_scan_forward(const ppn_scan_args* a, void* stream) {
   const Split s = forward_split(a);
   if (a->workspace_bytes < ppn_scan_forward_workspace(a) || (s.chunks > 1 && !a->workspace)) return fail(PPN_E_INVALID, "ppn_scan_forward: the workspace is too small");
   const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels;
-  if (waves > 0x7fffffff || ceil_div(cells, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many channels of too many environments");
+  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many channels of too many environments");
   const dim3 grid(waves, s.chunks);
   float* ends = (float*)a->workspace;
   float* sums = ends + cells * s.chunks;
@@ -732,7 +731,7 @@ extern "C" int ppn_scan_forward(const ppn_scan_args* a, void* stream) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
       if (s.chunks > 1) {
         scan_forward<T, NS, LPC, SUMMARY><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, nullptr, ends, sums);
-        scan_join<false><<<dim3(ceil_div(cells, 256)), dim3(256), 0, (hipStream_t)stream>>>(*a, s.chunks, ends, sums);
+        scan_join<false><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunks, ends, sums);
       }
       const float* entering = s.chunks > 1 ? ends : nullptr;
       if (a->checkpoints) scan_forward<T, NS, LPC, TRAIN><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, entering, nullptr, nullptr);
@@ -762,7 +761,7 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
   float* ends = (float*)(w + p.rows_bytes + p.params_bytes);
   float* sums = (float*)(w + p.rows_bytes + p.params_bytes + p.ends_bytes);
   const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels, count = a->batch * a->time * a->groups * 2 * states_of(a);
-  if (waves > 0x7fffffff || ceil_div(cells, 256) > 0x7fffffff || ceil_div(count, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many rows");
+  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff || ceil_div(count, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many rows");
   const dim3 grid(waves, p.split.chunks);
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
@@ -771,7 +770,7 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
       const bool split = p.split.chunks > 1;
       if (split) {
         scan_backward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, nullptr, nullptr);
-        scan_join<true><<<dim3(ceil_div(cells, 256)), dim3(256), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
+        scan_join<true><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
       }
       scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, split ? ends : nullptr, nullptr, nullptr, rows, params);
       scan_reduce_rows<T, NS * LPC><<<dim3(ceil_div(count, 256)), dim3(256), 0, (hipStream_t)stream>>>(rows, tiles_of(a), a->batch * a->time * a->groups, a->states, (T*)a->dB, (T*)a->dC);
