@@ -326,41 +326,32 @@ __global__ void __launch_bounds__(256) conv_reduce(const float* partial, int64_t
 
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_step(ppn_conv_step_args a) {
-  const int64_t row = blockIdx.x, lanes = a.channels / VEC;
-  const int64_t cv = (int64_t)blockIdx.y * 256 + threadIdx.x;
-  const int64_t d = cv * VEC;
-  const int state = row_state(a.env_ids, row, a.environments);
-  if (cv >= lanes) return;
+  const int64_t row = blockIdx.x, lanes = a.channels / VEC, cv = (int64_t)blockIdx.y * 256 + threadIdx.x, d = (cv < lanes ? cv : lanes - 1) * VEC;
+  T* window = (T*)a.state + row_env(a.env_ids, row, a.environments) * (K - 1) * a.channels + d;
   T* y = (T*)a.y + row * a.y_row + d;
-  float out[VEC];
-  if (state != ROW_LIVE) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = state == ROW_PADDING ? 0.0f : __builtin_nanf("");
-    store_row<T, VEC>(y, out);
-    return;
-  }
-  const int64_t env = a.env_ids ? a.env_ids[row] : row;
-  T* window = (T*)a.state + env * (K - 1) * a.channels + d;
-  float w[K][VEC], c[VEC], rows[K][VEC];
+  float w[K][VEC], c[VEC], rows[K][VEC], out[VEC];
   const bool begins = a.starts && a.starts[row];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) {
-    load_row<T, VEC>(window + k * a.channels, rows[k]);
-    if (begins) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) rows[k][i] = 0.0f;
-    }
-  }
+  for (int k = 0; k < K - 1; ++k) load_row<T, VEC>(window + k * a.channels, rows[k]);
   load_row<T, VEC>((const T*)a.x + row * a.x_row + d, rows[K - 1]);
   load_weights<K, VEC>(a.weight, a.bias, d, w, c);
+  const int live = row_state(a.env_ids, row, a.environments);      // (the loads are under way while the ids are compared)
+  if (cv >= lanes) return;
+  if (begins) {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) rows[k][i] = 0.0f;
+  }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     float s = c[i] + w[K - 1][i] * rows[K - 1][i];           // (conv_forward's order: a window read row by row gives the same bits)
 #pragma unroll
     for (int k = K - 2; k >= 0; --k) s += w[k][i] * rows[k][i];
-    out[i] = a.silu ? s * sigmoid(s) : s;
+    out[i] = live == ROW_LIVE ? (a.silu ? s * sigmoid(s) : s) : live == ROW_PADDING ? 0.0f : __builtin_nanf("");
   }
   store_row<T, VEC>(y, out);
+  if (live != ROW_LIVE) return;
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) store_row<T, VEC>(window + k * a.channels, rows[k + 1]);
 }
@@ -495,7 +486,7 @@ extern "C" int ppn_conv_step(const ppn_conv_step_args* a, void* stream) {
     return fail(PPN_E_INVALID, "ppn_conv_step: a size is out of range");
   if (!a->env_ids && a->rows > a->environments) return fail(PPN_E_INVALID, "ppn_conv_step: more rows than environments and no env_ids");
   if (a->rows == 0) return PPN_OK;
-  if (!a->x || !a->weight || !a->y || (!a->state && a->environments)) return fail(PPN_E_INVALID, "ppn_conv_step: x, weight, state and y are needed");
+  if (!a->x || !a->weight || !a->y || !a->state || !a->environments) return fail(PPN_E_INVALID, "ppn_conv_step: x, weight, state (of one environment at least) and y are needed");
   const int64_t vec = WIDE, bytes = WIDE * size_of(a->type);
   const bool w = a->channels % vec == 0 && a->x_row % vec == 0 && a->y_row % vec == 0 && aligned(a->x, bytes) && aligned(a->y, bytes) && aligned(a->state, bytes);
   return by_type(a->type, [&](auto* t) {

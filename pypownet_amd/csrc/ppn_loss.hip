@@ -45,7 +45,7 @@ struct Operands {
 
 struct StatsArgs { const int32_t* allowed; int64_t allowed_row; float2* partial; int64_t columns; };
 struct GradArgs {
-  const int32_t* allowed; int64_t allowed_row; const int64_t* target; const float* lse; const float* dloss; const float* scale;
+  const int32_t* allowed; int64_t allowed_row; const int64_t* target; const float* lse; const float* loss; const float* dloss; const float* scale;
   void* dl; int64_t dl_row; void* dlt; int64_t dlt_row; int64_t first, rows_padded, cols_padded;
 };
 struct SumArgs { float* sums; bool add; };
@@ -136,24 +136,45 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
   __device__ int col_of(int j) const { return wave_n + j * 16 + (lane & 15); }
 };
 
-// Tiles are handed to the eight dies in turn, each with its own L2: neighbours in the list below go to one die, all row tiles of a
-// column tile one after the other, so that a die reads its share of the larger operand once.
-__device__ inline unsigned tile_of(unsigned id, unsigned count) {
-  const unsigned per = count / 8, whole = per * 8;
-  return id < whole ? (id % 8) * per + id / 8 : id;
+// Which tile a workgroup takes.  Workgroups are handed to the eight dies in turn, each with its own 4 MB of L2: neighbours in the list below go to
+// one die, and the list goes through eight tiles of rows (2 MB at 256 rows of 512 16-bit features) for every tile of columns, so that a die
+// keeps its rows and reads the columns once.  In the order of the rows alone 16384 x 24129 x 512 read 1.8 GB instead of 0.2.
+__device__ inline void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned* m, unsigned* n) {
+  const unsigned count = tiles_m * tiles_n, per = count / 8, whole = per * 8, tile = id < whole ? (id % 8) * per + id / 8 : id;
+  const unsigned group = tile / (8 * tiles_n), first = group * 8, rows = tiles_m - first < 8 ? tiles_m - first : 8, rest = tile - first * tiles_n;
+  *m = first + rest % rows;
+  *n = rest / rows;
 }
 
-template <int PATTERN> __device__ inline float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
+// The 16 lanes of a row of lanes hold one row's columns: their maximum, or sum, for four rows at once.  Written out because the compiler puts a
+// quieting instruction and a separate move in front of every maximum.  A lane exchange may follow the write of what it reads by two other
+// instructions: two idle ones in front, the other three rows' in between.
+#define PPN_OVER_16(OP)                                                                                                                       \
+  "s_nop 1\n"                                                                                                                                 \
+  OP " %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n" OP " %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf\n"                             \
+  OP " %2, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xf\n" OP " %3, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xf\n"                             \
+  OP " %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n" OP " %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n"                 \
+  OP " %2, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n" OP " %3, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xf\n"                 \
+  OP " %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n" OP " %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"         \
+  OP " %2, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n" OP " %3, %3, %3 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"         \
+  OP " %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n" OP " %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"         \
+  OP " %2, %2, %2 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n" OP " %3, %3, %3 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+__device__ inline void max_over_16(float (&v)[4]) { asm volatile(PPN_OVER_16("v_max_f32_dpp") : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])); }
+__device__ inline void sum_over_16(float (&v)[4]) { asm volatile(PPN_OVER_16("v_add_f32_dpp") : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])); }
+#undef PPN_OVER_16
+// Plain minimum and maximum, the same way (arguments are results of ordinary instructions, never of a matrix instruction: those need waits of their own).
+__device__ inline float least(float a, float b) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
-template <typename F> __device__ inline float over_16(float v, F f) {      // over the 16 lanes of a row of lanes
-  v = f(v, dpp<0x128>(v));      // row_ror:8
-  v = f(v, dpp<0x141>(v));      // row_half_mirror
-  v = f(v, dpp<0x4e>(v));       // quad_perm 2,3,0,1
-  return f(v, dpp<0xb1>(v));    // quad_perm 1,0,3,2
+__device__ inline float most(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 
-// The bits of BN columns from n0 (of N, whose word 0 is `word` words into a row of allowed) that row `row` may count: nothing past the last
+// The bits of BN columns from n0 (of N, whose word 0 is `word` words into a row of allowed) that row `row` may NOT count: every one past the last
 // column.  Called before the product, so that the loads' way is covered by it; read after it.
 template <int BN> __device__ inline void stage_mask(unsigned (*mask)[BN / 32], int at, const int32_t* allowed, int64_t allowed_row, int64_t row, int64_t word, int64_t n0, int64_t N,
                                                     bool live) {
@@ -163,82 +184,112 @@ template <int BN> __device__ inline void stage_mask(unsigned (*mask)[BN / 32], i
     unsigned bits = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
     if (!live) bits = 0;
     if (allowed && bits) bits &= (unsigned)allowed[row * allowed_row + word + n0 / 32 + w];
-    mask[at][w] = bits;
+    mask[at][w] = ~bits;
   }
 }
 
-// Forward: of every row and every 16 NI columns the maximum and the sum of exp(l - maximum).
+// Forward: of every row and every 16 NI columns the maximum and the sum of exp(l - maximum), [columns / 16 NI x rows].  Logarithms to base 2.
 template <typename T, int MI, int NI, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsArgs s, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
   __shared__ __align__(16) char lds[P::LDS_BYTES];
   __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
-  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
-  const int64_t m0 = (int64_t)(tile % tiles_m) * P::BM, n0 = (int64_t)(tile / tiles_m) * P::BN;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN;
   for (int r = threadIdx.x; r < P::BM; r += P::THREADS)
     stage_mask<P::BN>(mask, r, s.allowed, s.allowed_row, m0 + r < o.M ? m0 + r : o.M - 1, 0, n0, o.N, true);
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
-  const unsigned bit = 1u << (p.lane & 15);
-  float2* out = s.partial + m0 * s.columns + (n0 + p.wave_n) / (16 * NI);
+  const int column = p.lane & 15, low = 31 - column, high = 15 - column;      // left shifts that bring this lane's bit of a word's half to the top
+  float2* out = s.partial + (n0 + p.wave_n) / (16 * NI) * o.M + m0;
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < MI; ++i) {
+    float l[4][NI], top[4], sum[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = p.row_of(i, r);
-      float l[NI], top = -INFINITY, sum = 0.0f;
+      const unsigned* word = mask[p.row_of(i, r)] + p.wave_n / 32;
+      top[r] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const unsigned word = mask[row][p.wave_n / 32 + j / 2];
-        l[j] = word & (j & 1 ? bit << 16 : bit) ? p.c[i][j][r] : -INFINITY;
-        top = fmaxf(top, l[j]);      // (drops a NaN; the sum below does not)
+        // +infinity, or -infinity where the (inverted) bit says no: the sign bit on the pattern of infinity.  A NaN becomes +infinity here, and the sum NaN.
+        const unsigned limit = ((word[j / 2] << (j & 1 ? high : low)) & 0x80000000u) | 0x7f800000u;
+        l[r][j] = least(p.c[i][j][r] * LOG2E, __builtin_bit_cast(float, limit));
+        top[r] = most(top[r], l[r][j]);
       }
-      top = over_16(top, [](float a, float b) { return fmaxf(a, b); });
-      const float ref = top == -INFINITY ? 0.0f : top * LOG2E;
-#pragma unroll
-      for (int j = 0; j < NI; ++j) sum += __builtin_amdgcn_exp2f(l[j] * LOG2E - ref);
-      sum = over_16(sum, [](float a, float b) { return a + b; });
-      if ((p.lane & 15) == 0 && m0 + row < o.M) out[(unsigned)(row * (unsigned)s.columns)] = make_float2(top, sum);
     }
+    max_over_16(top);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float ref = top[r] == -INFINITY ? 0.0f : top[r];
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sum[r] += __builtin_amdgcn_exp2f(l[r][j] - ref);
+    }
+    sum_over_16(sum);
+    // lanes 0..3 of each 16 have a row to write
+    const float t = column & 2 ? (column & 1 ? top[3] : top[2]) : (column & 1 ? top[1] : top[0]);
+    const float u = column & 2 ? (column & 1 ? sum[3] : sum[2]) : (column & 1 ? sum[1] : sum[0]);
+    const int row = p.row_of(i, column);
+    if (column < 4 && m0 + row < o.M) out[row] = make_float2(t, u);
+  }
 }
 
-// One wave a row: joins the tiles' maxima and sums, and takes the target's logit as a product of its own.
+// Sixteen rows a workgroup: joins the tiles' maxima and sums, 16 lanes a row, and takes the target's logit as a product of its own, a wave a row.
 template <typename T>
 __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* partial, int64_t columns) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const int lane = threadIdx.x & 63;
-  if (row >= a.rows) return;
-  const int64_t at = a.target[row];
-  const bool inside = at >= 0 && at < a.actions;
-  float wanted = 0.0f;
-  if (inside) {
-    const T* h = (const T*)a.hidden + row * a.hidden_row;
-    const T* w = (const T*)a.weight + at * a.weight_row;
-    for (int64_t f = lane; f < a.features; f += 64) wanted += to_float(h[f]) * to_float(w[f]);
+  __shared__ float tops[16][17], sums[16][17], wanted[16];
+  const int64_t first = (int64_t)blockIdx.x * 16;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+  {
+    const int64_t row = first + (threadIdx.x & 15) < a.rows ? first + (threadIdx.x & 15) : a.rows - 1;
+    float top = -INFINITY, sum = 0.0f;
+    // (a tile without an allowed action has the sum 0 and the maximum -infinity; one with a NaN has the sum NaN whatever its maximum)
+    constexpr int AHEAD = 4;
+    for (int64_t c = threadIdx.x / 16; c < columns; c += 16 * AHEAD) {
+      float2 v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t at = c + 16 * k;
+        v[k] = partial[(at < columns ? at : c) * a.rows + row];
+        if (at >= columns) v[k] = make_float2(-INFINITY, 0.0f);
+      }
+      float high = top;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) high = fmaxf(high, v[k].x);
+      const float ref = high == -INFINITY ? 0.0f : high;
+      sum *= __builtin_amdgcn_exp2f(top - ref);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) sum += v[k].y * __builtin_amdgcn_exp2f(v[k].x - ref);
+      top = high;
+    }
+    tops[threadIdx.x & 15][threadIdx.x / 16] = top;
+    sums[threadIdx.x & 15][threadIdx.x / 16] = sum;
   }
+  for (int r = wave; r < 16; r += 4) {
+    const int64_t row = first + r, at = row < a.rows ? a.target[row] : -1;
+    float s = 0.0f;
+    if (at >= 0 && at < a.actions) {
+      const T* h = (const T*)a.hidden + row * a.hidden_row;
+      const T* w = (const T*)a.weight + at * a.weight_row;
+      for (int64_t f = lane; f < a.features; f += 64) s += to_float(h[f]) * to_float(w[f]);
+    }
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if (lane == 0) wanted[r] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16 || first + threadIdx.x >= a.rows) return;
+  const int64_t row = first + threadIdx.x, at = a.target[row];
   float top = -INFINITY, sum = 0.0f;
-  // (a tile without an allowed action has the sum 0 and the maximum -infinity; one with a NaN has the sum NaN whatever its maximum)
-  auto join = [&](float t, float s) {
-    const float high = fmaxf(top, t), ref = high == -INFINITY ? 0.0f : high;
-    sum = sum * exp_fast(top - ref) + s * exp_fast(t - ref);
-    top = high;
-  };
-  for (int64_t c = lane; c < columns; c += 64) {
-    const float2 v = partial[row * columns + c];
-    join(v.x, v.y);
-  }
-  for (int d = 32; d; d >>= 1) {
-    wanted += __shfl_xor(wanted, d);
-    const float t = __shfl_xor(top, d), s = __shfl_xor(sum, d);
-    join(t, s);
-  }
-  if (lane) return;
-  const bool nothing = top == -INFINITY && sum == 0.0f;
-  const float whole = top + 0.693147180559945309f * __builtin_amdgcn_logf(sum);
+  for (int k = 0; k < 16; ++k) top = fmaxf(top, tops[threadIdx.x][k]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  for (int k = 0; k < 16; ++k) sum += sums[threadIdx.x][k] * __builtin_amdgcn_exp2f(tops[threadIdx.x][k] - ref);
+  const bool nothing = top == -INFINITY && sum == 0.0f, inside = at >= 0 && at < a.actions;
+  const float whole = 0.693147180559945309f * (top + __builtin_amdgcn_logf(sum));
   float loss = 0.0f, lse = INFINITY;
   if (at != a.ignore_index && !nothing) {
     const bool legal = inside && (!a.allowed || ((a.allowed[row * a.allowed_row + (at >> 5)] >> (at & 31)) & 1));
-    loss = !inside ? NAN : legal ? whole - wanted : INFINITY;
+    loss = !inside ? NAN : legal ? whole - wanted[threadIdx.x] : INFINITY;
     lse = !inside || whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
   }
   a.loss[row] = loss;
@@ -266,53 +317,95 @@ __global__ void __launch_bounds__(256) loss_scale(const float* dloss, const floa
   }
 }
 
+// Two rows' (of a lane's column) values as one word, and the exchange that turns four rows of one column into two rows of two columns: lanes of
+// even columns keep the first two rows, those of odd ones the last two.
+__device__ inline unsigned pair(__bf16 a, __bf16 b) { return (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16; }
+__device__ inline unsigned pair(_Float16 a, _Float16 b) { return (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16; }
+__device__ inline unsigned from_neighbour(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true); }      // quad_perm 1,0,3,2
+
 // Backward, first product: dl of the columns first .. first + N of the catalogue, [rows x cols_padded] and [N x rows_padded], zeros in the padding.
+// The target's own entry, (e^-loss - 1) dloss, is written over its tile's value at the end.
 template <typename T, int MI, int NI, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArgs g, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
-  struct Row { float lse2, up; int target, unused; };
+  struct Row { float lse2, up; };
   __shared__ __align__(16) char lds[P::LDS_BYTES];
   __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
   __shared__ __align__(16) Row rows[P::BM];
-  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
-  const int64_t m0 = (int64_t)(tile % tiles_m) * P::BM, n0 = (int64_t)(tile / tiles_m) * P::BN;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN;
   for (int r = threadIdx.x; r < P::BM; r += P::THREADS) {
-    const int64_t row = m0 + r < o.M ? m0 + r : o.M - 1, target = g.target[row] - g.first - n0;
+    const int64_t row = m0 + r < o.M ? m0 + r : o.M - 1;
     const float lse = g.lse[row];
     const bool live = m0 + r < o.M && lse != INFINITY;                   // a row without a gradient, or past the last one: zeros
     stage_mask<P::BN>(mask, r, g.allowed, g.allowed_row, row, g.first / 32, n0, o.N, live);
-    rows[r] = Row{lse * LOG2E, live ? g.dloss[row] * g.scale[0] : 0.0f, target >= 0 && target < P::BN ? (int)target : -1, 0};
+    rows[r] = Row{lse * LOG2E, live ? g.dloss[row] * g.scale[0] : 0.0f};
   }
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
-  const unsigned bit = 1u << (p.lane & 15);
-  const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
+  const int column = p.lane & 15;
   T* dl = (T*)g.dl + m0 * g.dl_row + n0;
   T* dlt = (T*)g.dlt + n0 * g.dlt_row + m0;
-  const unsigned dl_row = (unsigned)g.dl_row, dlt_row = (unsigned)g.dlt_row;
+  const unsigned dl_row = (unsigned)g.dl_row * sizeof(T), dlt_row = (unsigned)g.dlt_row * sizeof(T);
+  auto write = [&](auto flag) {
+    constexpr bool EDGE = decltype(flag)::value;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    T out[NI][4];
+    for (int i = 0; i < MI; ++i) {
+      T out[NI][4];
+      const int row0 = p.row_of(i, 0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = p.row_of(i, r);
-      const Row q = rows[row];
+      for (int r = 0; r < 4; ++r) {
+        const Row q = rows[row0 + r];
+        const unsigned* word = mask[row0 + r] + p.wave_n / 32;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const float v = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2) * q.up;
+          const int no = (int)(word[j / 2] << (j & 1 ? 15 - column : 31 - column)) >> 31;      // all ones where the action is not allowed
+          out[j][r] = (T)__builtin_bit_cast(float, __builtin_bit_cast(int, v) & ~no);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const unsigned word = mask[row][p.wave_n / 32 + j / 2];
-        const float e = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2);
-        const float v = (e - (p.col_of(j) == q.target ? 1.0f : 0.0f)) * q.up;
-        out[j][r] = (T)(word & (j & 1 ? bit << 16 : bit) ? v : 0.0f);
-        if (whole || (m0 + row < o.M && n0 + p.col_of(j) < g.cols_padded)) dl[row * dl_row + p.col_of(j)] = out[j][r];
+        const int col = p.col_of(j);
+        if (!EDGE || (n0 + col < o.N && m0 + row0 < g.rows_padded)) {      // rows_padded is a multiple of 16: the four rows are in or out together
+          struct alignas(4 * sizeof(T)) Quad { T v[4]; } f = {{out[j][0], out[j][1], out[j][2], out[j][3]}};
+          *(Quad*)((char*)dlt + (col * dlt_row + row0 * (unsigned)sizeof(T))) = f;
+        }
+        if constexpr (sizeof(T) == 2) {
+          const unsigned a = pair(out[j][0], out[j][1]), b = pair(out[j][2], out[j][3]);
+          const bool odd = column & 1;
+          const unsigned keep = odd ? b : a, got = from_neighbour(odd ? a : b);
+          const unsigned left = odd ? got : keep, right = odd ? keep : got;      // columns col & ~1 and the next, two rows each
+          const unsigned lower = __builtin_amdgcn_perm(right, left, 0x05040100), upper = __builtin_amdgcn_perm(right, left, 0x07060302);
+          const int row = row0 + (odd ? 2 : 0);
+          char* at = (char*)dl + (row * dl_row + (col & ~1) * 2u);
+          const bool in = !EDGE || n0 + col < g.cols_padded;
+          if (in && (!EDGE || m0 + row < o.M)) *(unsigned*)at = lower;
+          if (in && (!EDGE || m0 + row + 1 < o.M)) *(unsigned*)(at + dl_row) = upper;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!EDGE || (m0 + row0 + r < o.M && n0 + col < g.cols_padded)) *(T*)((char*)dl + ((row0 + r) * dl_row + col * (unsigned)sizeof(T))) = out[j][r];
+        }
       }
     }
-    const int row = p.row_of(i, 0);
-#pragma unroll
-    for (int j = 0; j < NI; ++j)
-      if (whole || (n0 + p.col_of(j) < o.N && m0 + row < g.rows_padded)) {      // rows_padded is a multiple of 16: the four rows are in or out together
-        struct alignas(4 * sizeof(T)) Four { T v[4]; } f = {{out[j][0], out[j][1], out[j][2], out[j][3]}};
-        *(Four*)(dlt + p.col_of(j) * dlt_row + row) = f;
-      }
+  };
+  if (m0 + P::BM <= o.M && n0 + P::BN <= o.N) write(std::false_type());
+  else write(std::true_type());
+  // the targets' entries, behind the tile's own stores
+  __threadfence_block();
+  __syncthreads();
+  for (int r = threadIdx.x; r < P::BM; r += P::THREADS) {
+    if (m0 + r >= o.M) break;
+    const int64_t target = g.target[m0 + r] - g.first - n0;
+    if (target < 0 || target >= P::BN || n0 + target >= o.N || g.lse[m0 + r] == INFINITY) continue;
+    const int t = (int)target;
+    if ((mask[r][t / 32] >> (t & 31)) & 1) continue;
+    const float loss = g.loss[m0 + r];
+    const T v = (T)((loss != loss ? loss : expm1f(-loss)) * rows[r].up);
+    *(T*)((char*)dl + (r * dl_row + t * (unsigned)sizeof(T))) = v;
+    *(T*)((char*)dlt + (t * dlt_row + r * (unsigned)sizeof(T))) = v;
   }
 }
 
@@ -321,8 +414,9 @@ template <typename T, int MI, int NI, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(Operands o, SumArgs s, int64_t share, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
   __shared__ __align__(16) char lds[P::LDS_BYTES];
-  const unsigned tile = tile_of(blockIdx.x, tiles_m * tiles_n);
-  const int64_t n0 = (int64_t)(tile % tiles_n) * P::BN, m0 = (int64_t)(tile / tiles_n) * P::BM;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN;
   const int64_t k0 = blockIdx.y * share, k1 = k0 + share < o.K ? k0 + share : o.K;
   P p;
   p.run(o, lds, m0, n0, k0, k1);
@@ -440,8 +534,9 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   p.features_padded = padded(a->features, unit);
   p.rows_padded = padded(a->rows, 32);
   p.actions_padded = padded(a->actions, 32);
-  // a piece's dl and its transpose take 64 MB each: both stay in the last-level cache between the kernel that writes and those that read them
-  p.piece = padded((int64_t)(64 << 20) / (p.rows_padded * size), 128);
+  // A piece's dl and its transpose take 256 MB each.  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
+  // of dweight's: 16384 rows of 24129 actions take 3.65, 3.02, 2.71, 2.44 and 2.33 ms behind the loss at 32, 64, 128, 256 and 512 MB.
+  p.piece = padded((int64_t)(256 << 20) / (p.rows_padded * size), 128);
   if (p.piece < 1024) p.piece = 1024;
   if (p.piece > p.actions_padded) p.piece = p.actions_padded;
   p.grad = config_for(a->rows, p.piece, 1);
@@ -512,7 +607,7 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
     if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
     if (p.config.large) loss_stats<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
     else loss_stats<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
-    loss_join<T><<<dim3(ceil_div(a->rows, 4)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
+    loss_join<T><<<dim3(ceil_div(a->rows, 16)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
     return launched("ppn_loss_forward");
   });
 }
@@ -525,7 +620,8 @@ extern "C" int64_t ppn_loss_backward_workspace(const ppn_loss_args* a) {
 extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
   if (int rc = check(a)) return rc;
   if (a->rows == 0) return fail(PPN_E_INVALID, "ppn_loss_backward: there are no rows");
-  if (!a->hidden || !a->weight || !a->target || !a->lse || !a->dloss) return fail(PPN_E_INVALID, "ppn_loss_backward: hidden, weight, target, lse and dloss are needed");
+  if (!a->hidden || !a->weight || !a->target || !a->loss || !a->lse || !a->dloss)
+    return fail(PPN_E_INVALID, "ppn_loss_backward: hidden, weight, target, loss, lse and dloss are needed");
   if (a->allowed && a->allowed_row < ceil_div(a->actions, 32)) return fail(PPN_E_INVALID, "ppn_loss_backward: a row of allowed has too few words");
   const BackwardPlan p = plan_backward(a);
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_backward: the workspace is too small");
@@ -555,7 +651,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
     for (int64_t first = 0; first < a->actions; first += p.piece) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 32);
       const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
-      const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
+      const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->loss, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
       const int64_t tm = ceil_div(a->rows, p.grad.bm), tn = ceil_div(n, p.grad.bn);
       if (p.grad.large) loss_grad<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);
       else loss_grad<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);

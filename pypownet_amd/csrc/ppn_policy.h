@@ -36,14 +36,28 @@ __device__ inline float softplus(float v) {
 // Which environment's state a row of a step call may touch: read by every workgroup of the row, so that all decide alike.  A row whose
 // id an earlier row has (or that is out of range) must not move the state on a second time: it is refused with NaN.  The ids in front of
 // the row are compared one a lane; at 4096 rows that is 8 KB a workgroup on average, out of the L2.
+// A caller may read the state before it knows (row_env has checked the range); it may not write it.
 enum { ROW_LIVE = 0, ROW_PADDING = 1, ROW_REFUSED = 2 };
+__device__ inline int64_t row_env(const int32_t* env_ids, int64_t row, int64_t environments) {      // an environment that exists, the row's if it is live
+  const int64_t id = env_ids ? env_ids[row] : row;
+  return id >= 0 && id < environments ? id : 0;
+}
 __device__ inline int row_state(const int32_t* env_ids, int64_t row, int64_t environments) {
   if (!env_ids) return ROW_LIVE;
   const int32_t id = env_ids[row];
   if (id < 0) return ROW_PADDING;
   if (id >= environments) return ROW_REFUSED;
   bool met = false;
-  for (int64_t i = threadIdx.x; i < row; i += blockDim.x) met |= env_ids[i] == id;
+  for (int64_t i = threadIdx.x; i < row; i += 4 * (int64_t)blockDim.x) {
+    int32_t other[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = i + k * (int64_t)blockDim.x;
+      other[k] = env_ids[at < row ? at : i];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) met |= other[k] == id;
+  }
   return __syncthreads_or(met) ? ROW_REFUSED : ROW_LIVE;
 }
 

@@ -575,65 +575,85 @@ template <int LPC> __device__ inline float sum_neighbours(float v) {
   return v;
 }
 
-template <typename T, int LPC, bool WIDE>
+template <typename T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+
+// WIDE: four states (and four of B and C) are one load.  AHEAD channels of a lane are loaded together, and the first of them before the ids
+// are compared.
+template <typename T, int LPC, bool WIDE, int AHEAD>
 __global__ void __launch_bounds__(256) scan_step(ppn_scan_step_args a) {
-  const int64_t row = blockIdx.x;
-  const int state = row_state(a.env_ids, row, a.environments);
-  const int part = threadIdx.x % LPC, n0 = part * 4;
-  const int64_t wide = a.channels / a.groups;
-  const int64_t env = a.env_ids && state == ROW_LIVE ? a.env_ids[row] : row;
-  const bool begins = a.starts && a.starts[row];
-  for (int64_t d0 = (int64_t)blockIdx.y * (256 / LPC); d0 < a.channels; d0 += (int64_t)gridDim.y * (256 / LPC)) {
-    const int64_t d = d0 + threadIdx.x / LPC;
-    const bool live = d < a.channels;
-    T* y = (T*)a.y + row * a.y_row + d;
-    if (state != ROW_LIVE) {
-      if (live && part == 0) *y = (T)(state == ROW_PADDING ? 0.0f : __builtin_nanf(""));
-      continue;
-    }
-    float s = 0.0f, xv = 0.0f, zv = 0.0f;
-    if (live) {
-      const int64_t g = d / wide;
-      float* hp = a.state + (env * a.channels + d) * a.states + n0;
-      const float* ap = a.A + d * a.states + n0;
-      const T* bp = (const T*)a.B + row * a.B_row + g * a.B_group + n0;
-      const T* cp = (const T*)a.C + row * a.C_row + g * a.C_group + n0;
-      float h[4], A2[4], bv[4], cv[4];
-      if constexpr (WIDE) {
-        const bool in = n0 < a.states;
-        float4 h4 = in ? *(const float4*)hp : float4{0, 0, 0, 0}, a4 = in ? *(const float4*)ap : float4{0, 0, 0, 0};
-        h[0] = h4.x, h[1] = h4.y, h[2] = h4.z, h[3] = h4.w;
-        A2[0] = a4.x, A2[1] = a4.y, A2[2] = a4.z, A2[3] = a4.w;
-      }
+  constexpr int PER = 256 / LPC;        // channels a workgroup takes at a time, AHEAD times over
+  const int64_t row = blockIdx.x, env = row_env(a.env_ids, row, a.environments);
+  const int part = threadIdx.x % LPC, n0 = part * 4, states = (int)a.states, channels = (int)a.channels, wide = (int)(a.channels / a.groups);
+  const int last = min(n0, states - 1) & ~3;       // (a lane past the last state reads the last four)
+  const bool begins = a.starts && a.starts[row], gated = a.z != nullptr, soft = a.softplus;
+  const T* x = (const T*)a.x + row * a.x_row;
+  const T* dt = (const T*)a.dt + row * a.dt_row;
+  const T* z = gated ? (const T*)a.z + row * a.z_row : x;
+  const T* B = (const T*)a.B + row * a.B_row;
+  const T* C = (const T*)a.C + row * a.C_row;
+  T* y = (T*)a.y + row * a.y_row;
+  float* state = a.state + env * a.channels * a.states;
+  Four<float> h[AHEAD], A[AHEAD];
+  Four<T> b[AHEAD], c[AHEAD];
+  T rx[AHEAD], rdt[AHEAD], rz[AHEAD];
+  float bias[AHEAD], skip[AHEAD];
+  auto fetch = [&](int d0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = n0 + i < a.states;
-        if constexpr (!WIDE) h[i] = in ? hp[i] : 0.0f, A2[i] = in ? ap[i] : 0.0f;
-        bv[i] = in ? to_float(bp[i]) : 0.0f;
-        cv[i] = in ? to_float(cp[i]) : 0.0f;
-      }
-      xv = to_float(((const T*)a.x)[row * a.x_row + d]);
-      const float raw = to_float(((const T*)a.dt)[row * a.dt_row + d]) + (a.dt_bias ? a.dt_bias[d] : 0.0f), delta = a.softplus ? softplus(raw) : raw;
-      if (a.z) zv = to_float(((const T*)a.z)[row * a.z_row + d]);
-      const float w = delta * xv;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[i] = begins ? w * bv[i] : __builtin_amdgcn_exp2f(delta * A2[i] * LOG2E) * h[i] + w * bv[i];
-        s += cv[i] * h[i];
-      }
+    for (int k = 0; k < AHEAD; ++k) {
+      const int d = min(d0 + k * PER + (int)threadIdx.x / LPC, channels - 1), g = d / wide;
       if constexpr (WIDE) {
-        if (n0 < a.states) *(float4*)hp = float4{h[0], h[1], h[2], h[3]};
+        h[k] = *(const Four<float>*)(state + (int64_t)d * states + last);
+        A[k] = *(const Four<float>*)(a.A + (int64_t)d * states + last);
+        b[k] = *(const Four<T>*)(B + g * a.B_group + last);
+        c[k] = *(const Four<T>*)(C + g * a.C_group + last);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n0 + i < a.states) hp[i] = h[i];
+        for (int i = 0; i < 4; ++i) {
+          const int n = min(n0 + i, states - 1);
+          h[k].v[i] = state[(int64_t)d * states + n];
+          A[k].v[i] = a.A[(int64_t)d * states + n];
+          b[k].v[i] = B[g * a.B_group + n];
+          c[k].v[i] = C[g * a.C_group + n];
+        }
       }
+      rx[k] = x[d];
+      rdt[k] = dt[d];
+      rz[k] = z[d];
+      bias[k] = a.dt_bias ? a.dt_bias[d] : 0.0f;
+      skip[k] = a.D ? a.D[d] : 0.0f;
     }
-    s = sum_neighbours<LPC>(s);
-    if (live && part == 0) {
-      if (a.D) s += a.D[d] * xv;
-      if (a.z) s *= zv * sigmoid(zv);
-      *y = (T)s;
+  };
+  const int first = blockIdx.y * PER * AHEAD, step = gridDim.y * PER * AHEAD;
+  fetch(first);
+  const int live = row_state(a.env_ids, row, a.environments);
+  for (int d0 = first; d0 < channels; d0 += step) {
+    if (d0 != first) fetch(d0);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int d = d0 + k * PER + (int)threadIdx.x / LPC;
+      const float xv = to_float(rx[k]), raw = to_float(rdt[k]) + bias[k], delta = soft ? softplus(raw) : raw, w = delta * xv;
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = n0 + i < states;
+        const float bv = in ? to_float(b[k].v[i]) : 0.0f, cv = in ? to_float(c[k].v[i]) : 0.0f;
+        h[k].v[i] = begins ? w * bv : __builtin_amdgcn_exp2f(delta * (A[k].v[i] * LOG2E)) * h[k].v[i] + w * bv;
+        s += in ? cv * h[k].v[i] : 0.0f;
+      }
+      s = sum_neighbours<LPC>(s);
+      if (live == ROW_LIVE && d < channels) {
+        if constexpr (WIDE) {
+          if (n0 < states) *(Four<float>*)(state + (int64_t)d * states + n0) = h[k];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n0 + i < states) state[(int64_t)d * states + n0 + i] = h[k].v[i];
+        }
+      }
+      if (part == 0 && d < channels) {
+        const float zv = to_float(rz[k]), gate = gated ? zv * sigmoid(zv) : 1.0f;
+        y[d] = (T)(live == ROW_LIVE ? (s + skip[k] * xv) * gate : live == ROW_PADDING ? 0.0f : __builtin_nanf(""));
+      }
     }
   }
 }
@@ -788,22 +808,28 @@ extern "C" int ppn_scan_step(const ppn_scan_step_args* a, void* stream) {
   if (a->states < 1 || a->states > 64) return fail(PPN_E_INVALID, "states must be 1..64, got %lld", (long long)a->states);
   if (!a->env_ids && a->rows > a->environments) return fail(PPN_E_INVALID, "ppn_scan_step: more rows than environments and no env_ids");
   if (a->rows == 0) return PPN_OK;
-  if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || (!a->state && a->environments)) return fail(PPN_E_INVALID, "ppn_scan_step: x, dt, A, B, C, state and y are needed");
-  const bool wide = a->states % 4 == 0 && aligned(a->state, 16) && aligned(a->A, 16);
+  if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || !a->state || !a->environments) return fail(PPN_E_INVALID, "ppn_scan_step: x, dt, A, B, C, state (of one environment at least) and y are needed");
+  const int64_t four = 4 * size_of(a->type);
+  const bool wide = a->states % 4 == 0 && aligned(a->state, 16) && aligned(a->A, 16) && aligned(a->B, four) && aligned(a->C, four) && a->B_row % 4 == 0 &&
+                    a->C_row % 4 == 0 && a->B_group % 4 == 0 && a->C_group % 4 == 0;
   int lpc = 1;
   while (lpc * 4 < a->states) lpc *= 2;
-  // a workgroup takes all channels of its row (the ids in front of it are compared once) unless there are too few rows to fill the chip
-  const int64_t slices = ceil_div(a->channels, 256 / lpc);
-  int64_t y = ceil_div(1024, a->rows);
-  if (y > slices) y = slices;
+  // Four channels a lane in flight and at most 4096 workgroups, so that a row's ids are compared by one or a few of them (4096 rows of 512 x 16
+  // states out of memory: 72 us, 76 with two workgroups a row); one channel a lane where that leaves less than one workgroup a CU.
+  const int64_t per = 256 / lpc;
+  const bool few = a->rows * ceil_div(a->channels, 4 * per) < 256;
+  int64_t y = ceil_div(a->channels, few ? per : 4 * per);
+  if (!few && a->rows * y > 4096) y = ceil_div(4096, a->rows);
   if (y > 65535) y = 65535;
   const dim3 grid(a->rows, y);
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     auto go = [&](auto l) {
       constexpr int LPC = decltype(l)::value;
-      if (wide) scan_step<T, LPC, true><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
-      else scan_step<T, LPC, false><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
+      if (wide && few) scan_step<T, LPC, true, 1><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
+      else if (wide) scan_step<T, LPC, true, 4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
+      else if (few) scan_step<T, LPC, false, 1><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
+      else scan_step<T, LPC, false, 4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
       return launched("ppn_scan_step");
     };
     switch (lpc) {

@@ -41,13 +41,22 @@ def _load():
 
 def _call(function, packed, device):
     """Queues one entry point on torch's current stream of `device`."""
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            rc = function(packed, torch.cuda.current_stream().cuda_stream)
+            rc = function(packed, _stream_of(index))
     else:
-        rc = function(packed, torch.cuda.current_stream().cuda_stream)
+        rc = function(packed, _stream_of(index))
     if rc != 0:
         _refused(rc)
+
+
+def _stream_of(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same number without a Stream object around it (a fifth of a short call)
+_stream_of = getattr(torch._C, '_cuda_getCurrentRawStream', _stream_of)
 
 
 def _refused(rc):
@@ -421,14 +430,14 @@ class _ActionCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, allowed, ignore):
         hidden, weight = _rows(hidden), _rows(weight)
         loss, lse = _loss_forward(hidden, weight, target, allowed, ignore)
-        ctx.save_for_backward(hidden, weight, target, allowed, lse)
+        ctx.save_for_backward(hidden, weight, target, allowed, loss, lse)
         ctx.ignore = ignore
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        hidden, weight, target, allowed, lse = ctx.saved_tensors
+        hidden, weight, target, allowed, loss, lse = ctx.saved_tensors
         dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if ctx.needs_input_grad[0] else None
         dweight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
         if hidden.shape[0] == 0:
@@ -436,7 +445,7 @@ class _ActionCrossEntropy(torch.autograd.Function):
         given = (hidden, weight, target, allowed, ctx.ignore)
         lib = _load()
         work = _workspace(lib.ppn_loss_backward_workspace(_loss_args(*given)), hidden.device)
-        _call(lib.ppn_loss_backward, _loss_args(*given, lse=lse, dloss=dloss.contiguous(), dhidden=dhidden, dweight=dweight, workspace=work), hidden.device)
+        _call(lib.ppn_loss_backward, _loss_args(*given, loss=loss, lse=lse, dloss=dloss.contiguous(), dhidden=dhidden, dweight=dweight, workspace=work), hidden.device)
         return dhidden, dweight, None, None, None
 
 
