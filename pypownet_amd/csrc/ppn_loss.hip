@@ -36,7 +36,7 @@ __device__ inline void multiply(f32x4& c, u32x4 a, u32x4 b, float) {
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
 }
 
-// Operands of one product: C[m, n] = sum_k A[m, k] B[n, k]; the inner dimension padded to whole 64-byte rows, rows 16-byte aligned.
+// Operands of one product: C[m, n] = sum_k A[m, k] B[n, k]; the inner dimension padded to whole lines, rows 16-byte aligned.
 struct Operands {
   const void* A; int64_t lda, M;
   const void* B; int64_t ldb, N;
@@ -50,24 +50,25 @@ struct GradArgs {
 };
 struct SumArgs { float* sums; bool add; };
 
-constexpr int LINE = 64;          // bytes of the inner dimension per step
+constexpr int LINE = 128;         // bytes of the inner dimension per stage: a cache line, so that none is brought twice
 
-// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go from memory straight into LDS, into one of three
-// buffers two steps ahead of the step that is multiplied; one barrier a step.  A line's four 16-byte parts are stored with
-// part ^ (row / 2 % 4), so that the 16 rows a fragment read touches fall into different banks; the transfer writes 64 lanes' 16 bytes in
-// a row (16 lines), so the exchange is made in the addresses it reads.
+// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go from memory straight into LDS, into one of two
+// buffers, one stage ahead; a stage is multiplied in two halves, and a half's fragments are read into registers during the half before it, so
+// the matrix units wait for neither.  One barrier a stage.  A line's eight 16-byte parts are stored with part ^ (row % 8), so that the
+// rows a fragment read touches fall into different banks; the transfer writes 64 lanes' 16 bytes in a row (8 lines), so the exchange is
+// made in the addresses it reads.
 template <typename T, int MI, int NI, int WM, int WN> struct Product {
   static constexpr int BM = 16 * MI * WM, BN = 16 * NI * WN, THREADS = 64 * WM * WN;
-  static constexpr int GROUPS = (BM + BN) / 16, LOADS = GROUPS / (WM * WN);      // transfers of 16 lines: in all, and per wave
-  static constexpr int STAGE = (BM + BN) * LINE, LDS_BYTES = 3 * STAGE;
-  static_assert(GROUPS % (WM * WN) == 0 && BM % 16 == 0, "");
+  static constexpr int GROUPS = (BM + BN) / 8, LOADS = GROUPS / (WM * WN);      // transfers of 8 lines: in all, and per wave
+  static constexpr int STAGE = (BM + BN) * LINE, LDS_BYTES = 2 * STAGE;
+  static_assert(GROUPS % (WM * WN) == 0 && BM % (8 * LOADS) == 0, "a wave's lines belong to one operand");
 
   f32x4 c[MI][NI];
   int wave_m, wave_n, lane;
 
-  __device__ static int spot(int row, int part) { return row * LINE + ((part ^ ((row >> 1) & 3)) << 4); }
+  __device__ static int spot(int row, int part) { return row * LINE + ((part ^ (row & 7)) << 4); }
 
-  // 16 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().
+  // 8 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().
   __device__ static void transfer(unsigned to, const char* base, unsigned offset) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
   }
@@ -86,49 +87,59 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) c[i][j] = f32x4{0, 0, 0, 0};
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    const char* base[LOADS];
-    unsigned offset[LOADS], to[LOADS];
+    // this wave's lines: 8 LOADS neighbouring ones of one operand; lines past the last one read the last one again
+    const int line0 = wave * LOADS * 8, row = lane >> 3;
+    const bool left = line0 < BM;
+    const int64_t first = left ? m0 + line0 : n0 + line0 - BM, rows = left ? o.M : o.N, ld = (left ? o.lda : o.ldb) * (int64_t)sizeof(T);
+    const int64_t top = first < rows ? first : rows - 1;
+    const int spare = (int)(rows - 1 - top < 8 * LOADS ? rows - 1 - top : 8 * LOADS);
+    const char* base = scalar((const char*)(left ? o.A : o.B) + top * ld + k0 * (int64_t)sizeof(T));
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + line0 * LINE);
+    unsigned offset[LOADS];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int group = wave * LOADS + i, row = lane >> 2, part = (lane & 3) ^ ((row >> 1) & 3);
-      const bool left = group * 16 < BM;
-      const int64_t first = left ? m0 + group * 16 : n0 + group * 16 - BM, rows = left ? o.M : o.N, ld = (left ? o.lda : o.ldb) * (int64_t)sizeof(T);
-      const int64_t top = first < rows ? first : rows - 1, spare = rows - 1 - top;             // lines past the last one read the last one again
-      base[i] = scalar((const char*)(left ? o.A : o.B) + top * ld + k0 * (int64_t)sizeof(T));
-      offset[i] = (unsigned)((row < spare ? row : spare) * ld) + part * 16;
-      to[i] = lds0 + group * 16 * LINE;
-    }
-    const int steps = (int)((k1 - k0) * (int64_t)sizeof(T) / LINE);
-    int filled = 0;                                                    // buffer the next transfers go to
-    auto fetch = [&]() {
+    for (int i = 0; i < LOADS; ++i) offset[i] = (unsigned)min(8 * i + row, spare) * (unsigned)ld + (((lane & 7) ^ row) << 4);
+    const int stages = (int)((k1 - k0) * (int64_t)sizeof(T) / LINE);
+    auto fetch = [&](int stage) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        transfer(to[i] + filled * STAGE, base[i], offset[i]);
-        base[i] += LINE;
-      }
-      filled = filled == 2 ? 0 : filled + 1;
+      for (int i = 0; i < LOADS; ++i) transfer(to + (stage & 1) * STAGE + i * 8 * LINE, base, offset[i]);
+      base += LINE;
     };
-    fetch();
-    if (steps > 1) fetch();
-    int turn = 0;
-    for (int s = 0; s < steps; ++s) {
-      // This step's lines are in (the next step's LOADS transfers may be under way), for every wave once all have passed the barrier; and
-      // every wave is done reading the buffer of the step before, which the transfers below fill.
-      if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 2 < steps) fetch();
-      const char* buf = lds + turn * STAGE;
-      turn = turn == 2 ? 0 : turn + 1;
-      u32x4 a[MI], b[NI];
+    struct Fragments { u32x4 a[MI], b[NI]; };
+    int at_a[2], at_b[2];      // where this lane's fragments begin, by half; rows 16 apart have the same row % 8
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = *(const u32x4*)(buf + spot(BM + wave_n + j * 16 + (lane & 15), lane >> 4));
+    for (int h = 0; h < 2; ++h) {
+      at_a[h] = spot(wave_m + (lane & 15), 4 * h + (lane >> 4));
+      at_b[h] = spot(BM + wave_n + (lane & 15), 4 * h + (lane >> 4));
+    }
+    auto read = [&](Fragments& f, int stage, int h) {
+      const char* buf = lds + (stage & 1) * STAGE;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = *(const u32x4*)(buf + spot(wave_m + i * 16 + (lane & 15), lane >> 4));
+      for (int j = 0; j < NI; ++j) f.b[j] = *(const u32x4*)(buf + at_b[h] + j * 16 * LINE);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) f.a[i] = *(const u32x4*)(buf + at_a[h] + i * 16 * LINE);
+      __builtin_amdgcn_sched_barrier(0);      // (issued here: the compiler would put each in front of its use)
+    };
+    auto multiply_all = [&](const Fragments& f) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) multiply(c[i][j], a[i], b[j], T());
+        for (int j = 0; j < NI; ++j) multiply(c[i][j], f.a[i], f.b[j], T());
+    };
+    fetch(0);
+    if (stages > 1) fetch(1);
+    if (stages > 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    Fragments even, odd;
+    read(even, 0, 0);
+    for (int s = 0; s < stages; ++s) {
+      read(odd, s, 1);
+      multiply_all(even);
+      // The next stage's lines are in, for every wave once all have passed the barrier; and every wave has this stage's fragments in registers, so
+      // that the transfers of the stage after the next may overwrite its buffer.  (Behind the last stage an old buffer is read again.)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 2 < stages) fetch(s + 2);
+      read(even, s + 1, 0);
+      multiply_all(odd);
     }
   }
   // Sum (i, j, r) of this lane: row wave_m + 16 i + 4 (lane / 16) + r, column wave_n + 16 j + lane % 16 of the tile.
@@ -162,19 +173,24 @@ __device__ inline void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, 
 __device__ inline void max_over_16(float (&v)[4]) { asm volatile(PPN_OVER_16("v_max_f32_dpp") : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])); }
 __device__ inline void sum_over_16(float (&v)[4]) { asm volatile(PPN_OVER_16("v_add_f32_dpp") : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])); }
 #undef PPN_OVER_16
-// Plain minimum and maximum, the same way (arguments are results of ordinary instructions, never of a matrix instruction: those need waits of their own).
-__device__ inline float least(float a, float b) {
-  float r;
-  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
+// Plain maxima, the same way (arguments are results of ordinary instructions, never of a matrix instruction: those need waits of their own).
 __device__ inline float most(float a, float b) {
   float r;
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
+__device__ inline float most(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// a where the bit of the word is set, else b: two instructions, and nothing of a is looked at where it is not.
+__device__ inline float chosen(unsigned word, int bit, float a, int b) {
+  const int yes = __builtin_amdgcn_sbfe((int)word, bit, 1);
+  return __builtin_bit_cast(float, (yes & __builtin_bit_cast(int, a)) | (~yes & b));
+}
 
-// The bits of BN columns from n0 (of N, whose word 0 is `word` words into a row of allowed) that row `row` may NOT count: every one past the last
+// The bits of BN columns from n0 (of N, whose word 0 is `word` words into a row of allowed) that row `row` may count: none past the last
 // column.  Called before the product, so that the loads' way is covered by it; read after it.
 template <int BN> __device__ inline void stage_mask(unsigned (*mask)[BN / 32], int at, const int32_t* allowed, int64_t allowed_row, int64_t row, int64_t word, int64_t n0, int64_t N,
                                                     bool live) {
@@ -184,7 +200,7 @@ template <int BN> __device__ inline void stage_mask(unsigned (*mask)[BN / 32], i
     unsigned bits = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0;
     if (!live) bits = 0;
     if (allowed && bits) bits &= (unsigned)allowed[row * allowed_row + word + n0 / 32 + w];
-    mask[at][w] = ~bits;
+    mask[at][w] = bits;
   }
 }
 
@@ -201,7 +217,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsA
     stage_mask<P::BN>(mask, r, s.allowed, s.allowed_row, m0 + r < o.M ? m0 + r : o.M - 1, 0, n0, o.N, true);
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
-  const int column = p.lane & 15, low = 31 - column, high = 15 - column;      // left shifts that bring this lane's bit of a word's half to the top
+  const int column = p.lane & 15, next = column + 16;      // this lane's bit in a word's halves
   float2* out = s.partial + (n0 + p.wave_n) / (16 * NI) * o.M + m0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
@@ -209,22 +225,19 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsA
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const unsigned* word = mask[p.row_of(i, r)] + p.wave_n / 32;
-      top[r] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        // +infinity, or -infinity where the (inverted) bit says no: the sign bit on the pattern of infinity.  A NaN becomes +infinity here, and the sum NaN.
-        const unsigned limit = ((word[j / 2] << (j & 1 ? high : low)) & 0x80000000u) | 0x7f800000u;
-        l[r][j] = least(p.c[i][j][r] * LOG2E, __builtin_bit_cast(float, limit));
-        top[r] = most(top[r], l[r][j]);
-      }
+      for (int j = 0; j < NI; ++j) l[r][j] = chosen(word[j / 2], j & 1 ? next : column, p.c[i][j][r], (int)0xff800000);      // -infinity
+      if constexpr (NI == 4) top[r] = most(most(l[r][0], l[r][1], l[r][2]), l[r][3]);
+      else top[r] = most(l[r][0], l[r][1]);
     }
     max_over_16(top);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+      top[r] *= LOG2E;
       const float ref = top[r] == -INFINITY ? 0.0f : top[r];
       sum[r] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sum[r] += __builtin_amdgcn_exp2f(l[r][j] - ref);
+      for (int j = 0; j < NI; ++j) sum[r] += __builtin_amdgcn_exp2f(l[r][j] * LOG2E - ref);
     }
     sum_over_16(sum);
     // lanes 0..3 of each 16 have a row to write
@@ -235,7 +248,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsA
   }
 }
 
-// Sixteen rows a workgroup: joins the tiles' maxima and sums, 16 lanes a row, and takes the target's logit as a product of its own, a wave a row.
+// Sixteen rows a workgroup: joins the tiles' maxima and sums, 16 lanes a row, and takes the target's logit as a product of its own, a wave a row (four
+// rows' worth of loads at a time).
 template <typename T>
 __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* partial, int64_t columns) {
   __shared__ float tops[16][17], sums[16][17], wanted[16];
@@ -266,16 +280,24 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
     tops[threadIdx.x & 15][threadIdx.x / 16] = top;
     sums[threadIdx.x & 15][threadIdx.x / 16] = sum;
   }
-  for (int r = wave; r < 16; r += 4) {
-    const int64_t row = first + r, at = row < a.rows ? a.target[row] : -1;
-    float s = 0.0f;
-    if (at >= 0 && at < a.actions) {
-      const T* h = (const T*)a.hidden + row * a.hidden_row;
-      const T* w = (const T*)a.weight + at * a.weight_row;
-      for (int64_t f = lane; f < a.features; f += 64) s += to_float(h[f]) * to_float(w[f]);
-    }
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) wanted[r] = s;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const T* h[4];
+  const T* w[4];
+  bool inside[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t row = first + wave * 4 + k < a.rows ? first + wave * 4 + k : a.rows - 1, at = a.target[row];
+    inside[k] = at >= 0 && at < a.actions;
+    h[k] = (const T*)a.hidden + row * a.hidden_row;
+    w[k] = (const T*)a.weight + (inside[k] ? at : 0) * a.weight_row;
+  }
+  for (int64_t f = lane; f < a.features; f += 64)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += to_float(h[k][f]) * to_float(w[k][f]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    for (int d = 32; d; d >>= 1) s[k] += __shfl_xor(s[k], d);
+    if (lane == 0) wanted[wave * 4 + k] = s[k];
   }
   __syncthreads();
   if (threadIdx.x >= 16 || first + threadIdx.x >= a.rows) return;
@@ -284,13 +306,13 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
   for (int k = 0; k < 16; ++k) top = fmaxf(top, tops[threadIdx.x][k]);
   const float ref = top == -INFINITY ? 0.0f : top;
   for (int k = 0; k < 16; ++k) sum += sums[threadIdx.x][k] * __builtin_amdgcn_exp2f(tops[threadIdx.x][k] - ref);
-  const bool nothing = top == -INFINITY && sum == 0.0f, inside = at >= 0 && at < a.actions;
+  const bool nothing = top == -INFINITY && sum == 0.0f, known = at >= 0 && at < a.actions;
   const float whole = 0.693147180559945309f * (top + __builtin_amdgcn_logf(sum));
   float loss = 0.0f, lse = INFINITY;
   if (at != a.ignore_index && !nothing) {
-    const bool legal = inside && (!a.allowed || ((a.allowed[row * a.allowed_row + (at >> 5)] >> (at & 31)) & 1));
-    loss = !inside ? NAN : legal ? whole - wanted[threadIdx.x] : INFINITY;
-    lse = !inside || whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
+    const bool legal = known && (!a.allowed || ((a.allowed[row * a.allowed_row + (at >> 5)] >> (at & 31)) & 1));
+    loss = !known ? NAN : legal ? whole - wanted[threadIdx.x] : INFINITY;
+    lse = !known || whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
   }
   a.loss[row] = loss;
   a.lse[row] = lse;
@@ -361,8 +383,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
           const float v = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2) * q.up;
-          const int no = (int)(word[j / 2] << (j & 1 ? 15 - column : 31 - column)) >> 31;      // all ones where the action is not allowed
-          out[j][r] = (T)__builtin_bit_cast(float, __builtin_bit_cast(int, v) & ~no);
+          out[j][r] = (T)chosen(word[j / 2], column + (j & 1 ? 16 : 0), v, 0);
         }
       }
 #pragma unroll
@@ -401,7 +422,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
     const int64_t target = g.target[m0 + r] - g.first - n0;
     if (target < 0 || target >= P::BN || n0 + target >= o.N || g.lse[m0 + r] == INFINITY) continue;
     const int t = (int)target;
-    if ((mask[r][t / 32] >> (t & 31)) & 1) continue;
+    if (!((mask[r][t / 32] >> (t & 31)) & 1)) continue;
     const float loss = g.loss[m0 + r];
     const T v = (T)((loss != loss ? loss : expm1f(-loss)) * rows[r].up);
     *(T*)((char*)dl + (r * dl_row + t * (unsigned)sizeof(T))) = v;
@@ -487,11 +508,20 @@ bool in_place(const void* p, int64_t row, int64_t features, int64_t type) {
   return features % (LINE / size_of(type)) == 0 && row * size_of(type) % 16 == 0 && aligned(p, 16);
 }
 
-struct Config { int64_t bm, bn, columns_per_wave; bool large; };
-// 256 x 128 tiles where they fill the chip's 256 CUs; 64 x 64 ones elsewhere.
+// 256 x 256 tiles (a workgroup to a CU) where they fill three quarters of the chip's 256 CUs, since the larger the tile, the less is read from the
+// L2 and from LDS for an operation; else 128 x 128, else 64 x 64.  times: workgroups that can share the inner dimension of a tile.
+struct Config { int64_t tile, columns_per_wave; };
 Config config_for(int64_t m, int64_t n, int64_t times) {
-  const bool large = ceil_div(m, 256) * ceil_div(n, 128) * times >= 256;
-  return large ? Config{256, 128, 64, true} : Config{64, 64, 32, false};
+  if (ceil_div(m, 256) * ceil_div(n, 256) * times >= 192) return {256, 64};
+  if (ceil_div(m, 128) * ceil_div(n, 128) * times >= 192) return {128, 64};
+  return {64, 32};
+}
+// f(fragments of a wave across the rows, across the columns, waves across the columns; two across the rows)
+template <int MI, int NI, int WN> struct Shape { static constexpr int mi = MI, ni = NI, wn = WN, threads = 128 * WN; };
+template <typename F> void by_tile(const Config& c, F f) {
+  if (c.tile == 256) f(Shape<8, 4, 4>());
+  else if (c.tile == 128) f(Shape<4, 4, 2>());
+  else f(Shape<2, 2, 2>());
 }
 
 struct Layout { int64_t bytes = 0; int64_t take(int64_t n) { int64_t at = bytes; bytes += padded(n, 256); return at; } };
@@ -503,7 +533,7 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
   const int64_t size = size_of(a->type);
   p.features_padded = padded(a->features, inner(a));
   p.config = config_for(a->rows, a->actions, 1);
-  p.columns = padded(a->actions, p.config.bn) / p.config.columns_per_wave;
+  p.columns = padded(a->actions, p.config.tile) / p.config.columns_per_wave;
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
   p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
   p.partial = l.take(a->rows * p.columns * 8);
@@ -517,10 +547,9 @@ struct BackwardPlan {
   int64_t dh_share, dh_slots, dw_share, dw_slots;
 };
 
-// Shares of the inner dimension K that bring a product of few tiles to about 512 workgroups, at least 512 long each.
+// Shares of the inner dimension K that bring a product of few tiles to 256 workgroups, at least 512 long each.
 void split_inner(const Config& c, int64_t m, int64_t n, int64_t k, int64_t unit, int64_t* share, int64_t* slots) {
-  const int64_t tiles = ceil_div(m, c.bm) * ceil_div(n, c.bn);
-  int64_t want = 512 / tiles;
+  int64_t want = 256 / (ceil_div(m, c.tile) * ceil_div(n, c.tile));
   if (want > k / 512) want = k / 512;
   if (want < 1) want = 1;
   *share = padded(ceil_div(k, want), unit);
@@ -532,8 +561,8 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   Layout l;
   const int64_t size = size_of(a->type), unit = inner(a);
   p.features_padded = padded(a->features, unit);
-  p.rows_padded = padded(a->rows, 32);
-  p.actions_padded = padded(a->actions, 32);
+  p.rows_padded = padded(a->rows, 64);
+  p.actions_padded = padded(a->actions, 64);
   // A piece's dl and its transpose take 256 MB each.  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
   // of dweight's: 16384 rows of 24129 actions take 3.65, 3.02, 2.71, 2.44 and 2.33 ms behind the loss at 32, 64, 128, 256 and 512 MB.
   p.piece = padded((int64_t)(256 << 20) / (p.rows_padded * size), 128);
@@ -603,10 +632,9 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
       o.B = w + p.weight, o.ldb = p.features_padded;
     }
     const StatsArgs st = {a->allowed, a->allowed_row, (float2*)(w + p.partial), p.columns};
-    const int64_t tm = ceil_div(a->rows, p.config.bm), tn = ceil_div(a->actions, p.config.bn);
+    const int64_t tm = ceil_div(a->rows, p.config.tile), tn = ceil_div(a->actions, p.config.tile);
     if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
-    if (p.config.large) loss_stats<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
-    else loss_stats<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn);
+    by_tile(p.config, [&](auto t) { loss_stats<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(tm * tn), dim3(decltype(t)::threads), 0, s>>>(o, st, tm, tn); });
     loss_join<T><<<dim3(ceil_div(a->rows, 16)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
     return launched("ppn_loss_forward");
   });
@@ -649,28 +677,25 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
                                                                                                              a->features, (T*)(w + p.weight_t), p.actions_padded, nullptr);
     loss_scale<<<dim3(1), dim3(256), 0, s>>>(a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale);
     for (int64_t first = 0; first < a->actions; first += p.piece) {
-      const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 32);
+      const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 64);
       const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
       const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->loss, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
-      const int64_t tm = ceil_div(a->rows, p.grad.bm), tn = ceil_div(n, p.grad.bn);
-      if (p.grad.large) loss_grad<T, 8, 4, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);
-      else loss_grad<T, 2, 2, 2, 2><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn);
+      const int64_t tm = ceil_div(a->rows, p.grad.tile), tn = ceil_div(n, p.grad.tile);
+      by_tile(p.grad, [&](auto t) { loss_grad<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(tm * tn), dim3(decltype(t)::threads), 0, s>>>(o, g, tm, tn); });
       if (a->dhidden) {
         const Operands q = {w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np};
-        const int64_t um = ceil_div(a->rows, p.dh_config.bm), un = ceil_div(a->features, p.dh_config.bn);
+        const int64_t um = ceil_div(a->rows, p.dh_config.tile), un = ceil_div(a->features, p.dh_config.tile);
         // (the last piece is shorter: a share that begins past its end adds nothing, so every slot is written by the first piece)
         const SumArgs sums = {(float*)(w + p.dh), first > 0};
         const dim3 grid(um * un, first > 0 ? ceil_div(np, p.dh_share) : p.dh_slots);
-        if (p.dh_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
-        else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dh_share, um, un);
+        by_tile(p.dh_config, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<grid, dim3(decltype(t)::threads), 0, s>>>(q, sums, p.dh_share, um, un); });
       }
       if (a->dweight) {
         const Operands q = {w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded};
-        const int64_t um = ceil_div(n, p.dw_config.bm), un = ceil_div(a->features, p.dw_config.bn);
+        const int64_t um = ceil_div(n, p.dw_config.tile), un = ceil_div(a->features, p.dw_config.tile);
         const SumArgs sums = {(float*)(w + p.dw), false};
         const dim3 grid(um * un, p.dw_slots);
-        if (p.dw_config.large) loss_sums<T, 8, 4, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
-        else loss_sums<T, 2, 2, 2, 2><<<grid, dim3(256), 0, s>>>(q, sums, p.dw_share, um, un);
+        by_tile(p.dw_config, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<grid, dim3(decltype(t)::threads), 0, s>>>(q, sums, p.dw_share, um, un); });
         loss_finish<T><<<dim3(ceil_div(n * a->features, 256)), dim3(256), 0, s>>>((const float*)(w + p.dw), p.dw_slots, n * a->features, scale,
                                                                                    (T*)a->dweight + first * a->features);
       }
