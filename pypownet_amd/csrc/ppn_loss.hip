@@ -36,11 +36,11 @@ __device__ inline void multiply(f32x4& c, u32x4 a, u32x4 b, float) {
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
 }
 
-// Operands of one product: C[m, n] = sum_k A[m, k] B[n, k]; the inner dimension padded to whole lines, rows 16-byte aligned.
+// Operands of one product: C[m, n] = sum_k A[m, k] B[n, k]; rows and the inner dimension in whole 16 bytes.
 struct Operands {
   const void* A; int64_t lda, M;
   const void* B; int64_t ldb, N;
-  int64_t K;                      // padded
+  int64_t K;
 };
 
 struct StatsArgs { const int32_t* allowed; int64_t allowed_row; float2* partial; int64_t columns; };
@@ -48,7 +48,11 @@ struct GradArgs {
   const int32_t* allowed; int64_t allowed_row; const int64_t* target; const float* lse; const float* loss; const float* dloss; const float* scale;
   void* dl; int64_t dl_row; void* dlt; int64_t dlt_row; int64_t first, rows_padded, cols_padded;
 };
-struct SumArgs { float* sums; bool add; };
+// A product of the backward pass: shares of the inner dimension, `share` long, by tiles; 32-bit sums of share k to sums + k M N (on top of what is
+// there with add), or, with one share and nothing to add to, the result itself to out.
+struct SumJob { Operands o; float* sums; void* out; int64_t share; unsigned tiles_m, tiles_n, blocks; bool add; };
+
+__device__ const u32x4 zeros = {0, 0, 0, 0};
 
 constexpr int LINE = 128;         // bytes of the inner dimension per stage: a cache line, so that none is brought twice
 
@@ -71,6 +75,11 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
   // 8 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().
   __device__ static void transfer(unsigned to, const char* base, unsigned offset) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+  }
+
+  // The same with an address a lane, for the last stage where it is not a whole line: what is past its end is read from `zeros`.
+  __device__ static void transfer(unsigned to, const char* address) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(address) : "memory", "m0");
   }
 
   // The same for all lanes of the wave, and in scalar registers.
@@ -98,10 +107,18 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
     unsigned offset[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) offset[i] = (unsigned)min(8 * i + row, spare) * (unsigned)ld + (((lane & 7) ^ row) << 4);
-    const int stages = (int)((k1 - k0) * (int64_t)sizeof(T) / LINE);
+    const int bytes = (int)((k1 - k0) * (int64_t)sizeof(T)), stages = (bytes + LINE - 1) / LINE;
     auto fetch = [&](int stage) {
+      const unsigned at = to + (stage & 1) * STAGE;
+      const int left_over = bytes - stage * LINE;
+      if (left_over >= LINE) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) transfer(to + (stage & 1) * STAGE + i * 8 * LINE, base, offset[i]);
+        for (int i = 0; i < LOADS; ++i) transfer(at + i * 8 * LINE, base, offset[i]);
+      } else {
+        const bool in = (((lane & 7) ^ row) << 4) < left_over;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) transfer(at + i * 8 * LINE, in ? base + offset[i] : (const char*)&zeros);
+      }
       base += LINE;
     };
     struct Fragments { u32x4 a[MI], b[NI]; };
@@ -318,27 +335,6 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
   a.lse[row] = lse;
 }
 
-// scale[0] = the power of two dl is multiplied by, scale[1] = 1 / it.
-__global__ void __launch_bounds__(256) loss_scale(const float* dloss, const float* lse, int64_t rows, bool needed, float* scale) {
-  __shared__ float tops[256];
-  float top = 0.0f;
-  if (needed)
-    for (int64_t i = threadIdx.x; i < rows; i += 256) {
-      const float g = fabsf(dloss[i]);
-      if (lse[i] != INFINITY && g < INFINITY && g > top) top = g;
-    }
-  tops[threadIdx.x] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 256; ++i) top = tops[i] > top ? tops[i] : top;
-    int e = 0;
-    if (top > 0.0f) frexpf(top, &e);
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
-    scale[0] = needed && top > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
-    scale[1] = needed && top > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
-  }
-}
-
 // Two rows' (of a lane's column) values as one word, and the exchange that turns four rows of one column into two rows of two columns: lanes of
 // even columns keep the first two rows, those of odd ones the last two.
 __device__ inline unsigned pair(__bf16 a, __bf16 b) { return (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16; }
@@ -430,20 +426,35 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
   }
 }
 
-// Backward, second products: 32-bit sums of one share of the inner dimension (grid.y shares, a slot of [M x N] floats each).
+// Backward, second products: dhidden's and dweight's at once, so that the one fills the CUs the other leaves.
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(Operands o, SumArgs s, int64_t share, unsigned tiles_m, unsigned tiles_n) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(SumJob one, SumJob two, const float* scale) {
   typedef Product<T, MI, NI, WM, WN> P;
   __shared__ __align__(16) char lds[P::LDS_BYTES];
+  const bool second = blockIdx.x >= one.blocks;
+  const SumJob job = second ? two : one;
+  const Operands& o = job.o;
+  const unsigned id = blockIdx.x - (second ? one.blocks : 0), tiles = job.tiles_m * job.tiles_n, k = id / tiles;
   unsigned tm, tn;
-  tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN;
-  const int64_t k0 = blockIdx.y * share, k1 = k0 + share < o.K ? k0 + share : o.K;
+  tile_of(id - k * tiles, job.tiles_m, job.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN, k0 = k * job.share, k1 = k0 + job.share < o.K ? k0 + job.share : o.K;
   P p;
   p.run(o, lds, m0, n0, k0, k1);
-  float* sums = s.sums + blockIdx.y * o.M * o.N + m0 * o.N + n0;
   const unsigned ld = (unsigned)o.N;
   const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
+  if (job.out) {
+    T* out = (T*)job.out + m0 * o.N + n0;
+    const float unscale = scale[1];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+          if (whole || (m0 + p.row_of(i, r) < o.M && n0 + p.col_of(j) < o.N)) out[p.row_of(i, r) * ld + p.col_of(j)] = (T)(p.c[i][j][r] * unscale);
+    return;
+  }
+  float* sums = job.sums + k * o.M * o.N + m0 * o.N + n0;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     float old[4][NI];
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(Operands o, SumArgs
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         old[r][j] = 0.0f;
-        if (s.add && (whole || (m0 + p.row_of(i, r) < o.M && n0 + p.col_of(j) < o.N))) old[r][j] = sums[p.row_of(i, r) * ld + p.col_of(j)];
+        if (job.add && (whole || (m0 + p.row_of(i, r) < o.M && n0 + p.col_of(j) < o.N))) old[r][j] = sums[p.row_of(i, r) * ld + p.col_of(j)];
       }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -462,13 +473,17 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(Operands o, SumArgs
   }
 }
 
+// What is left to do with the products' 32-bit sums: two jobs (dhidden, dweight), `count` elements of `slots` slots each.
+struct FinishJob { const float* sums; int64_t slots, count; void* out; };
 template <typename T>
-__global__ void __launch_bounds__(256) loss_finish(const float* sums, int64_t slots, int64_t count, const float* scale, T* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
+__global__ void __launch_bounds__(256) loss_finish(FinishJob one, FinishJob two, int64_t blocks_one, const float* scale) {
+  const bool second = blockIdx.x >= blocks_one;
+  const FinishJob job = second ? two : one;
+  const int64_t i = ((int64_t)blockIdx.x - (second ? blocks_one : 0)) * 256 + threadIdx.x;
+  if (i >= job.count) return;
   float v = 0.0f;
-  for (int64_t s = 0; s < slots; ++s) v += sums[s * count + i];
-  out[i] = (T)(v * scale[1]);
+  for (int64_t s = 0; s < job.slots; ++s) v += job.sums[s * job.count + i];
+  ((T*)job.out)[i] = (T)(v * scale[1]);
 }
 
 // [rows x cols] with any row stride -> [rows x cols_padded], zeros in the padding.
@@ -480,32 +495,59 @@ __global__ void __launch_bounds__(256) loss_pad(const T* in, int64_t in_row, int
   out[i] = c < cols ? in[r * in_row + c] : (T)0.0f;
 }
 
-// [rows x cols] with any row stride -> [cols x rows_padded], zeros in the padding.  64 x 64 tiles through LDS.  A row without a gradient (lse
-// +infinity) becomes zeros: whatever stands in it, its product with dl's zeros is zero.
+// In front of the backward products: the transposed copies of hidden and weight, [cols x rows_padded] with zeros in the padding (64 x 64 tiles
+// through LDS, `across` of them along the rows), and dl's scale.  A row of hidden without a gradient (lse +infinity) becomes zeros: whatever
+// stands in it, its product with dl's zeros is zero.
+struct TransposeJob { const void* in; int64_t in_row, rows, cols; void* out; int64_t rows_padded; const float* lse; int64_t across, blocks; };
+struct ScaleJob { const float* dloss; const float* lse; int64_t rows; bool needed; float* scale; };      // scale[0]: a power of two, scale[1] = 1 / it
 template <typename T>
-__global__ void __launch_bounds__(256) loss_transpose(const T* in, int64_t in_row, int64_t rows, int64_t cols, T* out, int64_t rows_padded, const float* lse) {
+__global__ void __launch_bounds__(256) loss_prepare(TransposeJob one, TransposeJob two, ScaleJob sc) {
   __shared__ T tile[64][64 + 4 / sizeof(T)];
-  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  __shared__ float tops[256];
+  if (blockIdx.x >= one.blocks + two.blocks) {
+    float top = 0.0f;
+    if (sc.needed)
+      for (int64_t i = threadIdx.x; i < sc.rows; i += 256) {
+        const float g = fabsf(sc.dloss[i]);
+        if (sc.lse[i] != INFINITY && g < INFINITY && g > top) top = g;
+      }
+    tops[threadIdx.x] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 256; ++i) top = tops[i] > top ? tops[i] : top;
+      int e = 0;
+      if (top > 0.0f) frexpf(top, &e);
+      e = e < -100 ? -100 : e > 100 ? 100 : e;
+      sc.scale[0] = top > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
+      sc.scale[1] = top > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
+    }
+    return;
+  }
+  const bool second = blockIdx.x >= one.blocks;
+  const TransposeJob job = second ? two : one;
+  const int64_t id = (int64_t)blockIdx.x - (second ? one.blocks : 0), r0 = id % job.across * 64, c0 = id / job.across * 64;
   const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const T* in = (const T*)job.in;
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
     const int64_t r = r0 + y + i, c = c0 + x;
-    tile[y + i][x] = r < rows && c < cols && !(lse && lse[r] == INFINITY) ? in[r * in_row + c] : (T)0.0f;
+    tile[y + i][x] = r < job.rows && c < job.cols && !(job.lse && job.lse[r] == INFINITY) ? in[r * job.in_row + c] : (T)0.0f;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
     const int64_t c = c0 + y + i, r = r0 + x;
-    if (c < cols && r < rows_padded) out[c * rows_padded + r] = tile[x][y + i];
+    if (c < job.cols && r < job.rows_padded) ((T*)job.out)[c * job.rows_padded + r] = tile[x][y + i];
   }
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------------------------
 int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-int64_t inner(const ppn_loss_args* a) { return LINE / size_of(a->type); }
+int64_t part(const ppn_loss_args* a) { return 16 / size_of(a->type); }      // elements of 16 bytes
 
+// Rows that the product reads as they are; others are copied into whole 16 bytes first.
 bool in_place(const void* p, int64_t row, int64_t features, int64_t type) {
-  return features % (LINE / size_of(type)) == 0 && row * size_of(type) % 16 == 0 && aligned(p, 16);
+  return features % (16 / size_of(type)) == 0 && row * size_of(type) % 16 == 0 && row <= (1 << 23) && aligned(p, 16);
 }
 
 // 256 x 256 tiles (a workgroup to a CU) where they fill three quarters of the chip's 256 CUs, since the larger the tile, the less is read from the
@@ -531,7 +573,7 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
   ForwardPlan p;
   Layout l;
   const int64_t size = size_of(a->type);
-  p.features_padded = padded(a->features, inner(a));
+  p.features_padded = padded(a->features, part(a));
   p.config = config_for(a->rows, a->actions, 1);
   p.columns = padded(a->actions, p.config.tile) / p.config.columns_per_wave;
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
@@ -543,24 +585,17 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
 
 struct BackwardPlan {
   int64_t features_padded, rows_padded, actions_padded, piece, hidden, weight, hidden_t, weight_t, dl, dlt, scale, dh, dw, bytes;
-  Config grad, dh_config, dw_config;
-  int64_t dh_share, dh_slots, dw_share, dw_slots;
+  Config grad, sums;
+  int64_t share, dh_slots, dw_slots;
+  bool direct_dh, direct_dw;
 };
 
-// Shares of the inner dimension K that bring a product of few tiles to 256 workgroups, at least 512 long each.
-void split_inner(const Config& c, int64_t m, int64_t n, int64_t k, int64_t unit, int64_t* share, int64_t* slots) {
-  int64_t want = 256 / (ceil_div(m, c.tile) * ceil_div(n, c.tile));
-  if (want > k / 512) want = k / 512;
-  if (want < 1) want = 1;
-  *share = padded(ceil_div(k, want), unit);
-  *slots = ceil_div(k, *share);
-}
-
+// (The same whether both gradients are wanted or one: the sizes alone tell how much memory a call needs.)
 BackwardPlan plan_backward(const ppn_loss_args* a) {
   BackwardPlan p;
   Layout l;
-  const int64_t size = size_of(a->type), unit = inner(a);
-  p.features_padded = padded(a->features, unit);
+  const int64_t size = size_of(a->type);
+  p.features_padded = padded(a->features, part(a));
   p.rows_padded = padded(a->rows, 64);
   p.actions_padded = padded(a->actions, 64);
   // A piece's dl and its transpose take 256 MB each.  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
@@ -569,10 +604,21 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   if (p.piece < 1024) p.piece = 1024;
   if (p.piece > p.actions_padded) p.piece = p.actions_padded;
   p.grad = config_for(a->rows, p.piece, 1);
-  p.dh_config = config_for(a->rows, a->features, p.piece / 1024 + 1);
-  p.dw_config = config_for(p.piece, a->features, a->rows / 1024 + 1);
-  split_inner(p.dh_config, a->rows, a->features, p.piece, unit, &p.dh_share, &p.dh_slots);
-  split_inner(p.dw_config, p.piece, a->features, p.rows_padded, unit, &p.dw_share, &p.dw_slots);
+  // The second products: the largest tile with which shares of at least 512 of the inner dimensions make 192 workgroups of the two, then the
+  // shortest share with which they are at most 256 (512 of the smaller tiles, of which two and more fit a CU).
+  const int64_t most[] = {256, 512, 512}, tiles[] = {256, 128, 64};
+  for (int i = 0; i < 3; ++i) {
+    p.sums = {tiles[i], 0};
+    const int64_t across = ceil_div(a->features, tiles[i]), dh = ceil_div(a->rows, tiles[i]) * across, dw = ceil_div(p.piece, tiles[i]) * across;
+    auto blocks = [&](int64_t share) { return dh * ceil_div(p.piece, share) + dw * ceil_div(p.rows_padded, share); };
+    if (i < 2 && blocks(512) < 192) continue;
+    p.share = 512;
+    const int64_t longest = p.piece > p.rows_padded ? p.piece : p.rows_padded;
+    while (p.share < longest && blocks(p.share) > most[i]) p.share += 128;
+    break;
+  }
+  p.dh_slots = ceil_div(p.piece, p.share), p.dw_slots = ceil_div(p.rows_padded, p.share);
+  p.direct_dh = p.dh_slots == 1 && p.piece >= a->actions, p.direct_dw = p.dw_slots == 1;
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
   p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
   p.hidden_t = l.take(a->features * p.rows_padded * size);
@@ -580,8 +626,8 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   p.dl = l.take(a->rows * p.piece * size);
   p.dlt = l.take(p.piece * p.rows_padded * size);
   p.scale = l.take(8);
-  p.dh = l.take(p.dh_slots * a->rows * a->features * 4);
-  p.dw = l.take(p.dw_slots * p.piece * a->features * 4);
+  p.dh = l.take(p.direct_dh ? 0 : p.dh_slots * a->rows * a->features * 4);
+  p.dw = l.take(p.direct_dw ? 0 : p.dw_slots * p.piece * a->features * 4);
   p.bytes = l.bytes;
   return p;
 }
@@ -590,7 +636,7 @@ int check(const ppn_loss_args* a) {
   if (!a || a->struct_bytes != (int64_t)sizeof *a) return fail(PPN_E_INVALID, "ppn_loss_args: struct_bytes does not match this library");
   if (a->type < 0 || a->type > PPN_T_F16) return fail(PPN_E_INVALID, "element type %lld is unknown", (long long)a->type);
   if (a->rows < 0 || a->actions < 1 || a->features < 1) return fail(PPN_E_INVALID, "loss: rows >= 0, actions >= 1 and features >= 1 are needed");
-  if (a->rows > (1 << 27) || a->actions > (1 << 27) || a->features > (1 << 20)) return fail(PPN_E_INVALID, "loss: a size is out of range");
+  if (a->rows > (1 << 21) || a->actions > (1 << 23) || a->features > (1 << 20)) return fail(PPN_E_INVALID, "loss: a size is out of range");
   return PPN_OK;
 }
 
@@ -669,40 +715,38 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
       if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
       weight = w + p.weight, weight_row = p.features_padded;
     }
-    if (a->dweight)
-      loss_transpose<T><<<dim3(ceil_div(p.rows_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->hidden, a->hidden_row, a->rows, a->features,
-                                                                                                          (T*)(w + p.hidden_t), p.rows_padded, a->lse);
-    if (a->dhidden)
-      loss_transpose<T><<<dim3(ceil_div(p.actions_padded, 64), ceil_div(a->features, 64)), dim3(256), 0, s>>>((const T*)a->weight, a->weight_row, a->actions,
-                                                                                                             a->features, (T*)(w + p.weight_t), p.actions_padded, nullptr);
-    loss_scale<<<dim3(1), dim3(256), 0, s>>>(a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale);
+    const int64_t down = ceil_div(a->features, 64), hidden_across = ceil_div(p.rows_padded, 64), weight_across = ceil_div(p.actions_padded, 64);
+    const TransposeJob th = {a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden_t, p.rows_padded, a->lse, hidden_across, a->dweight ? hidden_across * down : 0};
+    const TransposeJob tw = {a->weight, a->weight_row, a->actions, a->features, w + p.weight_t, p.actions_padded, nullptr, weight_across, a->dhidden ? weight_across * down : 0};
+    if (th.blocks + tw.blocks > 0x7ffffff0) return fail(PPN_E_INVALID, "loss: an operand is too large");
+    loss_prepare<T><<<dim3(th.blocks + tw.blocks + 1), dim3(256), 0, s>>>(th, tw, ScaleJob{a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale});
     for (int64_t first = 0; first < a->actions; first += p.piece) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 64);
       const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
       const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->loss, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
       const int64_t tm = ceil_div(a->rows, p.grad.tile), tn = ceil_div(n, p.grad.tile);
       by_tile(p.grad, [&](auto t) { loss_grad<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(tm * tn), dim3(decltype(t)::threads), 0, s>>>(o, g, tm, tn); });
-      if (a->dhidden) {
-        const Operands q = {w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np};
-        const int64_t um = ceil_div(a->rows, p.dh_config.tile), un = ceil_div(a->features, p.dh_config.tile);
-        // (the last piece is shorter: a share that begins past its end adds nothing, so every slot is written by the first piece)
-        const SumArgs sums = {(float*)(w + p.dh), first > 0};
-        const dim3 grid(um * un, first > 0 ? ceil_div(np, p.dh_share) : p.dh_slots);
-        by_tile(p.dh_config, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<grid, dim3(decltype(t)::threads), 0, s>>>(q, sums, p.dh_share, um, un); });
-      }
-      if (a->dweight) {
-        const Operands q = {w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded};
-        const int64_t um = ceil_div(n, p.dw_config.tile), un = ceil_div(a->features, p.dw_config.tile);
-        const SumArgs sums = {(float*)(w + p.dw), false};
-        const dim3 grid(um * un, p.dw_slots);
-        by_tile(p.dw_config, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<grid, dim3(decltype(t)::threads), 0, s>>>(q, sums, p.dw_share, um, un); });
-        loss_finish<T><<<dim3(ceil_div(n * a->features, 256)), dim3(256), 0, s>>>((const float*)(w + p.dw), p.dw_slots, n * a->features, scale,
-                                                                                   (T*)a->dweight + first * a->features);
+      const int64_t across = ceil_div(a->features, p.sums.tile);
+      // (the last piece is shorter: a share that begins past its end adds nothing, and every slot has been written by the first piece)
+      auto job = [&](const Operands& q, int64_t at, void* out, bool wanted, bool add) {
+        const int64_t down = ceil_div(q.M, p.sums.tile);
+        return SumJob{q, (float*)(w + at), out, p.share, (unsigned)down, (unsigned)across, wanted ? (unsigned)(down * across * ceil_div(q.K, p.share)) : 0u, add};
+      };
+      const SumJob dh = job({w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np}, p.dh,
+                            p.direct_dh ? a->dhidden : nullptr, a->dhidden, first > 0);
+      T* dw_out = (T*)a->dweight + (a->dweight ? first * a->features : 0);
+      const SumJob dw = job({w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded}, p.dw,
+                            p.direct_dw ? dw_out : nullptr, a->dweight, false);
+      if (dh.blocks + dw.blocks)
+        by_tile(p.sums, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(dh.blocks + dw.blocks), dim3(decltype(t)::threads), 0, s>>>(dh, dw, scale); });
+      const bool last = first + p.piece >= a->actions;
+      const FinishJob fh = {(const float*)(w + p.dh), p.dh_slots, last && a->dhidden && !p.direct_dh ? a->rows * a->features : 0, a->dhidden};
+      const FinishJob fw = {(const float*)(w + p.dw), p.dw_slots, a->dweight && !p.direct_dw ? n * a->features : 0, dw_out};
+      if (fh.count + fw.count) {
+        const int64_t blocks = ceil_div(fh.count, 256);
+        loss_finish<T><<<dim3(blocks + ceil_div(fw.count, 256)), dim3(256), 0, s>>>(fh, fw, blocks, scale);
       }
     }
-    if (a->dhidden)
-      loss_finish<T><<<dim3(ceil_div(a->rows * a->features, 256)), dim3(256), 0, s>>>((const float*)(w + p.dh), p.dh_slots, a->rows * a->features, scale,
-                                                                                      (T*)a->dhidden);
     return launched("ppn_loss_backward");
   });
 }
