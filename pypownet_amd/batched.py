@@ -189,15 +189,44 @@ class BatchedRunEnv(object):
             e.rollout_device(t.data_ptr(), n_steps, per_step_actions=per_step, auto_reset=auto_reset)
         return e.read('RETURN'), e.read('DONE').astype(bool), e.read('FLAG'), e.read('N_STEPS')
 
-    def policy_actions(self, policy='line_relief', params=(1.0,)):
-        """The built-in device policy's choice for the CURRENT state of every environment of this shard (include/ppn.h,
-        ppn_policy_actions) as a torch CUDA uint8 tensor [batch x action_length] -- ready for ``step``."""
+    def policy_actions(self, policy='line_relief', params=(1.0,), memory=None, layout='full', sample=False):
+        """A device policy's choice for the CURRENT state of every environment of this shard as a torch CUDA uint8 tensor
+        [batch x action_length] -- ready for ``step``.  ``policy``: the name of a built-in one with its ``params`` (include/ppn.h,
+        ppn_policy_actions), or a ``policy.RecurrentPolicy`` with the ``memory`` it keeps of these environments (moved on by one row; an
+        environment whose last step ended its episode begins a new one), the observation ``layout`` it reads, and ``sample``."""
         import torch
+        if isinstance(policy, torch.nn.Module):
+            if memory is None:
+                raise ValueError('policy_actions: a policy module needs its memory of these environments (policy.memory(env.batch))')
+            policy._check_memory(memory, self.batch)
+            obs, starts, allowed = self.policy_rows(policy, layout=layout)
+            return policy.vectors[policy.act(obs, memory, starts=starts, allowed=allowed, sample=sample)]
         out = torch.empty((self.batch, self.action_length), dtype=torch.uint8, device='cuda:%d' % self.device)
         self._sync_torch(out)
         self.engine.policy_actions(policy, list(params), out.data_ptr())
         self.engine.wait()
         return out
+
+    def policy_rows(self, policy, layout='full'):
+        """What a ``policy.RecurrentPolicy`` decides from, for the CURRENT state of every environment, as torch CUDA tensors: observation rows
+        (float32), starts (uint8 [batch]: the last step ended the episode before) and the allowed actions of its catalogue (bool
+        [batch x actions]: a line that is cooling down or not reconnectable yet, or a substation that is cooling down, is refused by
+        the rules of ``step``)."""
+        import torch
+        e, dev = self.engine, 'cuda:%d' % self.device
+        c = policy.catalogue
+        if c.action_length != self.action_length:
+            raise ValueError('this policy chooses actions of length %d, the environments take %d' % (c.action_length, self.action_length))
+        obs = torch.empty((self.batch, e.observation_length(layout)), dtype=torch.float32, device=dev)
+        starts = torch.empty((self.batch,), dtype=torch.uint8, device=dev)
+        wait = [torch.empty((self.batch, n), dtype=torch.int32, device=dev) for n in (c.n_lines, c.n_lines, c.n_substations)]
+        self._sync_torch(obs)      # (the memory may still be in use by what torch has queued)
+        e.read_into_device('DONE', starts.data_ptr(), starts.numel())      # (a report field, read before a restart that is owed is settled)
+        e.observations_into_device(obs.data_ptr(), 4 * obs.numel(), layout=layout, dtype=np.float32)
+        for name, t in zip(('RECONNECTABLE', 'LINE_COOLDOWN', 'NODE_COOLDOWN'), wait):
+            e.read_into_device(name, t.data_ptr(), 4 * t.numel())
+        e.wait()
+        return obs, starts, c.allowed((wait[0] == 0) & (wait[1] == 0), wait[2] == 0, policy.asset)
 
     def rollout_policy(self, n_steps, policy='line_relief', params=(1.0,)):
         """``n_steps`` closed-loop steps of a built-in device policy in ONE launch, every environment on its own clock (include/ppn.h,

@@ -609,6 +609,38 @@ def test_gpu_action_cross_entropy(case, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_action_cross_entropy_in_pieces(dtype):
+    """So many logits that the backward pass takes the catalogue in several pieces, the last one shorter."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(25)
+    n, v, f = 16400, 9001, 24
+    hidden, weight = rand(gen, n, f, dtype=dtype), rand(gen, v, f, scale=0.3, dtype=dtype)
+    target = torch.randint(0, v, (n,), generator=gen)
+    dloss = rand(gen, n)
+    own = on_gpu(hidden, weight, grad=True)
+    loss = ops.action_cross_entropy(own[0], own[1], target.cuda())
+    grads = torch.autograd.grad(loss, own, dloss.cuda())
+    h, w, g = hidden.cuda().double(), weight.cuda().double(), dloss.cuda().double()[:, None]
+    logits = h @ w.t()
+    size = float((h.abs() @ w.abs().t()).max())
+    p = torch.softmax(logits, 1)
+    at = torch.arange(n, device='cuda')
+    close('loss', loss, (torch.logsumexp(logits, 1) - logits[at, target.cuda()]).cpu(), torch.float32, f + 64, size + 16)
+    p[at, target.cuda()] -= 1
+    dl = p * g
+    # as in test_gpu_action_cross_entropy, |p - one| being a probability's size or more
+    each = (half(dtype) + 2 * (f + 32) * STEP * (size + 16)) * dl.abs() + (2 * (f + 32) * STEP * (size + 16)) * g.abs() * (p < 0)
+    if dtype == torch.float16:
+        each = each + float(dloss.abs().max()) * 2.0 ** -38
+    for name, got, want, slack, total in (('dhidden', grads[0], dl @ w, each @ w.abs(), dl.abs() @ w.abs()),
+                                          ('dweight', grads[1], dl.t().contiguous() @ h, each.t().contiguous() @ h.abs(), dl.abs().t().contiguous() @ h.abs())):
+        limit = slack + half(dtype) * want.abs() * 1.01 + 2 * (n + 8) * STEP * total + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        off = (got.double() - want).abs()
+        assert (off <= limit).all(), '%s: worst %.3g of its limit' % (name, float((off / limit).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
 def test_gpu_action_cross_entropy_of_bad_targets_and_values(dtype):
     from pypownet_amd import policy_ops as ops
     gen = torch.Generator().manual_seed(22)

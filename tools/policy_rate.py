@@ -1,7 +1,9 @@
 #!/usr/bin/env python
 """Closed-loop stepping without the batch barrier (GPU box): env-steps/s of ppn_rollout_policy (device-side policy, every environment
 on its own clock) next to the synchronous forms on the bench workload.
-    python tools/policy_rate.py [batch] [steps]"""
+    python tools/policy_rate.py [batch] [steps]
+    python tools/policy_rate.py --recurrent [batch] [steps]      a RecurrentPolicy (pypownet_amd/policy.py) in the loop instead: acting, and learning
+                                                                 from the search"""
 import json
 import os
 import sys
@@ -13,7 +15,48 @@ ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), '..'))
 sys.path.insert(0, ROOT)
 
 
+def recurrent(B, K):
+    import torch
+    import bench
+    from pypownet_amd.batched import BatchedRunEnv
+    from pypownet_amd.policy import ActionCatalogue, RecurrentPolicy, imitate
+    case, _, _ = bench.load_workload()
+    env = BatchedRunEnv(os.path.join(ROOT, 'tests', 'golden', 'envs', bench.ENV_NAME), 'level0', B, device=0, config_overrides={'solver': 'newton'},
+                        thermal_limits=bench.bench_limits(case), max_active_buses=case.nS)
+    env.reset()
+    catalogue = ActionCatalogue(env.case)
+    policy = RecurrentPolicy(catalogue, env.engine.observation_length('minimalist'), features=256).cuda()
+    memory = policy.memory(B)
+
+    def timed(f, n):
+        f()
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        for _ in range(n):
+            f()
+        torch.cuda.synchronize()
+        return (time.perf_counter() - t) / n
+    out = {'batch': B, 'steps': K, 'actions': len(catalogue), 'features': policy.features}
+    obs, starts, allowed = env.policy_rows(policy, layout='minimalist')
+    out['policy_rows_ms'] = 1e3 * timed(lambda: env.policy_rows(policy, layout='minimalist'), K)
+    out['act_ms'] = 1e3 * timed(lambda: policy.act(obs, memory, starts=starts, allowed=allowed), K)
+    step = timed(lambda: env.step(env.policy_actions(policy, memory=memory, layout='minimalist'), want_obs=False), K)
+    out['closed_loop_env_steps_per_s'] = B / step
+    window = [v[:, None].expand(v.shape[0], 32, *v.shape[1:]) for v in (obs, starts)]
+    target = torch.zeros((B, 32), dtype=torch.int64, device='cuda')
+
+    def learn():
+        policy.loss(window[0], target, starts=window[1], memory=memory)[0].mean().backward()
+    out['learn_32_rows_ms'] = 1e3 * timed(learn, 3)
+    optimizer = torch.optim.SGD(policy.parameters(), lr=1e-3)
+    out['imitate_4_steps_of_8_candidates_ms'] = 1e3 * timed(lambda: imitate(env, policy, optimizer, memory, steps=4, layout='minimalist'), 1)
+    print(json.dumps(out))
+
+
 def main():
+    if '--recurrent' in sys.argv[1:]:
+        given = [int(a) for a in sys.argv[1:] if a != '--recurrent']
+        return recurrent(given[0] if given else 1024, given[1] if len(given) > 1 else 20)
     import torch
     import bench
     from pypownet_amd.engine import Engine
