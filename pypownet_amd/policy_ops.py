@@ -83,21 +83,23 @@ def _need(condition, *text):
 
 def _leading(name, x):
     """The tensor that names a call's type and device."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TYPES:
+        return _TYPES[x.dtype]
     if not torch.is_tensor(x):
         raise TypeError('%s must be a torch tensor, got %s' % (name, type(x).__name__))
     if x.dtype not in _TYPES:
         raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, x.dtype))
-    _need(x.is_cuda, name, 'must live on a GPU: these operators have no CPU form')
-    return _TYPES[x.dtype]
+    raise ValueError('%s must live on a GPU: these operators have no CPU form' % name)
 
 
 def _like(name, t, shape, dtype, device):
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        return
     if not torch.is_tensor(t):
         raise TypeError('%s must be a torch tensor, got %s' % (name, type(t).__name__))
     if t.dtype != dtype:
         raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
-    if t.device != device or tuple(t.shape) != shape:
-        raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
+    raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
 
 
 def _rows(t):
@@ -121,8 +123,8 @@ def _window_like(x):
     """An output with x's order in memory: time outermost where x has it outermost."""
     b, t, d = x.shape
     if b > 1 and t > 1 and x.stride(0) < x.stride(1):
-        return torch.empty((t, b, d), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+        return x.new_empty((t, b, d)).transpose(0, 1)
+    return x.new_empty((b, t, d))
 
 
 def _at(t):
@@ -131,12 +133,41 @@ def _at(t):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _window_rows(x):
+    if x.dim() != 3 or x.shape[2] == 0:
+        raise ValueError('x must be [batch, time, channels], got %s' % list(x.shape))
+    return x.shape
+
+
+def _step_rows(x):
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError('x must be [rows, channels], got %s' % list(x.shape))
+    return x.shape
+
+
+def _step_state(state, of):
+    if not isinstance(state, torch.Tensor):
+        raise TypeError('state must be a torch tensor, got %s' % type(state).__name__)
+    if state.dim() != 3 or not state.is_contiguous():
+        raise ValueError('state must be [environments, %s] and contiguous, got %s' % (of, list(state.shape)))
+    return state.shape[0]
+
+
+def _step_flags(starts, rows, device):
+    return None if starts is None else _flags('starts', starts, (rows,), device).contiguous()
 
 
 def _step_ids(env_ids, rows, environments, device):
     if env_ids is None:
-        _need(rows <= environments, 'there are', rows, 'rows and', environments, 'environments: env_ids must say whose rows they are')
+        if rows > environments:
+            raise ValueError('there are %d rows and %d environments: env_ids must say whose rows they are' % (rows, environments))
         return None
     if not torch.is_tensor(env_ids):
         raise TypeError('env_ids must be a torch tensor, got %s' % type(env_ids).__name__)
@@ -202,10 +233,13 @@ def _activation(activation):
 
 
 def _conv_parameters(channels, weight, bias, device):
-    _need(torch.is_tensor(weight) and weight.dim() == 2 and 2 <= weight.shape[1] <= 8, 'weight must be a tensor [channels, taps] with 2 to 8 taps')
-    _like('weight', weight, (channels, weight.shape[1]), torch.float32, device)
+    if not (isinstance(weight, torch.Tensor) and weight.dim() == 2 and 2 <= weight.shape[1] <= 8):
+        raise ValueError('weight must be a tensor [channels, taps] with 2 to 8 taps')
+    taps = weight.shape[1]
+    _like('weight', weight, (channels, taps), torch.float32, device)
     if bias is not None:
         _like('bias', bias, (channels,), torch.float32, device)
+    return taps
 
 
 def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state=None, return_final_state=False):
@@ -217,9 +251,7 @@ def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state
     episode that is running at the window's end, i.e. the next window's ``initial_state`` and ``short_conv_step``'s state.  Differentiable in
     x, weight, bias and initial_state; the parameters' gradients are summed in a fixed order."""
     _leading('x', x)
-    _need(x.dim() == 3, 'x must be [batch, time, channels], got', list(x.shape))
-    b, t, d = x.shape
-    _need(d > 0, 'x must have channels')
+    b, t, d = _window_rows(x)
     silu = _activation(activation)
     _conv_parameters(d, weight, bias, x.device)
     if initial_state is not None:
@@ -239,24 +271,22 @@ def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, 
     None); a negative id is padding: y = 0 and no state is touched.  An id out of range, or one that an earlier row has, gives NaN and touches no
     state.  ``starts [rows]`` empties the window first.  Returns y [rows, channels]."""
     kind = _leading('x', x)
-    _need(x.dim() == 2 and x.shape[1] > 0, 'x must be [rows, channels], got', list(x.shape))
-    n, d = x.shape
+    n, d = _step_rows(x)
+    device = x.device
     silu = _activation(activation)
-    _conv_parameters(d, weight, bias, x.device)
-    if not torch.is_tensor(state):
-        raise TypeError('state must be a torch tensor, got %s' % type(state).__name__)
-    _need(state.dim() == 3, 'state must be [environments, taps - 1, channels], got', list(state.shape))
-    _like('state', state, (state.shape[0], weight.shape[1] - 1, d), x.dtype, x.device)
-    _need(state.is_contiguous(), 'state must be contiguous')
+    taps = _conv_parameters(d, weight, bias, device)
+    environments = _step_state(state, 'taps - 1, channels')
+    _like('state', state, (environments, taps - 1, d), x.dtype, device)
     if _wants_grad(x, state, weight, bias):
         raise ValueError('short_conv_step has no gradient: call it under torch.no_grad(), or short_conv on the window')
-    starts = _flags('starts', starts, (n,), x.device)
-    env_ids = _step_ids(env_ids, n, state.shape[0], x.device)
+    starts = _step_flags(starts, n, device)
+    env_ids = _step_ids(env_ids, n, environments, device)
     x, weight = _rows(x), weight.contiguous()
-    bias, starts = (None if v is None else v.contiguous() for v in (bias, starts))
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, kind, silu, n, state.shape[0], d, weight.shape[1], x.data_ptr(), x.stride(0),
-                                                 weight.data_ptr(), _ptr(bias), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), x.device)
+    if bias is not None:
+        bias = bias.contiguous()
+    y = x.new_empty((n, d))
+    _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, kind, silu, n, environments, d, taps, x.data_ptr(), x.stride(0), weight.data_ptr(),
+                                                 _ptr(bias), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
     return y
 
 
@@ -286,8 +316,8 @@ def _scan_forward(inputs, want_final, train):
 
 
 def _scan_layout(x, dt, A, B, C, D, z, dt_bias, initial):
-    dense = lambda v: None if v is None else v.contiguous()      # noqa: E731
-    return _rows(x), _rows(dt), A.contiguous(), _rows(B), _rows(C), dense(D), None if z is None else _rows(z), dense(dt_bias), dense(initial)
+    return (_rows(x), _rows(dt), A.contiguous(), _rows(B), _rows(C), None if D is None else D.contiguous(), None if z is None else _rows(z),
+            None if dt_bias is None else dt_bias.contiguous(), None if initial is None else initial.contiguous())
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -328,17 +358,23 @@ class _SelectiveScan(torch.autograd.Function):
 
 
 def _scan_parameters(channels, A, D, dt_bias, device):
-    _need(torch.is_tensor(A) and A.dim() == 2 and 1 <= A.shape[1] <= 64, 'A must be a tensor [channels, states] with 1 to 64 states')
-    _like('A', A, (channels, A.shape[1]), torch.float32, device)
-    for name, v in (('D', D), ('dt_bias', dt_bias)):
-        if v is not None:
-            _like(name, v, (channels,), torch.float32, device)
+    if not (isinstance(A, torch.Tensor) and A.dim() == 2 and 1 <= A.shape[1] <= 64):
+        raise ValueError('A must be a tensor [channels, states] with 1 to 64 states')
+    states = A.shape[1]
+    _like('A', A, (channels, states), torch.float32, device)
+    if D is not None:
+        _like('D', D, (channels,), torch.float32, device)
+    if dt_bias is not None:
+        _like('dt_bias', dt_bias, (channels,), torch.float32, device)
+    return states
 
 
 def _groups_of(channels, B, dims):
-    _need(torch.is_tensor(B) and B.dim() == dims, 'B must be a tensor of', dims, 'dimensions: [..., groups, states]')
+    if not (isinstance(B, torch.Tensor) and B.dim() == dims):
+        raise ValueError('B must be a tensor of %d dimensions: [..., groups, states]' % dims)
     groups = B.shape[-2]
-    _need(groups >= 1 and channels % groups == 0, channels, 'channels cannot be shared among', groups, 'groups of B and C')
+    if groups < 1 or channels % groups:
+        raise ValueError('%d channels cannot be shared among %d groups of B and C' % (channels, groups))
     return groups
 
 
@@ -354,9 +390,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     ``(y, final_state)``, the next window's ``initial_state`` and ``selective_scan_step``'s state.  Differentiable in every tensor but ``starts``; sums
     run in a fixed order, so gradients repeat bit for bit.  A differentiable call keeps the states in front of every 8th row for the backward pass."""
     _leading('x', x)
-    _need(x.dim() == 3, 'x must be [batch, time, channels], got', list(x.shape))
-    b, t, d = x.shape
-    _need(d > 0, 'x must have channels')
+    b, t, d = _window_rows(x)
     _like('dt', dt, (b, t, d), x.dtype, x.device)
     if z is not None:
         _like('z', z, (b, t, d), x.dtype, x.device)
@@ -380,31 +414,26 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
     """One row of each of ``x``'s environments: ``x, dt, z [rows, channels]``, ``B, C [rows, groups, states]``, ``state [environments, channels, states]``
     (float32, contiguous) moved on in place; ``env_ids`` and ``starts`` as in ``short_conv_step``.  Returns y [rows, channels]."""
     kind = _leading('x', x)
-    _need(x.dim() == 2 and x.shape[1] > 0, 'x must be [rows, channels], got', list(x.shape))
-    n, d = x.shape
-    _like('dt', dt, (n, d), x.dtype, x.device)
+    n, d = _step_rows(x)
+    dtype, device = x.dtype, x.device
+    _like('dt', dt, (n, d), dtype, device)
     if z is not None:
-        _like('z', z, (n, d), x.dtype, x.device)
-    _scan_parameters(d, A, D, dt_bias, x.device)
-    states, groups = A.shape[1], _groups_of(d, B, 3)
-    for name, v in (('B', B), ('C', C)):
-        _like(name, v, (n, groups, states), x.dtype, x.device)
-    if not torch.is_tensor(state):
-        raise TypeError('state must be a torch tensor, got %s' % type(state).__name__)
-    _need(state.dim() == 3, 'state must be [environments, channels, states], got', list(state.shape))
-    _like('state', state, (state.shape[0], d, states), torch.float32, x.device)
-    _need(state.is_contiguous(), 'state must be contiguous')
+        _like('z', z, (n, d), dtype, device)
+    states, groups = _scan_parameters(d, A, D, dt_bias, device), _groups_of(d, B, 3)
+    _like('B', B, (n, groups, states), dtype, device)
+    _like('C', C, (n, groups, states), dtype, device)
+    environments = _step_state(state, 'channels, states')
+    _like('state', state, (environments, d, states), torch.float32, device)
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
         raise ValueError('selective_scan_step has no gradient: call it under torch.no_grad(), or selective_scan on the window')
-    starts = _flags('starts', starts, (n,), x.device)
-    env_ids = _step_ids(env_ids, n, state.shape[0], x.device)
-    starts = None if starts is None else starts.contiguous()
+    starts = _step_flags(starts, n, device)
+    env_ids = _step_ids(env_ids, n, environments, device)
     x, dt, A, B, C, D, z, dt_bias, _ = _scan_layout(x, dt, A, B, C, D, z, dt_bias, None)
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, d))
     _call(_load().ppn_scan_step,
-          _SCAN_STEP.pack(_SCAN_STEP.size, kind, 1 if dt_softplus else 0, n, state.shape[0], d, groups, states, x.data_ptr(), x.stride(0), dt.data_ptr(),
+          _SCAN_STEP.pack(_SCAN_STEP.size, kind, 1 if dt_softplus else 0, n, environments, d, groups, states, x.data_ptr(), x.stride(0), dt.data_ptr(),
                           dt.stride(0), A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1), _ptr(D), _ptr(dt_bias),
-                          _ptr(z), 0 if z is None else z.stride(0), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), x.device)
+                          _ptr(z), 0 if z is None else z.stride(0), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
     return y
 
 
