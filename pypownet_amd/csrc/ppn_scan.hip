@@ -685,17 +685,17 @@ struct Split { int64_t chunk, chunks; };
 Split split_time(const ppn_scan_args* a, int64_t waves, int64_t wanted) {
   int64_t chunks = waves * 2 > wanted ? 1 : ceil_div(wanted, waves < 1 ? 1 : waves);
   int64_t chunk = ceil_div(ceil_div(a->time, chunks), ROWS) * ROWS;
-  if (chunk < 32) chunk = 32;
+  if (chunk < 16) chunk = 16;
   if (ceil_div(a->time, chunk) > 65535) chunk = ceil_div(ceil_div(a->time, 65535), ROWS) * ROWS;
   chunks = a->time ? ceil_div(a->time, chunk) : 1;
   return {chunk, chunks < 1 ? 1 : chunks};
 }
-Split forward_split(const ppn_scan_args* a) { return split_time(a, a->batch * a->groups * tiles_of(a), 4096); }
+Split forward_split(const ppn_scan_args* a) { return split_time(a, a->batch * a->groups * tiles_of(a), 3072); }
 
 struct BackwardPlan { Split split; int64_t rows_bytes, params_bytes, ends_bytes, sums_bytes; };
 BackwardPlan plan_backward(const ppn_scan_args* a) {
   BackwardPlan p;
-  p.split = split_time(a, a->batch * a->groups * tiles_of(a), 2048);
+  p.split = split_time(a, a->batch * a->groups * tiles_of(a), 4096);
   auto round = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int64_t cells = a->batch * p.split.chunks;
   p.rows_bytes = round(tiles_of(a) * a->batch * a->time * a->groups * 2 * states_of(a) * 4);
