@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(64) scan_join(ppn_scan_args a, int64_t chunks,
 // The rows are taken in blocks of 8 from the last to the first.  A block's states are recomputed from its checkpoint, four rows' worth kept in
 // registers at a time with 16 states a lane (5 x 16; the first four rows are walked twice for that: 8 % more work, and two waves fit a SIMD
 // where all eight rows' states left room for one), eight with 8 states.  The sums over channels (dB, dC) are the wave's part of them, one row of
-// partial sums per tile of channels, added up by scan_reduce_rows; dA, dD and ddt_bias stay in registers over the wave's rows and leave one
+// partial sums per tile of channels, added up by scan_reduce; dA, dD and ddt_bias stay in registers over the wave's rows and leave one
 // row of partial sums for each environment and chunk.  Both reductions run in a fixed order.
 //
 // ADJOINT: only what a chunk adds to the adjoint in front of it, and its sum of delta, for chunks that are worked on at once.
@@ -524,27 +524,36 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
   }
 }
 
-// dB and dC out of the tiles' partial rows [tiles x rows x 2 STATES], padded to the states of whole lanes.
+// The backward pass's partial sums added up, in a fixed order: the first `row_blocks` workgroups make dB and dC out of the tiles' rows [tiles x rows
+// x 2 STATES] (padded to the states of whole lanes; four states a lane), the others dA, dD and ddt_bias out of the waves' rows [shares x
+// (states + 2) x channels] (32 columns a workgroup, 8 lanes a column).  One launch: 63 MB and 38 MB take 20 and 15 us one after the other.
+struct ReduceArgs { const float* rows_in; int64_t tiles, rows; const float* params_in; int64_t shares, states, channels; void *dB, *dC; float *dA, *dD, *dbias; int64_t row_blocks; };
 template <typename T, int STATES>
-__global__ void __launch_bounds__(256) scan_reduce_rows(const float* in, int64_t tiles, int64_t rows, int64_t states, T* dB, T* dC) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, count = rows * 2 * STATES, row = id / (2 * STATES);
-  const int v = (int)(id % (2 * STATES)), n = v % STATES;
-  if (id >= count || n >= states) return;
-  float s = 0.0f;
-  for (int64_t t = 0; t < tiles; ++t) s += in[t * count + id];
-  (v < STATES ? dB : dC)[row * states + n] = (T)s;
-}
-
-// dA, dD, ddt_bias out of the workgroups' partial rows [shares x (states + 2) x channels].
-__global__ void __launch_bounds__(256) scan_reduce_params(const float* in, int64_t shares, int64_t states, int64_t channels, float* dA, float* dD, float* dbias) {
-  const int64_t columns = (states + 2) * channels, col = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
+__global__ void __launch_bounds__(256) scan_reduce(ReduceArgs a) {
+  if (blockIdx.x < a.row_blocks) {
+    const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, count = a.rows * 2 * STATES, row = id / (2 * STATES);
+    const int v = (int)(id % (2 * STATES)), n = v % STATES;
+    if (id >= count || n >= a.states) return;
+    float4 s = {0, 0, 0, 0};
+    for (int64_t t = 0; t < a.tiles; ++t) {
+      const float4 part = *(const float4*)(a.rows_in + t * count + id);
+      s.x += part.x, s.y += part.y, s.z += part.z, s.w += part.w;
+    }
+    T* out = (T*)(v < STATES ? a.dB : a.dC) + row * a.states + n;
+    const float sums[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.states) out[i] = (T)sums[i];
+    return;
+  }
+  const int64_t columns = (a.states + 2) * a.channels, col = ((int64_t)blockIdx.x - a.row_blocks) * 32 + threadIdx.x % 32;
   const int part = threadIdx.x / 32;
   float s = 0.0f;
   if (col < columns)
-    for (int64_t r = part; r < shares; r += 64) {
+    for (int64_t r = part; r < a.shares; r += 64) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = r + 8 * i < shares ? in[(r + 8 * i) * columns + col] : 0.0f;
+      for (int i = 0; i < 8; ++i) v[i] = r + 8 * i < a.shares ? a.params_in[(r + 8 * i) * columns + col] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[i];
     }
@@ -553,13 +562,13 @@ __global__ void __launch_bounds__(256) scan_reduce_params(const float* in, int64
   __syncthreads();
   if (part == 0 && col < columns) {
     for (int q = 1; q < 8; ++q) s += sums[q][threadIdx.x];
-    const int64_t n = col / channels, d = col - n * channels;
-    if (n < states) {
-      if (dA) dA[d * states + n] = s;
-    } else if (n == states) {
-      if (dD) dD[d] = s;
-    } else if (dbias) {
-      dbias[d] = s;
+    const int64_t n = col / a.channels, d = col - n * a.channels;
+    if (n < a.states) {
+      if (a.dA) a.dA[d * a.states + n] = s;
+    } else if (n == a.states) {
+      if (a.dD) a.dD[d] = s;
+    } else if (a.dbias) {
+      a.dbias[d] = s;
     }
   }
 }
@@ -781,7 +790,7 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
   float* ends = (float*)(w + p.rows_bytes + p.params_bytes);
   float* sums = (float*)(w + p.rows_bytes + p.params_bytes + p.ends_bytes);
   const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels, count = a->batch * a->time * a->groups * 2 * states_of(a);
-  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff || ceil_div(count, 256) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many rows");
+  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff || ceil_div(count, 1024) > 0x70000000) return fail(PPN_E_INVALID, "scan: too many rows");
   const dim3 grid(waves, p.split.chunks);
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
@@ -793,9 +802,10 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
         scan_join<true><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
       }
       scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, split ? ends : nullptr, nullptr, nullptr, rows, params);
-      scan_reduce_rows<T, NS * LPC><<<dim3(ceil_div(count, 256)), dim3(256), 0, (hipStream_t)stream>>>(rows, tiles_of(a), a->batch * a->time * a->groups, a->states, (T*)a->dB, (T*)a->dC);
-      scan_reduce_params<<<dim3(ceil_div((a->states + 2) * a->channels, 32)), dim3(256), 0, (hipStream_t)stream>>>(params, a->batch * p.split.chunks, a->states,
-                                                                                                                   a->channels, a->dA, a->dD, a->ddt_bias);
+      const int64_t row_blocks = ceil_div(count, 1024);
+      const ReduceArgs r = {rows, tiles_of(a), a->batch * a->time * a->groups, params, a->batch * p.split.chunks, a->states, a->channels, a->dB, a->dC, a->dA, a->dD,
+                            a->ddt_bias, row_blocks};
+      scan_reduce<T, NS * LPC><<<dim3(row_blocks + ceil_div((a->states + 2) * a->channels, 32)), dim3(256), 0, (hipStream_t)stream>>>(r);
       return launched("ppn_scan_backward");
     });
   });

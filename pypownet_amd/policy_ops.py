@@ -64,10 +64,18 @@ def _refused(rc):
     raise (ValueError if rc == -1 else EngineError)(text)
 
 
-def _workspace(size, device):
+_LAST_TWO = struct.Struct('2q')
+
+
+def _with_workspace(size_of, function, packed, device):
+    """Queues `function`, which needs as much memory as `size_of` says: the last two of its arguments."""
+    size = size_of(packed)
     if size < 0:
         _refused(size)
-    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    if size:
+        work = torch.empty((size,), dtype=torch.uint8, device=device)
+        packed = packed[:-16] + _LAST_TWO.pack(work.data_ptr(), size)
+    _call(function, packed, device)
 
 
 def _ptr(t):
@@ -75,11 +83,6 @@ def _ptr(t):
 
 
 # ---- arguments -----------------------------------------------------------------------------------------------------------------------
-
-def _need(condition, *text):
-    if not condition:
-        raise ValueError(' '.join(str(t) for t in text))
-
 
 def _leading(name, x):
     """The tensor that names a call's type and device."""
@@ -183,12 +186,10 @@ def _step_ids(env_ids, rows, environments, device):
 
 # ---- short causal convolution --------------------------------------------------------------------------------------------------------
 
-def _conv_args(x, weight, bias, initial, starts, silu, y=None, final=None, dy=None, dfinal=None, dx=None, dweight=None, dbias=None, dinitial=None,
-               workspace=None):
+def _conv_args(x, weight, bias, initial, starts, silu, y=None, final=None, dy=None, dfinal=None, dx=None, dweight=None, dbias=None, dinitial=None):
     b, t, d = x.shape
     return _CONV.pack(_CONV.size, _TYPES[x.dtype], silu, b, t, d, weight.shape[1], *_at(x), weight.data_ptr(), _ptr(bias), _ptr(initial), *_at(starts),
-                      *_at(y), _ptr(final), *_at(dy), _ptr(dfinal), *_at(dx), _ptr(dweight), _ptr(dbias), _ptr(dinitial), _ptr(workspace),
-                      0 if workspace is None else workspace.numel())
+                      *_at(y), _ptr(final), *_at(dy), _ptr(dfinal), *_at(dx), _ptr(dweight), _ptr(dbias), _ptr(dinitial), 0, 0)
 
 
 def _conv_forward(x, weight, bias, initial, starts, silu, want_final):
@@ -219,10 +220,9 @@ class _ShortConv(torch.autograd.Function):
         dx, dweight = _window_like(x), torch.empty_like(weight)
         dbias = None if bias is None else torch.empty_like(bias)
         dinitial = None if initial is None else torch.empty_like(initial)
-        given = dict(dy=dy, dfinal=dfinal, dx=dx, dweight=dweight, dbias=dbias, dinitial=dinitial)
         lib = _load()
-        work = _workspace(lib.ppn_conv_backward_workspace(_conv_args(x, weight, bias, initial, starts, ctx.silu, **given)), x.device)
-        _call(lib.ppn_conv_backward, _conv_args(x, weight, bias, initial, starts, ctx.silu, workspace=work, **given), x.device)
+        _with_workspace(lib.ppn_conv_backward_workspace, lib.ppn_conv_backward,
+                        _conv_args(x, weight, bias, initial, starts, ctx.silu, None, None, dy, dfinal, dx, dweight, dbias, dinitial), x.device)
         return dx, dweight, dbias, dinitial, None, None, None
 
 
@@ -293,12 +293,15 @@ def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, 
 # ---- selective scan ------------------------------------------------------------------------------------------------------------------
 
 def _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, soft, y=None, final=None, marks=None, dy=None, dfinal=None, dx=None, ddt=None, dz=None,
-               dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dinitial=None, workspace=None):
+               dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dinitial=None):
     b, t, d = x.shape
     return _SCAN.pack(_SCAN.size, _TYPES[x.dtype], soft, b, t, d, B.shape[2], A.shape[1], *_at(x), *_at(dt), A.data_ptr(),
                       B.data_ptr(), B.stride(0), B.stride(1), B.stride(2), C.data_ptr(), C.stride(0), C.stride(1), C.stride(2), _ptr(D), _ptr(dt_bias),
                       *_at(z), *_at(starts), _ptr(initial), *_at(y), _ptr(final), _ptr(marks), *_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz),
-                      _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dinitial), _ptr(workspace), 0 if workspace is None else workspace.numel())
+                      _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dinitial), 0, 0)
+
+
+_CHECKPOINT_ROWS = 8
 
 
 def _scan_forward(inputs, want_final, train):
@@ -306,12 +309,10 @@ def _scan_forward(inputs, want_final, train):
     lib = _load()
     y = _window_like(x)
     final = torch.empty((x.shape[0],) + tuple(A.shape), dtype=torch.float32, device=x.device) if want_final else None
-    probe = _scan_args(*inputs)
     marks = None
-    if train:
-        marks = torch.empty((lib.ppn_scan_checkpoint_bytes(probe) // 4,), dtype=torch.float32, device=x.device)
-    work = _workspace(lib.ppn_scan_forward_workspace(probe), x.device)
-    _call(lib.ppn_scan_forward, _scan_args(*inputs, y=y, final=final, marks=marks, workspace=work), x.device)
+    if train:      # (ppn_scan_checkpoint_bytes)
+        marks = torch.empty((x.shape[0], -(-x.shape[1] // _CHECKPOINT_ROWS), A.shape[1], A.shape[0]), dtype=torch.float32, device=x.device)
+    _with_workspace(lib.ppn_scan_forward_workspace, lib.ppn_scan_forward, _scan_args(*inputs, y, final, marks), x.device)
     return y, final, marks
 
 
@@ -340,7 +341,7 @@ class _SelectiveScan(torch.autograd.Function):
         dfinal = None if dfinal is None else dfinal.contiguous()
         dx, ddt, dz = _window_like(x), _window_like(dt), None if z is None else _window_like(z)
         dA, dD, dbias, dinitial = empty(A), empty(D), empty(dt_bias), empty(initial)
-        dB, dC = (torch.empty(v.shape, dtype=v.dtype, device=v.device) for v in (B, C))
+        dB, dC = B.new_empty(B.shape), C.new_empty(C.shape)
         if x.shape[0] == 0 or x.shape[1] == 0:          # no rows: the state passes through
             for v in (dA, dD, dbias):
                 if v is not None:
@@ -349,11 +350,10 @@ class _SelectiveScan(torch.autograd.Function):
                 dinitial.zero_() if dfinal is None else dinitial.copy_(dfinal)
             return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
-        inputs = (x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft)
-        given = dict(marks=marks, dy=dy, dfinal=dfinal, dx=dx, ddt=ddt, dz=dz, dB=dB, dC=dC, dA=dA, dD=dD, ddt_bias=dbias, dinitial=dinitial)
         lib = _load()
-        work = _workspace(lib.ppn_scan_backward_workspace(_scan_args(*inputs)), x.device)
-        _call(lib.ppn_scan_backward, _scan_args(*inputs, workspace=work, **given), x.device)
+        _with_workspace(lib.ppn_scan_backward_workspace, lib.ppn_scan_backward,
+                        _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft, None, None, marks, dy, dfinal, dx, ddt, dz, dB, dC, dA, dD, dbias,
+                                   dinitial), x.device)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
 
 
@@ -439,18 +439,18 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
 
 # ---- cross entropy over a catalogue of actions -----------------------------------------------------------------------------------------
 
-def _loss_args(hidden, weight, target, allowed, ignore, loss=None, lse=None, dloss=None, dhidden=None, dweight=None, workspace=None):
+def _loss_args(hidden, weight, target, allowed, ignore, loss=None, lse=None, dloss=None, dhidden=None, dweight=None):
     return _LOSS.pack(_LOSS.size, _TYPES[hidden.dtype], hidden.shape[0], weight.shape[0], hidden.shape[1], ignore, hidden.data_ptr(), hidden.stride(0),
                       weight.data_ptr(), weight.stride(0), target.data_ptr(), _ptr(allowed), 0 if allowed is None else allowed.stride(0), _ptr(loss),
-                      _ptr(lse), _ptr(dloss), _ptr(dhidden), _ptr(dweight), _ptr(workspace), 0 if workspace is None else workspace.numel())
+                      _ptr(lse), _ptr(dloss), _ptr(dhidden), _ptr(dweight), 0, 0)
 
 
 def _loss_forward(hidden, weight, target, allowed, ignore):
-    n = hidden.shape[0]
-    loss, lse = (torch.empty((n,), dtype=torch.float32, device=hidden.device) for _ in range(2))
+    n, device = hidden.shape[0], hidden.device
+    loss = torch.empty((n,), dtype=torch.float32, device=device)
+    lse = torch.empty((n,), dtype=torch.float32, device=device)
     lib = _load()
-    work = _workspace(lib.ppn_loss_forward_workspace(_loss_args(hidden, weight, target, allowed, ignore)), hidden.device)
-    _call(lib.ppn_loss_forward, _loss_args(hidden, weight, target, allowed, ignore, loss, lse, workspace=work), hidden.device)
+    _with_workspace(lib.ppn_loss_forward_workspace, lib.ppn_loss_forward, _loss_args(hidden, weight, target, allowed, ignore, loss, lse), device)
     return loss, lse
 
 
@@ -467,14 +467,13 @@ class _ActionCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss):
         hidden, weight, target, allowed, loss, lse = ctx.saved_tensors
-        dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if ctx.needs_input_grad[0] else None
-        dweight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if ctx.needs_input_grad[1] else None
+        dhidden = hidden.new_empty(hidden.shape) if ctx.needs_input_grad[0] else None
+        dweight = weight.new_empty(weight.shape) if ctx.needs_input_grad[1] else None
         if hidden.shape[0] == 0:
             return dhidden, None if dweight is None else dweight.zero_(), None, None, None
-        given = (hidden, weight, target, allowed, ctx.ignore)
         lib = _load()
-        work = _workspace(lib.ppn_loss_backward_workspace(_loss_args(*given)), hidden.device)
-        _call(lib.ppn_loss_backward, _loss_args(*given, loss=loss, lse=lse, dloss=dloss.contiguous(), dhidden=dhidden, dweight=dweight, workspace=work), hidden.device)
+        _with_workspace(lib.ppn_loss_backward_workspace, lib.ppn_loss_backward,
+                        _loss_args(hidden, weight, target, allowed, ctx.ignore, loss, lse, dloss.contiguous(), dhidden, dweight), hidden.device)
         return dhidden, dweight, None, None, None
 
 
@@ -488,9 +487,11 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
     and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
     NaN.  ``-loss`` is the log-probability of the action ``target``.  Differentiable in hidden and weight; sums run in a fixed order."""
     _leading('hidden', hidden)
-    _need(hidden.dim() == 2 and hidden.shape[1] > 0, 'hidden must be [rows, features], got', list(hidden.shape))
+    if hidden.dim() != 2 or hidden.shape[1] == 0:
+        raise ValueError('hidden must be [rows, features], got %s' % list(hidden.shape))
     n, f = hidden.shape
-    _need(torch.is_tensor(weight) and weight.dim() == 2 and weight.shape[0] > 0, 'weight must be a tensor [actions, features]')
+    if not (isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] > 0):
+        raise ValueError('weight must be a tensor [actions, features]')
     v = weight.shape[0]
     _like('weight', weight, (v, f), hidden.dtype, hidden.device)
     _like('target', target, (n,), torch.int64, hidden.device)
@@ -506,7 +507,8 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
 
 def pack_allowed(mask):
     """``mask [rows, actions]`` (bool) as the bits ``action_cross_entropy`` takes: int32 ``[rows, ceil(actions / 32)]``, action v in bit v % 32 of word v // 32."""
-    _need(torch.is_tensor(mask) and mask.dim() == 2, 'mask must be a tensor [rows, actions]')
+    if not (torch.is_tensor(mask) and mask.dim() == 2):
+        raise ValueError('mask must be a tensor [rows, actions]')
     n, v = mask.shape
     words = (v + 31) // 32
     bits = torch.nn.functional.pad(mask != 0, (0, words * 32 - v)).view(n, words, 4, 8)

@@ -5,6 +5,7 @@ Tolerances.  A result is computed in 32 bits and rounded once to its type t: hal
 argument, which is below 8 in size here).  A result whose longest chain has c such operations, none of whose intermediate sums exceeds `size`, is
 therefore within 2 c 2^-24 size; `size` is the same formula over absolute values, in 64 bits, or an upper bound of it."""
 import os
+import struct
 import subprocess
 import tempfile
 
@@ -165,6 +166,17 @@ def test_entry_points_refuse_a_bad_struct():
     ready = dict(loss, hidden=16, weight=16, target=16, loss=16, lse=16, dloss=16, workspace=256, workspace_bytes=255, hidden_row=4, weight_row=4)
     assert lib.ppn_loss_forward(packed('ppn_loss_args', **ready), None) == -1 and b'workspace' in lib.ppn_policy_error()
     assert lib.ppn_loss_backward(packed('ppn_loss_args', **ready), None) == -1 and b'workspace' in lib.ppn_policy_error()
+
+
+@pytest.mark.parametrize('shape', [(1, 1, 1, 1, 1), (3, 17, 200, 2, 12), (5, 8, 64, 1, 64), (2, 0, 7, 1, 3)])
+def test_checkpoints_are_as_large_as_the_library_says(shape):
+    from pypownet_amd import _lib, policy_ops as ops
+    b, t, d, g, n = shape
+    lib = _lib.load_library()
+    fields = _lib.POLICY_STRUCTS['ppn_scan_args']
+    values = dict(struct_bytes=8 * len(fields), batch=b, time=t, channels=d, groups=g, states=n)
+    args = struct.pack('%dq' % len(fields), *[values.get(f, 0) for f in fields])
+    assert lib.ppn_scan_checkpoint_bytes(args) == 4 * b * -(-t // ops._CHECKPOINT_ROWS) * n * d
 
 
 def test_policy_kernels_mir_has_no_vector_code_in_front_of_an_exec_restore():
