@@ -110,6 +110,9 @@ template <int V, int LPC> struct Kept {
 // an offset: strides of time are at most 2^27 elements, as the entry points check.
 template <typename V> __device__ inline V& at(const void* base, unsigned bytes) { return *(V*)((char*)base + bytes); }
 
+// Loads waited for here: else the first round's waits, which have few operations behind them, stand in every round of the loop that follows.
+template <typename V> __device__ inline void settled(V& v) { asm volatile("" : "+v"(v)); }
+
 // ROWS rows of B and C of one environment and group, as 32-bit floats in LDS, zero beyond the last state: fetched into registers while the
 // rows before are worked on, put into LDS when their turn comes.
 template <typename T, int STATES, bool WITH_B, bool WITH_C> struct Staged {
@@ -197,7 +200,9 @@ template <int NS, int LPC> __device__ inline Place place(const ppn_scan_args& a)
 // Row-major [.. x channels x states] tensors of the caller (A, initial and final states).
 template <int NS> __device__ inline void load_states(const float* p, int64_t states, int part, float (&v)[NS]) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) v[n] = part * NS + n < states ? p[part * NS + n] : 0.0f;
+  for (int n = 0; n < NS; ++n) v[n] = p[min(part * NS + n, (int)states - 1)];      // (a branch for the last ones would wait for each load in turn)
+#pragma unroll
+  for (int n = 0; n < NS; ++n) v[n] = part * NS + n < (int)states ? v[n] : 0.0f;
 }
 template <int NS> __device__ inline void store_states(float* p, int64_t states, int part, const float (&v)[NS]) {
 #pragma unroll
@@ -206,14 +211,20 @@ template <int NS> __device__ inline void store_states(float* p, int64_t states, 
 }
 // Workspace states: [.. x states x channels], so that a wave's lanes write next to each other.  Places past the last state are read as the last one
 // (and do not matter: B and C are zero there).
-template <int NS> __device__ inline void load_plane(const float* p, int64_t states, int64_t channels, unsigned d, int part, float (&v)[NS]) {
+template <int NS, int LPC> __device__ inline void load_plane(const float* p, int64_t states, int64_t channels, unsigned d, int part, float (&v)[NS]) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) v[n] = at<const float>(p, ((unsigned)min(part * NS + n, (int)states - 1) * (unsigned)channels + d) * 4u);
+  for (int n = 0; n < NS; ++n) {
+    if constexpr (LPC == 1) v[n] = at<const float>(p + min(n, (int)states - 1) * channels, d * 4u);
+    else v[n] = at<const float>(p, ((unsigned)min(part * NS + n, (int)states - 1) * (unsigned)channels + d) * 4u);
+  }
 }
-template <int NS> __device__ inline void store_plane(float* p, int64_t states, int64_t channels, unsigned d, int part, const float (&v)[NS]) {
+template <int NS, int LPC> __device__ inline void store_plane(float* p, int64_t states, int64_t channels, unsigned d, int part, const float (&v)[NS]) {
 #pragma unroll
   for (int n = 0; n < NS; ++n)
-    if (part * NS + n < (int)states) at<float>(p, ((unsigned)(part * NS + n) * (unsigned)channels + d) * 4u) = v[n];
+    if (part * NS + n < (int)states) {
+      if constexpr (LPC == 1) at<float>(p + n * channels, d * 4u) = v[n];
+      else at<float>(p, ((unsigned)(part * NS + n) * (unsigned)channels + d) * 4u) = v[n];
+    }
 }
 
 // softplus of a block's step sizes at once (one branch); rows past the block's last one: 0.
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
 #pragma unroll
   for (int n = 0; n < NS; ++n) A2[n] *= LOG2E, h[n] = 0.0f;
   if constexpr (MODE != SUMMARY) {
-    if (entering) load_plane<NS>(entering + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
+    if (entering) load_plane<NS, LPC>(entering + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
     else if (a.initial) load_states<NS>(a.initial + (p.b * a.channels + p.d) * a.states, a.states, p.part, h);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
@@ -270,9 +281,11 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
   const T* pC = (const T*)a.C + p.b * a.C_batch + p.g * a.C_group + t0 * a.C_time;
   T* py = (T*)a.y + p.b * a.y_batch + t0 * a.y_time;
   float* pmark = MODE == TRAIN ? a.checkpoints + (p.b * ((a.time + ROWS - 1) / ROWS) + t0 / ROWS) * plane : nullptr;
-  const unsigned y_step = (unsigned)a.y_time * (unsigned)sizeof(T);
+  const unsigned y_step = (unsigned)a.y_time;
   float total = 0.0f;
   bool cut = false;
+#pragma unroll
+  for (int n = 0; n < NS; ++n) settled(A2[n]), settled(h[n]);
   for (int64_t t = t0; t < t1; t += ROWS) {
     const int rows = (int)min(t1 - t, (int64_t)ROWS);
     Column<T> x, dt, z;
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
     bc.put((int)a.states, sb, sc);
     __syncthreads();
     if constexpr (MODE == TRAIN) {
-      store_plane<NS>(pmark, a.states, a.channels, p.d, p.part, h);
+      store_plane<NS, LPC>(pmark, a.states, a.channels, p.d, p.part, h);
       pmark += plane;
     }
 #pragma unroll
@@ -314,13 +327,13 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
         read_states<NS>(sc + j * STATES + p.part * NS, cv);
 #pragma unroll
         for (int n = 0; n < NS; ++n) s += cv[n] * h[n];
-        at<T>(py, (unsigned)min(j, rows - 1) * y_step + p.d * (unsigned)sizeof(T)) = (T)((sum_parts<LPC>(s) + skip * xv) * gate[j]);
+        at<T>(py + (uint64_t)((unsigned)min(j, rows - 1) * y_step), p.d * (unsigned)sizeof(T)) = (T)((sum_parts<LPC>(s) + skip * xv) * gate[j]);
       }
     }
     py += ROWS * a.y_time;
   }
   if constexpr (MODE == SUMMARY) {
-    store_plane<NS>(ends + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
+    store_plane<NS, LPC>(ends + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
     sums[((p.b * chunks + k) * 2 + 0) * a.channels + p.d] = total;
     sums[((p.b * chunks + k) * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
   } else if (a.final_state && t1 == a.time) {
@@ -401,13 +414,15 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
 #pragma unroll
   for (int n = 0; n < NS; ++n) A2[n] *= LOG2E, dA[n] = 0.0f, e[n] = 0.0f;
   if constexpr (!ADJOINT) {
-    if (entering) load_plane<NS>(entering + cell * plane, a.states, a.channels, p.d, p.part, e);
+    if (entering) load_plane<NS, LPC>(entering + cell * plane, a.states, a.channels, p.d, p.part, e);
     else if (a.dfinal) load_states<NS>(a.dfinal + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
   const unsigned mine = p.d * (unsigned)sizeof(T);
   float dskip = 0.0f, dbias = 0.0f, total = 0.0f;
   bool cut = false;
+#pragma unroll
+  for (int n = 0; n < NS; ++n) settled(A2[n]), settled(e[n]);
   for (; t >= first; t -= ROWS) {
     const int rows = (int)min(last - t, (int64_t)ROWS);
     Column<T> x, dt, z, dy;
@@ -415,7 +430,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
     float mark[NS], h[ADJOINT ? 1 : KEPT + 1][NS], delta[ROWS];
     dt.fetch(pdt, dt_time, p.d, rows);
     bc.fetch(a, pB, pC, rows);
-    if constexpr (!ADJOINT) load_plane<NS>(pmark, a.states, a.channels, p.d, p.part, mark);
+    if constexpr (!ADJOINT) load_plane<NS, LPC>(pmark, a.states, a.channels, p.d, p.part, mark);
     if constexpr (!ADJOINT) x.fetch(px, x_time, p.d, rows);
     dy.fetch(pdy, dy_time, p.d, rows);
     z.fetch(pz, z_time, p.d, rows);
@@ -512,13 +527,13 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
     if constexpr (!ADJOINT) pdx -= ROWS * dx_time, pddt -= ROWS * ddt_time, pdz -= ROWS * dz_time, pout -= ROWS * pair;
   }
   if constexpr (ADJOINT) {
-    store_plane<NS>(ends + cell * plane, a.states, a.channels, p.d, p.part, e);
+    store_plane<NS, LPC>(ends + cell * plane, a.states, a.channels, p.d, p.part, e);
     sums[(cell * 2 + 0) * a.channels + p.d] = total;
     sums[(cell * 2 + 1) * a.channels + p.d] = cut ? 1.0f : 0.0f;
   } else {
     if (a.dinitial && first == 0) store_states<NS>(a.dinitial + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
     float* out = params_out + cell * (a.states + 2) * a.channels;
-    store_plane<NS>(out, a.states, a.channels, p.d, p.part, dA);
+    store_plane<NS, LPC>(out, a.states, a.channels, p.d, p.part, dA);
     out[a.states * a.channels + p.d] = dskip;
     out[(a.states + 1) * a.channels + p.d] = dbias;
   }
