@@ -10,6 +10,11 @@
 //   dl and dl^T against transposed copies of weight and hidden -> the two gradients.
 // The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size.
 //
+// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 538 us (750 TFLOP/s), the second 920 us (440; it
+// writes 1.6 GB), the third 1.05 ms for both (770).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
+// alone, 466 and 325 us for the other two.  A third of the first kind's time is its epilogue (10 vector instructions a logit), which nothing else
+// covers: one workgroup fills a CU.
+//
 // Rounding dl to 16 bits (as the operand of a 16-bit product it has to be) is off by half a step of each entry, 2^-9 for bfloat16 and
 // 2^-12 for float16, independent from entry to entry; the gradients' own rounding is as large.  float16's range would lose small
 // probabilities, so dl is scaled by a power of two that brings the largest |dloss| to 2^14, and the scale is taken out at the end.
@@ -551,11 +556,12 @@ bool in_place(const void* p, int64_t row, int64_t features, int64_t type) {
 }
 
 // 256 x 256 tiles (a workgroup to a CU) where they fill three quarters of the chip's 256 CUs, since the larger the tile, the less is read from the
-// L2 and from LDS for an operation; else 128 x 128, else 64 x 64.  times: workgroups that can share the inner dimension of a tile.
+// L2 and from LDS for an operation; else 128 x 128, else 64 x 64.  The logits at 256, 128 and 64, in us: 128, 137, 177 for 4096 x 24129 x 512; 23, 26, 29
+// for 999 x 12099 x 392 (192 tiles of 256); 37, 13, 6 for 256 x 347 x 128 in 32 bits.
 struct Config { int64_t tile, columns_per_wave; };
-Config config_for(int64_t m, int64_t n, int64_t times) {
-  if (ceil_div(m, 256) * ceil_div(n, 256) * times >= 192) return {256, 64};
-  if (ceil_div(m, 128) * ceil_div(n, 128) * times >= 192) return {128, 64};
+Config config_for(int64_t m, int64_t n) {
+  if (ceil_div(m, 256) * ceil_div(n, 256) >= 192) return {256, 64};
+  if (ceil_div(m, 128) * ceil_div(n, 128) >= 192) return {128, 64};
   return {64, 32};
 }
 // f(fragments of a wave across the rows, across the columns, waves across the columns; two across the rows)
@@ -574,7 +580,7 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
   Layout l;
   const int64_t size = size_of(a->type);
   p.features_padded = padded(a->features, part(a));
-  p.config = config_for(a->rows, a->actions, 1);
+  p.config = config_for(a->rows, a->actions);
   p.columns = padded(a->actions, p.config.tile) / p.config.columns_per_wave;
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
   p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
@@ -599,13 +605,15 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   p.rows_padded = padded(a->rows, 64);
   p.actions_padded = padded(a->actions, 64);
   // A piece's dl and its transpose take 256 MB each.  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
-  // of dweight's: 16384 rows of 24129 actions take 3.65, 3.02, 2.71, 2.44 and 2.33 ms behind the loss at 32, 64, 128, 256 and 512 MB.
+  // of dweight's: 16384 rows of 24129 actions took 3.65, 3.02, 2.71 and 2.44 ms behind the loss at 32, 64, 128 and 256 MB; with both products in a
+  // launch 256, 512 and 1024 MB are within 2 % of each other.
   p.piece = padded((int64_t)(256 << 20) / (p.rows_padded * size), 128);
   if (p.piece < 1024) p.piece = 1024;
   if (p.piece > p.actions_padded) p.piece = p.actions_padded;
-  p.grad = config_for(a->rows, p.piece, 1);
+  p.grad = config_for(a->rows, p.piece);
   // The second products: the largest tile with which shares of at least 512 of the inner dimensions make 192 workgroups of the two, then the
-  // shortest share with which they are at most 256 (512 of the smaller tiles, of which two and more fit a CU).
+  // shortest share with which they are at most 256 (512 of the smaller tiles, of which two and more fit a CU).  At 256, 128 and 64, in us: 45, 51, 96
+  // for 999 x 12099 x 392; 105, 35, 12 for 256 x 347 x 128 in 32 bits.
   const int64_t most[] = {256, 512, 512}, tiles[] = {256, 128, 64};
   for (int i = 0; i < 3; ++i) {
     p.sums = {tiles[i], 0};

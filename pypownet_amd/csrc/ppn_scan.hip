@@ -3,11 +3,15 @@
 //   h[t,d,n] = exp(delta A[d,n]) h[t-1,d,n] + delta B[t,n] x[t,d]      delta = softplus(dt + dt_bias)
 //   y[t,d]   = (sum_n C[t,n] h[t,d,n] + D[d] x[t,d]) silu(z[t,d])
 //
-// Bound by the vector units: every element (environment, row, channel) takes one exponential and three multiply-adds per state,
-// against 4 elements moved.  The exponential runs at a quarter of the multiply-add's rate, so 16 states cost 128 slots of 4 clocks a
-// wave and row.  Hence: one lane owns one channel with all its states in registers (two or four lanes above 16 and 32 states), nothing
-// is exchanged between lanes in the forward pass, and B and C (the same for all lanes of a wave) are read once per wave and 8 rows,
-// widened to 32 bits in LDS and broadcast from there.  Workgroups are single waves: no barrier is waited for.
+// Bound by the vector units: every element (environment, row, channel) takes one exponential (2.7 slots of 4 clocks a wave, counted) and four
+// multiplications and additions per state, against 4 elements moved: 8 instructions a state forward, 27 backward, with all that is done once a
+// row.  Hence: one lane owns one channel with all its states in registers (two or four lanes above 16 and 32 states), nothing is
+// exchanged between lanes in the forward pass, and B and C (the same for all lanes of a wave) are read once per wave and 8 rows, widened
+// to 32 bits in LDS and broadcast from there.  Workgroups are single waves: no barrier is waited for.
+//
+// A window of 1024 x 60 rows of 512 bfloat16 channels with 16 states, for training: forward 205 us (60 % of the vector units' time; 520 MB, half of them
+// checkpoints), backward 554 us (75 %), the sums 27 us.  Twice 8724 rows of 768 float16 channels, no gradients: 54 us for the chunks' ends, 17 us to
+// join them, 67 us for y.  Fetching a block ahead, into registers or straight into LDS, made none of these faster.
 #include "ppn_policy.h"
 
 namespace ppn_policy {
@@ -113,8 +117,8 @@ template <typename V> __device__ inline V& at(const void* base, unsigned bytes) 
 // Loads waited for here: else the first round's waits, which have few operations behind them, stand in every round of the loop that follows.
 template <typename V> __device__ inline void settled(V& v) { asm volatile("" : "+v"(v)); }
 
-// ROWS rows of B and C of one environment and group, as 32-bit floats in LDS, zero beyond the last state: fetched into registers while the
-// rows before are worked on, put into LDS when their turn comes.
+// ROWS rows of B and C of one environment and group, as 32-bit floats in LDS, zero beyond the last state: fetched into registers with the block's
+// other loads, put into LDS when all are in.
 template <typename T, int STATES, bool WITH_B, bool WITH_C> struct Staged {
   static constexpr int COUNT = ROWS * STATES / 64;
   T b[COUNT], c[COUNT];
@@ -683,7 +687,8 @@ __global__ void __launch_bounds__(256) scan_step(ppn_scan_step_args a) {
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------------------------
-// States per lane and lanes per channel.
+// States per lane and lanes per channel.  All in one lane where the registers take it: 8 states in each of two lanes bring a third wave to a SIMD, but
+// every row's own work twice (backward, 16 states: 641 us against 600 at that time).
 template <typename F> int by_states(int64_t states, F f) {
   if (states <= 8) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
   if (states <= 16) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
@@ -704,7 +709,8 @@ int64_t states_of(const ppn_scan_args* a) {
 }
 
 // Chunks of time that are worked on at once: one while the waves of (environment, tile) alone fill the chip, since splitting walks the rows
-// twice; else as many as bring `wanted` waves, of at least 32 rows.
+// twice; else as many as bring `wanted` waves, of at least 16 rows.  Forward 3072 (2 x 8724 rows x 768: 138, 139, 143 and 154 us at 2048, 3072,
+// 4096 and 6144; 75 x 167 rows x 200: 54, 50, 48 at the first three), backward 4096 (the latter: 107, 103, 96 us at 1024, 2048, 4096).
 struct Split { int64_t chunk, chunks; };
 Split split_time(const ppn_scan_args* a, int64_t waves, int64_t wanted) {
   int64_t chunks = waves * 2 > wanted ? 1 : ceil_div(wanted, waves < 1 ? 1 : waves);

@@ -14,7 +14,8 @@ forms take one row of each listed environment and update that environment's stat
 Tensors are float32, bfloat16 or float16 on the GPU, all activations of a call of one type; parameters (convolution weights, ``A``, ``D``,
 ``dt_bias``) and states are float32 -- the convolution's window excepted, which holds rows and has their type.  Kernels are queued on torch's
 current stream of the tensors' device; nothing synchronises.  Workspaces come from torch's allocator, so the calls can be captured into a
-graph.  Arguments the kernels do not take are refused with TypeError / ValueError before anything is launched; gradients of gradients are
+graph -- a training step as usual with its own leaves: capturing a backward pass of leaves that an eager graph still holds ends in an error of torch's
+autograd, here as with any other function.  Arguments the kernels do not take are refused with TypeError / ValueError before anything is launched; gradients of gradients are
 not available.
 """
 import struct
