@@ -368,66 +368,114 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
   const int column = p.lane & 15;
-  T* dl = (T*)g.dl + m0 * g.dl_row + n0;
-  T* dlt = (T*)g.dlt + n0 * g.dlt_row + m0;
   const unsigned dl_row = (unsigned)g.dl_row * sizeof(T), dlt_row = (unsigned)g.dlt_row * sizeof(T);
-  auto write = [&](auto flag) {
-    constexpr bool EDGE = decltype(flag)::value;
+  char* dl = (char*)g.dl + (m0 * g.dl_row + n0) * (int64_t)sizeof(T);
+  char* dlt = (char*)g.dlt + (n0 * g.dlt_row + m0) * (int64_t)sizeof(T);
+  auto entry = [&](int i, int j, int r) {
+    const Row q = rows[p.row_of(i, r)];
+    const float v = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2) * q.up;
+    return (T)chosen(mask[p.row_of(i, r)][p.wave_n / 32 + j / 2], column + (j & 1 ? 16 : 0), v, 0);
+  };
+  // The entry of a row's target, exact where the probability is near one: (column of the tile, or -1; value).
+  struct Hit { int at; T v; };
+  auto target_of = [&](int r) {
+    Hit hit = {-1, (T)0.0f};
+    if (m0 + r >= o.M || g.lse[m0 + r] == INFINITY) return hit;
+    const int64_t target = g.target[m0 + r] - g.first - n0;
+    if (target < 0 || target >= P::BN || n0 + target >= o.N || !((mask[r][target / 32] >> (target & 31)) & 1)) return hit;
+    const float loss = g.loss[m0 + r];
+    hit.at = (int)target;
+    hit.v = (T)((loss != loss ? loss : expm1f(-loss)) * rows[r].up);
+    return hit;
+  };
+  if constexpr (sizeof(T) == 2) {
+    // The tile goes out through LDS, where the operands were, once by rows and once by columns, 16 bytes a lane and whole lines: straight from the
+    // registers it would be runs of 32 bytes (312 us against 260 for a piece of 16384 x 8192).  A line's 16-byte parts are exchanged as in the
+    // product, so that the lanes of a write fall into different banks.
+    constexpr int ROW = P::BN * 2, COL = P::BM * 2, CHUNKS = P::BM * P::BN / 8, EACH = CHUNKS / P::THREADS, BATCH = EACH < 4 ? EACH : 4;
+    static_assert(P::BM * P::BN * 2 <= P::LDS_BYTES && P::BM <= P::THREADS && EACH % BATCH == 0, "the tile fits where the operands were");
+    auto in_row = [&](int row, int bytes) { return row * ROW + ((((bytes >> 4) ^ (row >> 1 & 7)) << 4) | (bytes & 15)); };
+    auto in_col = [&](int col, int bytes) { return col * COL + ((((bytes >> 4) ^ (col & 7)) << 4) | (bytes & 15)); };
+    unsigned q[MI][NI][2];
+    Hit hit = {-1, (T)0.0f};
+    if (threadIdx.x < P::BM) hit = target_of(threadIdx.x);
+    __syncthreads();      // (the last fragments have been read)
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      T out[NI][4];
-      const int row0 = p.row_of(i, 0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const Row q = rows[row0 + r];
-        const unsigned* word = mask[row0 + r] + p.wave_n / 32;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const float v = __builtin_amdgcn_exp2f(p.c[i][j][r] * LOG2E - q.lse2) * q.up;
-          out[j][r] = (T)chosen(word[j / 2], column + (j & 1 ? 16 : 0), v, 0);
-        }
-      }
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int col = p.col_of(j);
-        if (!EDGE || (n0 + col < o.N && m0 + row0 < g.rows_padded)) {      // rows_padded is a multiple of 16: the four rows are in or out together
-          struct alignas(4 * sizeof(T)) Quad { T v[4]; } f = {{out[j][0], out[j][1], out[j][2], out[j][3]}};
-          *(Quad*)((char*)dlt + (col * dlt_row + row0 * (unsigned)sizeof(T))) = f;
-        }
-        if constexpr (sizeof(T) == 2) {
-          const unsigned a = pair(out[j][0], out[j][1]), b = pair(out[j][2], out[j][3]);
-          const bool odd = column & 1;
-          const unsigned keep = odd ? b : a, got = from_neighbour(odd ? a : b);
-          const unsigned left = odd ? got : keep, right = odd ? keep : got;      // columns col & ~1 and the next, two rows each
-          const unsigned lower = __builtin_amdgcn_perm(right, left, 0x05040100), upper = __builtin_amdgcn_perm(right, left, 0x07060302);
-          const int row = row0 + (odd ? 2 : 0);
-          char* at = (char*)dl + (row * dl_row + (col & ~1) * 2u);
-          const bool in = !EDGE || n0 + col < g.cols_padded;
-          if (in && (!EDGE || m0 + row < o.M)) *(unsigned*)at = lower;
-          if (in && (!EDGE || m0 + row + 1 < o.M)) *(unsigned*)(at + dl_row) = upper;
-        } else {
+        const unsigned a = pair(entry(i, j, 0), entry(i, j, 1)), b = pair(entry(i, j, 2), entry(i, j, 3));
+        q[i][j][0] = a, q[i][j][1] = b;
+        const bool odd = column & 1;
+        const unsigned keep = odd ? b : a, got = from_neighbour(odd ? a : b);
+        const unsigned left = odd ? got : keep, right = odd ? keep : got;      // columns col & ~1 and the next, two rows each
+        const unsigned lower = __builtin_amdgcn_perm(right, left, 0x05040100), upper = __builtin_amdgcn_perm(right, left, 0x07060302);
+        const int row = p.row_of(i, 0) + (odd ? 2 : 0), at = (p.col_of(j) & ~1) * 2;
+        *(unsigned*)(lds + in_row(row, at)) = lower;
+        *(unsigned*)(lds + in_row(row + 1, at)) = upper;
+      }
+    __syncthreads();
+    if (hit.at >= 0) *(T*)(lds + in_row(threadIdx.x, hit.at * 2)) = hit.v;
+    __syncthreads();
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!EDGE || (m0 + row0 + r < o.M && n0 + col < g.cols_padded)) *(T*)((char*)dl + ((row0 + r) * dl_row + col * (unsigned)sizeof(T))) = out[j][r];
-        }
+    for (int k = 0; k < EACH; k += BATCH) {
+      u32x4 part[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int id = threadIdx.x + (k + u) * P::THREADS;
+        part[u] = *(const u32x4*)(lds + in_row(id / (ROW / 16), id % (ROW / 16) * 16));
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int id = threadIdx.x + (k + u) * P::THREADS, row = id / (ROW / 16), at = id % (ROW / 16) * 16;
+        if (m0 + row < o.M && n0 + at / 2 < g.cols_padded) *(u32x4*)(dl + (row * dl_row + at)) = part[u];
       }
     }
-  };
-  if (m0 + P::BM <= o.M && n0 + P::BN <= o.N) write(std::false_type());
-  else write(std::true_type());
-  // the targets' entries, behind the tile's own stores
-  __threadfence_block();
-  __syncthreads();
-  for (int r = threadIdx.x; r < P::BM; r += P::THREADS) {
-    if (m0 + r >= o.M) break;
-    const int64_t target = g.target[m0 + r] - g.first - n0;
-    if (target < 0 || target >= P::BN || n0 + target >= o.N || g.lse[m0 + r] == INFINITY) continue;
-    const int t = (int)target;
-    if (!((mask[r][t / 32] >> (t & 31)) & 1)) continue;
-    const float loss = g.loss[m0 + r];
-    const T v = (T)((loss != loss ? loss : expm1f(-loss)) * rows[r].up);
-    *(T*)((char*)dl + (r * dl_row + t * (unsigned)sizeof(T))) = v;
-    *(T*)((char*)dlt + (t * dlt_row + r * (unsigned)sizeof(T))) = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) *(uint2*)(lds + in_col(p.col_of(j), p.row_of(i, 0) * 2)) = uint2{q[i][j][0], q[i][j][1]};
+    __syncthreads();
+    if (hit.at >= 0) *(T*)(lds + in_col(hit.at, threadIdx.x * 2)) = hit.v;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EACH; k += BATCH) {
+      u32x4 part[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int id = threadIdx.x + (k + u) * P::THREADS;
+        part[u] = *(const u32x4*)(lds + in_col(id / (COL / 16), id % (COL / 16) * 16));
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int id = threadIdx.x + (k + u) * P::THREADS, col = id / (COL / 16), at = id % (COL / 16) * 16;
+        if (n0 + col < o.N && m0 + at / 2 < g.rows_padded) *(u32x4*)(dlt + (col * dlt_row + at)) = part[u];
+      }
+    }
+  } else {
+    const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int row0 = p.row_of(i, 0), col = p.col_of(j);
+        const f32x4 f = {entry(i, j, 0), entry(i, j, 1), entry(i, j, 2), entry(i, j, 3)};
+        if (whole || (n0 + col < o.N && m0 + row0 < g.rows_padded))      // rows_padded is a multiple of 16: the four rows are in or out together
+          *(f32x4*)(dlt + (col * dlt_row + row0 * 4u)) = f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (whole || (m0 + row0 + r < o.M && n0 + col < g.cols_padded)) *(float*)(dl + ((row0 + r) * dl_row + col * 4u)) = f[r];
+      }
+    // the targets' entries, behind the tile's own stores
+    __threadfence_block();
+    __syncthreads();
+    for (int r = threadIdx.x; r < P::BM; r += P::THREADS) {
+      const Hit hit = target_of(r);
+      if (hit.at < 0) continue;
+      *(float*)(dl + (r * dl_row + hit.at * 4u)) = hit.v;
+      *(float*)(dlt + (hit.at * dlt_row + r * 4u)) = hit.v;
+    }
   }
 }
 
@@ -644,7 +692,8 @@ int check(const ppn_loss_args* a) {
   if (!a || a->struct_bytes != (int64_t)sizeof *a) return fail(PPN_E_INVALID, "ppn_loss_args: struct_bytes does not match this library");
   if (a->type < 0 || a->type > PPN_T_F16) return fail(PPN_E_INVALID, "element type %lld is unknown", (long long)a->type);
   if (a->rows < 0 || a->actions < 1 || a->features < 1) return fail(PPN_E_INVALID, "loss: rows >= 0, actions >= 1 and features >= 1 are needed");
-  if (a->rows > (1 << 21) || a->actions > (1 << 23) || a->features > (1 << 20)) return fail(PPN_E_INVALID, "loss: a size is out of range");
+  if (a->rows > (1 << 22) || a->actions > (1 << 23) || a->features > (1 << 20))
+    return fail(PPN_E_INVALID, "loss: at most 2^22 rows, 2^23 actions and 2^20 features, got %lld, %lld and %lld", (long long)a->rows, (long long)a->actions, (long long)a->features);
   return PPN_OK;
 }
 

@@ -37,6 +37,8 @@ __device__ inline float softplus(float v) {
 // id an earlier row has (or that is out of range) must not move the state on a second time: it is refused with NaN.  The ids in front of
 // the row are compared one a lane; at 4096 rows that is 8 KB a workgroup on average, out of the L2.
 // A caller may read the state before it knows (row_env has checked the range); it may not write it.
+// Every row is compared with all in front of it, so a call with ids has a most (a minute's work would be 2^24 rows).
+constexpr int MOST_IDS = 1 << 18;
 enum { ROW_LIVE = 0, ROW_PADDING = 1, ROW_REFUSED = 2 };
 __device__ inline int64_t row_env(const int32_t* env_ids, int64_t row, int64_t environments) {      // an environment that exists, the row's if it is live
   const int64_t id = env_ids ? env_ids[row] : row;

@@ -838,6 +838,7 @@ extern "C" int ppn_scan_step(const ppn_scan_step_args* a, void* stream) {
     return fail(PPN_E_INVALID, "ppn_scan_step: a size is out of range");
   if (a->states < 1 || a->states > 64) return fail(PPN_E_INVALID, "states must be 1..64, got %lld", (long long)a->states);
   if (!a->env_ids && a->rows > a->environments) return fail(PPN_E_INVALID, "ppn_scan_step: more rows than environments and no env_ids");
+  if (a->env_ids && a->rows > MOST_IDS) return fail(PPN_E_INVALID, "ppn_scan_step: at most %d rows with env_ids", MOST_IDS);
   if (a->rows == 0) return PPN_OK;
   if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || !a->state || !a->environments) return fail(PPN_E_INVALID, "ppn_scan_step: x, dt, A, B, C, state (of one environment at least) and y are needed");
   const int64_t four = 4 * size_of(a->type);
