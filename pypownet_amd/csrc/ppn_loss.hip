@@ -10,10 +10,10 @@
 //   dl and dl^T against transposed copies of weight and hidden -> the two gradients.
 // The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size.
 //
-// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 538 us (750 TFLOP/s), the second 920 us (440; it
-// writes 1.6 GB), the third 1.05 ms for both (770).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
-// alone, 466 and 325 us for the other two.  A third of the first kind's time is its epilogue (10 vector instructions a logit), which nothing else
-// covers: one workgroup fills a CU.
+// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 485 us (835 TFLOP/s), the second 765 us (530; it
+// writes 1.6 GB), the third 940 us for both (860).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
+// alone, 466 and 325 us for the other two.  4096 rows: 112 us, and 83 of those are the product without its epilogue (10 vector instructions a logit),
+// which the other workgroups of a CU cover in part.
 //
 // Rounding dl to 16 bits (as the operand of a 16-bit product it has to be) is off by half a step of each entry, 2^-9 for bfloat16 and
 // 2^-12 for float16, independent from entry to entry; the gradients' own rounding is as large.  float16's range would lose small
@@ -61,16 +61,18 @@ __device__ const u32x4 zeros = {0, 0, 0, 0};
 
 constexpr int LINE = 128;         // bytes of the inner dimension per stage: a cache line, so that none is brought twice
 
-// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go from memory straight into LDS, into one of two
-// buffers, one stage ahead; a stage is multiplied in two halves, and a half's fragments are read into registers during the half before it, so
-// the matrix units wait for neither.  One barrier a stage.  A line's eight 16-byte parts are stored with part ^ (row % 8), so that the
-// rows a fragment read touches fall into different banks; the transfer writes 64 lanes' 16 bytes in a row (8 lines), so the exchange is
-// made in the addresses it reads.
+// Tile of 16 MI WM x 16 NI WN by WM x WN waves of 16 MI x 16 NI.  Both operands' lines go from memory straight into LDS, a stage of one line a row
+// at a time.  A stage's fragments are all read into registers, so that the next stage's lines can come in its place while the matrix units work;
+// what is waited for in between (the lines' way, the reads), and the epilogue, is covered by the other workgroups of the CU: two of 256 x 128,
+// three of 128 x 128.  (Two buffers, a stage ahead, leave room for one workgroup of 256 x 256: 129 us against 112 for the logits of 4096 x 24129
+// x 512, whose epilogue then stands alone, and 343 against 313 for the gradients' products of 16384 x 8192 x 512.)  A line's eight 16-byte parts
+// are stored with part ^ (row % 8), so that the rows a fragment read touches fall into different banks; the transfer writes 64 lanes' 16 bytes in
+// a row (8 lines), so the exchange is made in the addresses it reads.
 template <typename T, int MI, int NI, int WM, int WN> struct Product {
   static constexpr int BM = 16 * MI * WM, BN = 16 * NI * WN, THREADS = 64 * WM * WN;
-  static constexpr int GROUPS = (BM + BN) / 8, LOADS = GROUPS / (WM * WN);      // transfers of 8 lines: in all, and per wave
-  static constexpr int STAGE = (BM + BN) * LINE, LDS_BYTES = 2 * STAGE;
-  static_assert(GROUPS % (WM * WN) == 0 && BM % (8 * LOADS) == 0, "a wave's lines belong to one operand");
+  static constexpr int OF_A = BM / 8 / (WM * WN), OF_B = BN / 8 / (WM * WN), LOADS = OF_A + OF_B;      // a wave's transfers of 8 lines
+  static constexpr int LDS_BYTES = (BM + BN) * LINE;
+  static_assert(OF_A * 8 * WM * WN == BM && OF_B * 8 * WM * WN == BN, "the lines are shared out evenly");
 
   f32x4 c[MI][NI];
   int wave_m, wave_n, lane;
@@ -101,30 +103,35 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) c[i][j] = f32x4{0, 0, 0, 0};
-    // this wave's lines: 8 LOADS neighbouring ones of one operand; lines past the last one read the last one again
-    const int line0 = wave * LOADS * 8, row = lane >> 3;
-    const bool left = line0 < BM;
-    const int64_t first = left ? m0 + line0 : n0 + line0 - BM, rows = left ? o.M : o.N, ld = (left ? o.lda : o.ldb) * (int64_t)sizeof(T);
-    const int64_t top = first < rows ? first : rows - 1;
-    const int spare = (int)(rows - 1 - top < 8 * LOADS ? rows - 1 - top : 8 * LOADS);
-    const char* base = scalar((const char*)(left ? o.A : o.B) + top * ld + k0 * (int64_t)sizeof(T));
-    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + line0 * LINE);
-    unsigned offset[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) offset[i] = (unsigned)min(8 * i + row, spare) * (unsigned)ld + (((lane & 7) ^ row) << 4);
+    // this wave's lines: 8 OF_A neighbouring ones of A, 8 OF_B of B; lines past the last one read the last one again
+    const int row = lane >> 3, swap = ((lane & 7) ^ row) << 4;
+    const unsigned start = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const unsigned to_a = __builtin_amdgcn_readfirstlane(start + wave * (OF_A * 8 * LINE)), to_b = __builtin_amdgcn_readfirstlane(start + (BM + wave * (OF_B * 8)) * LINE);
+    const int64_t first_a = m0 + wave * (OF_A * 8), first_b = n0 + wave * (OF_B * 8);
+    const int64_t top_a = first_a < o.M ? first_a : o.M - 1, top_b = first_b < o.N ? first_b : o.N - 1;
+    const int spare_a = (int)(o.M - 1 - top_a < 8 * OF_A ? o.M - 1 - top_a : 8 * OF_A), spare_b = (int)(o.N - 1 - top_b < 8 * OF_B ? o.N - 1 - top_b : 8 * OF_B);
+    const char* base_a = scalar((const char*)o.A + (top_a * o.lda + k0) * (int64_t)sizeof(T));
+    const char* base_b = scalar((const char*)o.B + (top_b * o.ldb + k0) * (int64_t)sizeof(T));
+    const unsigned ld_a = (unsigned)(o.lda * sizeof(T)), ld_b = (unsigned)(o.ldb * sizeof(T)), mine_a = row * ld_a + swap, mine_b = row * ld_b + swap;
+    const bool whole = spare_a >= 8 * OF_A - 1 && spare_b >= 8 * OF_B - 1;
     const int bytes = (int)((k1 - k0) * (int64_t)sizeof(T)), stages = (bytes + LINE - 1) / LINE;
     auto fetch = [&](int stage) {
-      const unsigned at = to + (stage & 1) * STAGE;
       const int left_over = bytes - stage * LINE;
-      if (left_over >= LINE) {
+      if (whole && left_over >= LINE) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) transfer(at + i * 8 * LINE, base, offset[i]);
+        for (int i = 0; i < OF_A; ++i) transfer(to_a + i * 8 * LINE, base_a + (uint64_t)i * 8 * ld_a, mine_a);
+#pragma unroll
+        for (int i = 0; i < OF_B; ++i) transfer(to_b + i * 8 * LINE, base_b + (uint64_t)i * 8 * ld_b, mine_b);
       } else {
-        const bool in = (((lane & 7) ^ row) << 4) < left_over;
+        const bool in = swap < left_over;
+        int here = row;
+        asm volatile("" : "+v"(here));      // (the addresses are made here: kept over the loop they do not fit the registers)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) transfer(at + i * 8 * LINE, in ? base + offset[i] : (const char*)&zeros);
+        for (int i = 0; i < OF_A; ++i) transfer(to_a + i * 8 * LINE, in ? base_a + (unsigned)min(8 * i + here, spare_a) * ld_a + swap : (const char*)&zeros);
+#pragma unroll
+        for (int i = 0; i < OF_B; ++i) transfer(to_b + i * 8 * LINE, in ? base_b + (unsigned)min(8 * i + here, spare_b) * ld_b + swap : (const char*)&zeros);
       }
-      base += LINE;
+      base_a += LINE, base_b += LINE;
     };
     struct Fragments { u32x4 a[MI], b[NI]; };
     int at_a[2], at_b[2];      // where this lane's fragments begin, by half; rows 16 apart have the same row % 8
@@ -133,13 +140,11 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
       at_a[h] = spot(wave_m + (lane & 15), 4 * h + (lane >> 4));
       at_b[h] = spot(BM + wave_n + (lane & 15), 4 * h + (lane >> 4));
     }
-    auto read = [&](Fragments& f, int stage, int h) {
-      const char* buf = lds + (stage & 1) * STAGE;
+    auto read = [&](Fragments& f, int h) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) f.b[j] = *(const u32x4*)(buf + at_b[h] + j * 16 * LINE);
+      for (int j = 0; j < NI; ++j) f.b[j] = *(const u32x4*)(lds + at_b[h] + j * 16 * LINE);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) f.a[i] = *(const u32x4*)(buf + at_a[h] + i * 16 * LINE);
-      __builtin_amdgcn_sched_barrier(0);      // (issued here: the compiler would put each in front of its use)
+      for (int i = 0; i < MI; ++i) f.a[i] = *(const u32x4*)(lds + at_a[h] + i * 16 * LINE);
     };
     auto multiply_all = [&](const Fragments& f) {
 #pragma unroll
@@ -148,19 +153,15 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
         for (int j = 0; j < NI; ++j) multiply(c[i][j], f.a[i], f.b[j], T());
     };
     fetch(0);
-    if (stages > 1) fetch(1);
-    if (stages > 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    Fragments even, odd;
-    read(even, 0, 0);
     for (int s = 0; s < stages; ++s) {
-      read(odd, s, 1);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the stage's lines are in, every wave's
+      Fragments even, odd;
+      read(even, 0);
+      read(odd, 1);
+      // Every wave has the stage's fragments in registers: the next stage's lines may come in their place.
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 1 < stages) fetch(s + 1);
       multiply_all(even);
-      // The next stage's lines are in, for every wave once all have passed the barrier; and every wave has this stage's fragments in registers, so
-      // that the transfers of the stage after the next may overwrite its buffer.  (Behind the last stage an old buffer is read again.)
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 2 < stages) fetch(s + 2);
-      read(even, s + 1, 0);
       multiply_all(odd);
     }
   }
@@ -249,7 +250,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsA
       const unsigned* word = mask[p.row_of(i, r)] + p.wave_n / 32;
 #pragma unroll
       for (int j = 0; j < NI; ++j) l[r][j] = chosen(word[j / 2], j & 1 ? next : column, p.c[i][j][r], (int)0xff800000);      // -infinity
-      if constexpr (NI == 4) top[r] = most(most(l[r][0], l[r][1], l[r][2]), l[r][3]);
+      if constexpr (NI == 8) top[r] = most(most(most(l[r][0], l[r][1], l[r][2]), l[r][3], l[r][4]), most(l[r][5], l[r][6], l[r][7]));
+      else if constexpr (NI == 4) top[r] = most(most(l[r][0], l[r][1], l[r][2]), l[r][3]);
       else top[r] = most(l[r][0], l[r][1]);
     }
     max_over_16(top);
@@ -352,7 +354,8 @@ template <typename T, int MI, int NI, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArgs g, unsigned tiles_m, unsigned tiles_n) {
   typedef Product<T, MI, NI, WM, WN> P;
   struct Row { float lse2, up; };
-  __shared__ __align__(16) char lds[P::LDS_BYTES];
+  constexpr int OUT = sizeof(T) == 2 ? P::BM * P::BN * 2 : 0;
+  __shared__ __align__(16) char lds[P::LDS_BYTES > OUT ? P::LDS_BYTES : OUT];
   __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
   __shared__ __align__(16) Row rows[P::BM];
   unsigned tm, tn;
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
     // registers it would be runs of 32 bytes (312 us against 260 for a piece of 16384 x 8192).  A line's 16-byte parts are exchanged as in the
     // product, so that the lanes of a write fall into different banks.
     constexpr int ROW = P::BN * 2, COL = P::BM * 2, CHUNKS = P::BM * P::BN / 8, EACH = CHUNKS / P::THREADS, BATCH = EACH < 4 ? EACH : 4;
-    static_assert(P::BM * P::BN * 2 <= P::LDS_BYTES && P::BM <= P::THREADS && EACH % BATCH == 0, "the tile fits where the operands were");
+    static_assert(P::BM <= P::THREADS && EACH % BATCH == 0, "the tile fits where the operands were");
     auto in_row = [&](int row, int bytes) { return row * ROW + ((((bytes >> 4) ^ (row >> 1 & 7)) << 4) | (bytes & 15)); };
     auto in_col = [&](int col, int bytes) { return col * COL + ((((bytes >> 4) ^ (col & 7)) << 4) | (bytes & 15)); };
     unsigned q[MI][NI][2];
@@ -603,21 +606,21 @@ bool in_place(const void* p, int64_t row, int64_t features, int64_t type) {
   return features % (16 / size_of(type)) == 0 && row * size_of(type) % 16 == 0 && row <= (1 << 23) && aligned(p, 16);
 }
 
-// 256 x 256 tiles (a workgroup to a CU) where they fill three quarters of the chip's 256 CUs, since the larger the tile, the less is read from the
-// L2 and from LDS for an operation; else 128 x 128, else 64 x 64.  The logits at 256, 128 and 64, in us: 128, 137, 177 for 4096 x 24129 x 512; 23, 26, 29
-// for 999 x 12099 x 392 (192 tiles of 256); 37, 13, 6 for 256 x 347 x 128 in 32 bits.
-struct Config { int64_t tile, columns_per_wave; };
-Config config_for(int64_t m, int64_t n) {
-  if (ceil_div(m, 256) * ceil_div(n, 256) >= 192) return {256, 64};
-  if (ceil_div(m, 128) * ceil_div(n, 128) >= 192) return {128, 64};
-  return {64, 32};
-}
-// f(fragments of a wave across the rows, across the columns, waves across the columns; two across the rows)
-template <int MI, int NI, int WN> struct Shape { static constexpr int mi = MI, ni = NI, wn = WN, threads = 128 * WN; };
+struct Config { int64_t m, n, columns_per_wave; };
+constexpr Config LARGE = {256, 128, 64}, MEDIUM = {128, 128, 128}, SMALL = {64, 64, 32};
+// The logits: 128 x 128 tiles where they make one and a half workgroups a CU, else 64 x 64.  At 256 x 128, 128 and 64, in us: 116, 112, 151 for 4096 x
+// 24129 x 512; 22, 21, 28 for 999 x 12099 x 392; -, 13, 6 for 256 x 347 x 128 in 32 bits.  The waves are 32 x 128: the epilogue's sums over a
+// row's columns cost half of what they do in 64 x 64.
+Config config_for(int64_t m, int64_t n) { return ceil_div(m, 128) * ceil_div(n, 128) >= 384 ? MEDIUM : SMALL; }
+// f(fragments of a wave across the rows, across the columns, waves across the rows, across the columns)
+template <int MI, int NI, int WM, int WN> struct Shape { static constexpr int mi = MI, ni = NI, wm = WM, wn = WN; };
 template <typename F> void by_tile(const Config& c, F f) {
-  if (c.tile == 256) f(Shape<8, 4, 4>());
-  else if (c.tile == 128) f(Shape<4, 4, 2>());
-  else f(Shape<2, 2, 2>());
+  if (c.m == 128) f(Shape<2, 8, 4, 1>());
+  else f(Shape<2, 2, 2, 2>());
+}
+template <typename F> void by_large_tile(const Config& c, F f) {
+  if (c.m == 256) f(Shape<8, 4, 2, 2>());
+  else by_tile(c, f);
 }
 
 struct Layout { int64_t bytes = 0; int64_t take(int64_t n) { int64_t at = bytes; bytes += padded(n, 256); return at; } };
@@ -629,7 +632,7 @@ ForwardPlan plan_forward(const ppn_loss_args* a) {
   const int64_t size = size_of(a->type);
   p.features_padded = padded(a->features, part(a));
   p.config = config_for(a->rows, a->actions);
-  p.columns = padded(a->actions, p.config.tile) / p.config.columns_per_wave;
+  p.columns = padded(a->actions, p.config.n) / p.config.columns_per_wave;
   p.hidden = in_place(a->hidden, a->hidden_row, a->features, a->type) ? -1 : l.take(a->rows * p.features_padded * size);
   p.weight = in_place(a->weight, a->weight_row, a->features, a->type) ? -1 : l.take(a->actions * p.features_padded * size);
   p.partial = l.take(a->rows * p.columns * 8);
@@ -658,19 +661,19 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   p.piece = padded((int64_t)(256 << 20) / (p.rows_padded * size), 128);
   if (p.piece < 1024) p.piece = 1024;
   if (p.piece > p.actions_padded) p.piece = p.actions_padded;
-  p.grad = config_for(a->rows, p.piece);
-  // The second products: the largest tile with which shares of at least 512 of the inner dimensions make 192 workgroups of the two, then the
-  // shortest share with which they are at most 256 (512 of the smaller tiles, of which two and more fit a CU).  At 256, 128 and 64, in us: 45, 51, 96
-  // for 999 x 12099 x 392; 105, 35, 12 for 256 x 347 x 128 in 32 bits.
-  const int64_t most[] = {256, 512, 512}, tiles[] = {256, 128, 64};
+  // dl: 256 x 128 where two rounds of them fill the chip (16384 x 8192: 255 us, 269 in 128 x 128; 999 x 12099: 27 and 25)
+  p.grad = ceil_div(a->rows, 256) * ceil_div(p.piece, 128) >= 1024 ? LARGE : config_for(a->rows, p.piece);
+  // The second products: the largest tile with which shares of at least 512 of the inner dimensions make 384 workgroups of the two, then the
+  // shortest share with which they are at most 512.  At 256 x 128, 128 and 64, in us: 48, 55, 113 for 999 x 12099 x 392; -, 35, 12 for 256 x 347 x
+  // 128 in 32 bits.
   for (int i = 0; i < 3; ++i) {
-    p.sums = {tiles[i], 0};
-    const int64_t across = ceil_div(a->features, tiles[i]), dh = ceil_div(a->rows, tiles[i]) * across, dw = ceil_div(p.piece, tiles[i]) * across;
+    p.sums = i == 0 ? LARGE : i == 1 ? MEDIUM : SMALL;
+    const int64_t across = ceil_div(a->features, p.sums.n), dh = ceil_div(a->rows, p.sums.m) * across, dw = ceil_div(p.piece, p.sums.m) * across;
     auto blocks = [&](int64_t share) { return dh * ceil_div(p.piece, share) + dw * ceil_div(p.rows_padded, share); };
-    if (i < 2 && blocks(512) < 192) continue;
+    if (i < 2 && blocks(512) < 384) continue;
     p.share = 512;
     const int64_t longest = p.piece > p.rows_padded ? p.piece : p.rows_padded;
-    while (p.share < longest && blocks(p.share) > most[i]) p.share += 128;
+    while (p.share < longest && blocks(p.share) > 512) p.share += 128;
     break;
   }
   p.dh_slots = ceil_div(p.piece, p.share), p.dw_slots = ceil_div(p.rows_padded, p.share);
@@ -735,9 +738,9 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
       o.B = w + p.weight, o.ldb = p.features_padded;
     }
     const StatsArgs st = {a->allowed, a->allowed_row, (float2*)(w + p.partial), p.columns};
-    const int64_t tm = ceil_div(a->rows, p.config.tile), tn = ceil_div(a->actions, p.config.tile);
+    const int64_t tm = ceil_div(a->rows, p.config.m), tn = ceil_div(a->actions, p.config.n);
     if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
-    by_tile(p.config, [&](auto t) { loss_stats<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(tm * tn), dim3(decltype(t)::threads), 0, s>>>(o, st, tm, tn); });
+    by_tile(p.config, [&](auto t) { loss_stats<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn); });
     loss_join<T><<<dim3(ceil_div(a->rows, 16)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
     return launched("ppn_loss_forward");
   });
@@ -781,12 +784,12 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 64);
       const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
       const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->loss, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
-      const int64_t tm = ceil_div(a->rows, p.grad.tile), tn = ceil_div(n, p.grad.tile);
-      by_tile(p.grad, [&](auto t) { loss_grad<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(tm * tn), dim3(decltype(t)::threads), 0, s>>>(o, g, tm, tn); });
-      const int64_t across = ceil_div(a->features, p.sums.tile);
+      const int64_t tm = ceil_div(a->rows, p.grad.m), tn = ceil_div(n, p.grad.n);
+      by_large_tile(p.grad, [&](auto t) { loss_grad<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn); });
+      const int64_t across = ceil_div(a->features, p.sums.n);
       // (the last piece is shorter: a share that begins past its end adds nothing, and every slot has been written by the first piece)
       auto job = [&](const Operands& q, int64_t at, void* out, bool wanted, bool add) {
-        const int64_t down = ceil_div(q.M, p.sums.tile);
+        const int64_t down = ceil_div(q.M, p.sums.m);
         return SumJob{q, (float*)(w + at), out, p.share, (unsigned)down, (unsigned)across, wanted ? (unsigned)(down * across * ceil_div(q.K, p.share)) : 0u, add};
       };
       const SumJob dh = job({w + p.dl, p.piece, a->rows, (const T*)(w + p.weight_t) + first, p.actions_padded, a->features, np}, p.dh,
@@ -795,7 +798,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
       const SumJob dw = job({w + p.dlt, p.rows_padded, n, w + p.hidden_t, p.rows_padded, a->features, p.rows_padded}, p.dw,
                             p.direct_dw ? dw_out : nullptr, a->dweight, false);
       if (dh.blocks + dw.blocks)
-        by_tile(p.sums, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, 2, decltype(t)::wn><<<dim3(dh.blocks + dw.blocks), dim3(decltype(t)::threads), 0, s>>>(dh, dw, scale); });
+        by_large_tile(p.sums, [&](auto t) { loss_sums<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(dh.blocks + dw.blocks), dim3(256), 0, s>>>(dh, dw, scale); });
       const bool last = first + p.piece >= a->actions;
       const FinishJob fh = {(const float*)(w + p.dh), p.dh_slots, last && a->dhidden && !p.direct_dh ? a->rows * a->features : 0, a->dhidden};
       const FinishJob fw = {(const float*)(w + p.dw), p.dw_slots, a->dweight && !p.direct_dw ? n * a->features : 0, dw_out};
