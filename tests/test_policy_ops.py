@@ -168,14 +168,43 @@ def test_entry_points_refuse_a_bad_struct():
     assert lib.ppn_loss_backward(packed('ppn_loss_args', **ready), None) == -1 and b'workspace' in lib.ppn_policy_error()
 
 
+def packed_args(name, **values):
+    from pypownet_amd import _lib
+    fields = _lib.POLICY_STRUCTS[name]
+    values.setdefault('struct_bytes', 8 * len(fields))
+    assert set(values) <= set(fields)
+    return struct.pack('%dq' % len(fields), *[values.get(f, 0) for f in fields])
+
+
+def test_entry_points_refuse_what_is_too_large():
+    """... before anything is launched: the pointers here are none."""
+    from pypownet_amd import _lib
+    lib = _lib.load_library()
+    conv = dict(rows=1, environments=1 << 19, channels=4, taps=4, x=16, weight=16, y=16, state=16)
+    scan = dict(rows=1, environments=1 << 19, channels=4, groups=1, states=4, x=16, dt=16, A=16, B=16, C=16, y=16, state=16)
+    for name, function, values in (('ppn_conv_step_args', lib.ppn_conv_step, conv), ('ppn_scan_step_args', lib.ppn_scan_step, scan)):
+        assert function(packed_args(name, **dict(values, rows=(1 << 18) + 1, env_ids=16)), None) == -1 and b'env_ids' in lib.ppn_policy_error()
+        assert function(packed_args(name, **dict(values, rows=(1 << 19) + 1)), None) == -1 and b'more rows than environments' in lib.ppn_policy_error()
+        assert function(packed_args(name, **dict(values, channels=(1 << 24) + 4)), None) == -1
+    loss = dict(rows=1, actions=1, features=1)
+    for field, most in (('rows', 22), ('actions', 23), ('features', 20)):
+        args = packed_args('ppn_loss_args', **dict(loss, **{field: (1 << most) + 1}))
+        assert lib.ppn_loss_forward(args, None) == -1 and ('2^%d %s' % (most, field)).encode() in lib.ppn_policy_error()
+        assert lib.ppn_loss_forward_workspace(args) == -1 and lib.ppn_loss_backward_workspace(args) == -1
+    window = dict(batch=1, time=1, channels=1, groups=1, states=1)
+    for values in (dict(window, channels=(1 << 22) + 1), dict(window, x_time=(1 << 27) + 1), dict(window, states=65), dict(window, groups=2)):
+        args = packed_args('ppn_scan_args', **values)
+        assert lib.ppn_scan_forward(args, None) == -1 and lib.ppn_scan_backward_workspace(args) == -1 and lib.ppn_scan_checkpoint_bytes(args) == -1
+    args = packed_args('ppn_conv_args', batch=(1 << 31) - 300, time=1, channels=1, taps=2, x=16, weight=16, y=16)
+    assert lib.ppn_conv_forward(args, None) == -1 and b'environments' in lib.ppn_policy_error()
+
+
 @pytest.mark.parametrize('shape', [(1, 1, 1, 1, 1), (3, 17, 200, 2, 12), (5, 8, 64, 1, 64), (2, 0, 7, 1, 3)])
 def test_checkpoints_are_as_large_as_the_library_says(shape):
     from pypownet_amd import _lib, policy_ops as ops
     b, t, d, g, n = shape
     lib = _lib.load_library()
-    fields = _lib.POLICY_STRUCTS['ppn_scan_args']
-    values = dict(struct_bytes=8 * len(fields), batch=b, time=t, channels=d, groups=g, states=n)
-    args = struct.pack('%dq' % len(fields), *[values.get(f, 0) for f in fields])
+    args = packed_args('ppn_scan_args', batch=b, time=t, channels=d, groups=g, states=n)
     assert lib.ppn_scan_checkpoint_bytes(args) == 4 * b * -(-t // ops._CHECKPOINT_ROWS) * n * d
 
 
