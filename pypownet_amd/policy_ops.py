@@ -27,6 +27,7 @@ from . import _lib
 from .engine import EngineError
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOAT = torch.float32
 _packers = {name: struct.Struct('%dq' % len(fields)) for name, fields in _lib.POLICY_STRUCTS.items()}
 _CONV, _CONV_STEP, _SCAN, _SCAN_STEP, _LOSS = (_packers[n] for n in ('ppn_conv_args', 'ppn_conv_step_args', 'ppn_scan_args', 'ppn_scan_step_args',
                                                                       'ppn_loss_args'))
@@ -165,6 +166,8 @@ def _step_state(state, of):
 
 
 def _step_flags(starts, rows, device):
+    if isinstance(starts, torch.Tensor) and starts.dtype in (torch.bool, torch.uint8) and starts.shape == (rows,) and starts.device == device and starts.is_contiguous():
+        return starts
     return None if starts is None else _flags('starts', starts, (rows,), device).contiguous()
 
 
@@ -173,6 +176,8 @@ def _step_ids(env_ids, rows, environments, device):
         if rows > environments:
             raise ValueError('there are %d rows and %d environments: env_ids must say whose rows they are' % (rows, environments))
         return None
+    if isinstance(env_ids, torch.Tensor) and env_ids.dtype is torch.int32 and env_ids.shape == (rows,) and env_ids.device == device and env_ids.is_contiguous():
+        return env_ids
     if not torch.is_tensor(env_ids):
         raise TypeError('env_ids must be a torch tensor, got %s' % type(env_ids).__name__)
     if env_ids.dtype not in (torch.int32, torch.int64):
@@ -271,23 +276,35 @@ def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, 
     place, parameters as for ``short_conv``.  ``env_ids [rows]`` says whose rows they are (``BatchedRunEnv.recv``'s ids; row i is environment i when
     None); a negative id is padding: y = 0 and no state is touched.  An id out of range, or one that an earlier row has, gives NaN and touches no
     state.  ``starts [rows]`` empties the window first.  Returns y [rows, channels]."""
-    kind = _leading('x', x)
-    n, d = _step_rows(x)
-    device = x.device
-    silu = _activation(activation)
-    taps = _conv_parameters(d, weight, bias, device)
-    environments = _step_state(state, 'taps - 1, channels')
-    _like('state', state, (environments, taps - 1, d), x.dtype, device)
+    try:      # as a loop calls it; the rest is looked at one by one
+        n, d = x.shape
+        environments, before, across = state.shape
+        dtype, device = x.dtype, x.device
+        usual = (x.is_cuda and dtype in _TYPES and d > 0 and 1 <= before <= 7 and across == d and state.dtype is dtype and state.device == device
+                 and weight.dtype is _FLOAT and weight.shape == (d, before + 1) and weight.device == device and x.is_contiguous() and state.is_contiguous()
+                 and weight.is_contiguous()
+                 and (bias is None or bias.dtype is _FLOAT and bias.shape == (d,) and bias.device == device and bias.is_contiguous()))
+    except (AttributeError, ValueError):
+        usual = False
+    if usual:
+        y, row = torch.empty_like(x), d
+    else:
+        _leading('x', x)
+        (n, d), device = _step_rows(x), x.device
+        before = _conv_parameters(d, weight, bias, device) - 1
+        environments = _step_state(state, 'taps - 1, channels')
+        _like('state', state, (environments, before, d), x.dtype, device)
+        x, weight, bias = _rows(x), weight.contiguous(), None if bias is None else bias.contiguous()
+        y, row = x.new_empty((n, d)), x.stride(0)
     if _wants_grad(x, state, weight, bias):
         raise ValueError('short_conv_step has no gradient: call it under torch.no_grad(), or short_conv on the window')
-    starts = _step_flags(starts, n, device)
-    env_ids = _step_ids(env_ids, n, environments, device)
-    x, weight = _rows(x), weight.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    y = x.new_empty((n, d))
-    _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, kind, silu, n, environments, d, taps, x.data_ptr(), x.stride(0), weight.data_ptr(),
-                                                 _ptr(bias), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
+    if starts is not None:
+        starts = _step_flags(starts, n, device)
+    if env_ids is not None or n > environments:
+        env_ids = _step_ids(env_ids, n, environments, device)
+    _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, _TYPES[x.dtype], _activation(activation), n, environments, d, before + 1, x.data_ptr(), row,
+                                                 weight.data_ptr(), 0 if bias is None else bias.data_ptr(), state.data_ptr(),
+                                                 0 if env_ids is None else env_ids.data_ptr(), 0 if starts is None else starts.data_ptr(), y.data_ptr(), d), device)
     return y
 
 
@@ -414,27 +431,49 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False, env_ids=None, starts=None):
     """One row of each of ``x``'s environments: ``x, dt, z [rows, channels]``, ``B, C [rows, groups, states]``, ``state [environments, channels, states]``
     (float32, contiguous) moved on in place; ``env_ids`` and ``starts`` as in ``short_conv_step``.  Returns y [rows, channels]."""
-    kind = _leading('x', x)
-    n, d = _step_rows(x)
-    dtype, device = x.dtype, x.device
-    _like('dt', dt, (n, d), dtype, device)
-    if z is not None:
-        _like('z', z, (n, d), dtype, device)
-    states, groups = _scan_parameters(d, A, D, dt_bias, device), _groups_of(d, B, 3)
-    _like('B', B, (n, groups, states), dtype, device)
-    _like('C', C, (n, groups, states), dtype, device)
-    environments = _step_state(state, 'channels, states')
-    _like('state', state, (environments, d, states), torch.float32, device)
+    try:      # as in short_conv_step
+        n, d = rows = x.shape
+        groups, states = B.shape[1:]
+        environments = state.shape[0]
+        dtype, device, cell = x.dtype, x.device, (d, states)
+        usual = (x.is_cuda and dtype in _TYPES and d > 0 and groups > 0 and d % groups == 0 and 1 <= states <= 64 and x.is_contiguous()
+                 and dt.dtype is dtype and dt.shape == rows and dt.device == device and dt.is_contiguous()
+                 and A.dtype is _FLOAT and A.shape == cell and A.device == device and A.is_contiguous()
+                 and B.dtype is dtype and B.shape[0] == n and B.device == device and B.stride()[2] == 1
+                 and C.dtype is dtype and C.shape == B.shape and C.device == device and C.stride()[2] == 1
+                 and state.dtype is _FLOAT and state.shape == (environments, d, states) and state.device == device and state.is_contiguous()
+                 and (z is None or z.dtype is dtype and z.shape == rows and z.device == device and z.is_contiguous())
+                 and (D is None or D.dtype is _FLOAT and D.shape == (d,) and D.device == device and D.is_contiguous())
+                 and (dt_bias is None or dt_bias.dtype is _FLOAT and dt_bias.shape == (d,) and dt_bias.device == device and dt_bias.is_contiguous()))
+    except (AttributeError, ValueError, TypeError):
+        usual = False
+    if usual:
+        y, strides, gate = torch.empty_like(x), (d, d), d
+    else:
+        _leading('x', x)
+        (n, d), dtype, device = _step_rows(x), x.dtype, x.device
+        _like('dt', dt, (n, d), dtype, device)
+        if z is not None:
+            _like('z', z, (n, d), dtype, device)
+        states, groups = _scan_parameters(d, A, D, dt_bias, device), _groups_of(d, B, 3)
+        _like('B', B, (n, groups, states), dtype, device)
+        _like('C', C, (n, groups, states), dtype, device)
+        environments = _step_state(state, 'channels, states')
+        _like('state', state, (environments, d, states), torch.float32, device)
+        x, dt, A, B, C, D, z, dt_bias, _ = _scan_layout(x, dt, A, B, C, D, z, dt_bias, None)
+        y, strides, gate = x.new_empty((n, d)), (x.stride(0), dt.stride(0)), 0 if z is None else z.stride(0)
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
         raise ValueError('selective_scan_step has no gradient: call it under torch.no_grad(), or selective_scan on the window')
-    starts = _step_flags(starts, n, device)
-    env_ids = _step_ids(env_ids, n, environments, device)
-    x, dt, A, B, C, D, z, dt_bias, _ = _scan_layout(x, dt, A, B, C, D, z, dt_bias, None)
-    y = x.new_empty((n, d))
+    if starts is not None:
+        starts = _step_flags(starts, n, device)
+    if env_ids is not None or n > environments:
+        env_ids = _step_ids(env_ids, n, environments, device)
+    b_row, b_group, _ = B.stride()
+    c_row, c_group, _ = C.stride()
     _call(_load().ppn_scan_step,
-          _SCAN_STEP.pack(_SCAN_STEP.size, kind, 1 if dt_softplus else 0, n, environments, d, groups, states, x.data_ptr(), x.stride(0), dt.data_ptr(),
-                          dt.stride(0), A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0), C.stride(1), _ptr(D), _ptr(dt_bias),
-                          _ptr(z), 0 if z is None else z.stride(0), state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
+          _SCAN_STEP.pack(_SCAN_STEP.size, _TYPES[dtype], 1 if dt_softplus else 0, n, environments, d, groups, states, x.data_ptr(), strides[0], dt.data_ptr(),
+                          strides[1], A.data_ptr(), B.data_ptr(), b_row, b_group, C.data_ptr(), c_row, c_group, _ptr(D), _ptr(dt_bias), _ptr(z), gate,
+                          state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
     return y
 
 
