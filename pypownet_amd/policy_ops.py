@@ -109,24 +109,24 @@ def _like(name, t, shape, dtype, device):
 
 def _rows(t):
     """Neighbouring channels next to each other in memory, as the kernels read them; a copy where they are not."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.stride()[-1] == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _flags(name, t, shape, device):
-    if t is None:
-        return None
+    if t is None or isinstance(t, torch.Tensor) and t.dtype in (torch.bool, torch.uint8) and t.shape == shape and t.device == device:
+        return t
     if not torch.is_tensor(t):
         raise TypeError('%s must be a torch tensor, got %s' % (name, type(t).__name__))
     if t.dtype not in (torch.bool, torch.uint8):
         raise TypeError('%s must be bool or uint8, got %s' % (name, t.dtype))
-    if t.device != device or tuple(t.shape) != shape:
-        raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
-    return t
+    raise ValueError('%s must be %s on %s, got %s on %s' % (name, list(shape), device, list(t.shape), t.device))
 
 
 def _window_like(x):
     """An output with x's order in memory: time outermost where x has it outermost."""
     b, t, d = x.shape
+    if x.is_contiguous():
+        return torch.empty_like(x)
     if b > 1 and t > 1 and x.stride(0) < x.stride(1):
         return x.new_empty((t, b, d)).transpose(0, 1)
     return x.new_empty((b, t, d))
@@ -134,7 +134,10 @@ def _window_like(x):
 
 def _at(t):
     """Address, batch stride, time stride."""
-    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    if t is None:
+        return 0, 0, 0
+    strides = t.stride()
+    return t.data_ptr(), strides[0], strides[1]
 
 
 def _wants_grad(*tensors):
@@ -166,8 +169,6 @@ def _step_state(state, of):
 
 
 def _step_flags(starts, rows, device):
-    if isinstance(starts, torch.Tensor) and starts.dtype in (torch.bool, torch.uint8) and starts.shape == (rows,) and starts.device == device and starts.is_contiguous():
-        return starts
     return None if starts is None else _flags('starts', starts, (rows,), device).contiguous()
 
 
@@ -200,7 +201,7 @@ def _conv_args(x, weight, bias, initial, starts, silu, y=None, final=None, dy=No
 
 def _conv_forward(x, weight, bias, initial, starts, silu, want_final):
     y = _window_like(x)
-    final = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if want_final else None
+    final = x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2])) if want_final else None
     _call(_load().ppn_conv_forward, _conv_args(x, weight, bias, initial, starts, silu, y, final), x.device)
     return y, final
 
@@ -258,11 +259,13 @@ def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state
     x, weight, bias and initial_state; the parameters' gradients are summed in a fixed order."""
     _leading('x', x)
     b, t, d = _window_rows(x)
+    device = x.device
     silu = _activation(activation)
-    _conv_parameters(d, weight, bias, x.device)
+    taps = _conv_parameters(d, weight, bias, device)
     if initial_state is not None:
-        _like('initial_state', initial_state, (b, weight.shape[1] - 1, d), x.dtype, x.device)
-    starts = _flags('starts', starts, (b, t), x.device)
+        _like('initial_state', initial_state, (b, taps - 1, d), x.dtype, device)
+    if starts is not None:
+        starts = _flags('starts', starts, (b, t), device)
     if _wants_grad(x, weight, bias, initial_state):
         y, final = _ShortConv.apply(x, weight, bias, initial_state, starts, silu, bool(return_final_state))
     else:
@@ -314,7 +317,7 @@ def _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, soft, y=None, fin
                dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dinitial=None):
     b, t, d = x.shape
     return _SCAN.pack(_SCAN.size, _TYPES[x.dtype], soft, b, t, d, B.shape[2], A.shape[1], *_at(x), *_at(dt), A.data_ptr(),
-                      B.data_ptr(), B.stride(0), B.stride(1), B.stride(2), C.data_ptr(), C.stride(0), C.stride(1), C.stride(2), _ptr(D), _ptr(dt_bias),
+                      B.data_ptr(), *B.stride()[:3], C.data_ptr(), *C.stride()[:3], _ptr(D), _ptr(dt_bias),
                       *_at(z), *_at(starts), _ptr(initial), *_at(y), _ptr(final), _ptr(marks), *_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz),
                       _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dinitial), 0, 0)
 
@@ -355,10 +358,10 @@ class _SelectiveScan(torch.autograd.Function):
         x, dt, A, B, C, D, z, dt_bias, initial, starts, marks = ctx.saved_tensors
         if dy is None and dfinal is None:
             return (None,) * 12
-        empty = lambda v: None if v is None else torch.empty_like(v)      # noqa: E731
         dfinal = None if dfinal is None else dfinal.contiguous()
         dx, ddt, dz = _window_like(x), _window_like(dt), None if z is None else _window_like(z)
-        dA, dD, dbias, dinitial = empty(A), empty(D), empty(dt_bias), empty(initial)
+        dA, dD = torch.empty_like(A), None if D is None else torch.empty_like(D)
+        dbias, dinitial = None if dt_bias is None else torch.empty_like(dt_bias), None if initial is None else torch.empty_like(initial)
         dB, dC = B.new_empty(B.shape), C.new_empty(C.shape)
         if x.shape[0] == 0 or x.shape[1] == 0:          # no rows: the state passes through
             for v in (dA, dD, dbias):
@@ -408,17 +411,18 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     ``(y, final_state)``, the next window's ``initial_state`` and ``selective_scan_step``'s state.  Differentiable in every tensor but ``starts``; sums
     run in a fixed order, so gradients repeat bit for bit.  A differentiable call keeps the states in front of every 8th row for the backward pass."""
     _leading('x', x)
-    b, t, d = _window_rows(x)
-    _like('dt', dt, (b, t, d), x.dtype, x.device)
+    b, t, d = shape = _window_rows(x)
+    dtype, device = x.dtype, x.device
+    _like('dt', dt, shape, dtype, device)
     if z is not None:
-        _like('z', z, (b, t, d), x.dtype, x.device)
-    _scan_parameters(d, A, D, dt_bias, x.device)
-    groups = _groups_of(d, B, 4)
-    for name, v in (('B', B), ('C', C)):
-        _like(name, v, (b, t, groups, A.shape[1]), x.dtype, x.device)
+        _like('z', z, shape, dtype, device)
+    states, groups = _scan_parameters(d, A, D, dt_bias, device), _groups_of(d, B, 4)
+    _like('B', B, (b, t, groups, states), dtype, device)
+    _like('C', C, (b, t, groups, states), dtype, device)
     if initial_state is not None:
-        _like('initial_state', initial_state, (b, d, A.shape[1]), torch.float32, x.device)
-    starts = _flags('starts', starts, (b, t), x.device)
+        _like('initial_state', initial_state, (b, d, states), torch.float32, device)
+    if starts is not None:
+        starts = _flags('starts', starts, (b, t), device)
     soft = 1 if dt_softplus else 0
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
         y, final = _SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, initial_state, starts, soft, bool(return_final_state))
