@@ -254,6 +254,31 @@ template <int NS> __device__ inline void advance(const float (&before)[NS], floa
   }
 }
 
+// What enters a chunk, from what the chunks before it do (`count` of them, from `first` in steps of `step`), in h: as scan_join, in the wave that goes on
+// with it.
+template <int NS, int LPC>
+__device__ inline void join_chunks(const ppn_scan_args& a, const Place& p, int64_t chunks, const float* ends, const float* sums, int first, int count, int step,
+                                   const float (&A2)[NS], float (&h)[NS]) {
+  constexpr int AHEAD = 2;
+  const int64_t plane = a.states * a.channels;
+  for (int i0 = 0; i0 < count; i0 += AHEAD) {
+    float own[AHEAD][NS], total[AHEAD], cut[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t at_chunk = p.b * chunks + first + step * min(i0 + j, count - 1);
+      load_plane<NS, LPC>(ends + at_chunk * plane, a.states, a.channels, p.d, p.part, own[j]);
+      total[j] = at<const float>(sums + (at_chunk * 2 + 0) * a.channels, p.d * 4u);
+      cut[j] = at<const float>(sums + (at_chunk * 2 + 1) * a.channels, p.d * 4u);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (i0 + j < count) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) h[n] = cut[j] != 0.0f ? own[j][n] : own[j][n] + __builtin_amdgcn_exp2f(total[j] * A2[n]) * h[n];
+      }
+  }
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------------
 // One wave: 64 / LPC channels of one environment over the rows of one chunk (grid.y chunks of `chunk` rows, a multiple of ROWS).
 // OUTPUT: y.  TRAIN: the states in front of every block as well.  SUMMARY: neither, only what the chunk does to a state that enters it: its
@@ -272,6 +297,7 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
   if constexpr (MODE != SUMMARY) {
     if (entering) load_plane<NS, LPC>(entering + (p.b * chunks + k) * plane, a.states, a.channels, p.d, p.part, h);
     else if (a.initial) load_states<NS>(a.initial + (p.b * a.channels + p.d) * a.states, a.states, p.part, h);
+    if (ends) join_chunks<NS, LPC>(a, p, chunks, ends, sums, 0, (int)k, 1, A2, h);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
   const bool soft = a.softplus, gated = a.z != nullptr;
@@ -420,6 +446,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
   if constexpr (!ADJOINT) {
     if (entering) load_plane<NS, LPC>(entering + cell * plane, a.states, a.channels, p.d, p.part, e);
     else if (a.dfinal) load_states<NS>(a.dfinal + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
+    if (ends) join_chunks<NS, LPC>(a, p, chunks, ends, sums, (int)chunks - 1, (int)(chunks - 1 - k), -1, A2, e);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
   const unsigned mine = p.d * (unsigned)sizeof(T);
@@ -712,6 +739,9 @@ int64_t states_of(const ppn_scan_args* a) {
 // twice; else as many as bring `wanted` waves, of at least 16 rows.  Forward 3072 (2 x 8724 rows x 768: 138, 139, 143 and 154 us at 2048, 3072,
 // 4096 and 6144; 75 x 167 rows x 200: 54, 50, 48 at the first three), backward 4096 (the latter: 107, 103, 96 us at 1024, 2048, 4096).
 struct Split { int64_t chunk, chunks; };
+// Up to this many chunks, each wave joins the ones before its own by itself, else a launch in between does (75 x 167 rows x 200, 11 chunks: a training step
+// takes 194 us against 202, its kernels 156 either way).
+constexpr int64_t FEW_CHUNKS = 16;
 Split split_time(const ppn_scan_args* a, int64_t waves, int64_t wanted) {
   int64_t chunks = waves * 2 > wanted ? 1 : ceil_div(wanted, waves < 1 ? 1 : waves);
   int64_t chunk = ceil_div(ceil_div(a->time, chunks), ROWS) * ROWS;
@@ -781,11 +811,12 @@ extern "C" int ppn_scan_forward(const ppn_scan_args* a, void* stream) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
       if (s.chunks > 1) {
         scan_forward<T, NS, LPC, SUMMARY><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, nullptr, ends, sums);
-        scan_join<false><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunks, ends, sums);
+        if (s.chunks > FEW_CHUNKS) scan_join<false><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunks, ends, sums);
       }
-      const float* entering = s.chunks > 1 ? ends : nullptr;
-      if (a->checkpoints) scan_forward<T, NS, LPC, TRAIN><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, entering, nullptr, nullptr);
-      else scan_forward<T, NS, LPC, OUTPUT><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, entering, nullptr, nullptr);
+      const float* joined = s.chunks > FEW_CHUNKS ? ends : nullptr;
+      float* apart = s.chunks > 1 && s.chunks <= FEW_CHUNKS ? ends : nullptr;
+      if (a->checkpoints) scan_forward<T, NS, LPC, TRAIN><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, joined, apart, sums);
+      else scan_forward<T, NS, LPC, OUTPUT><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, s.chunk, s.chunks, joined, apart, sums);
       return launched("ppn_scan_forward");
     });
   });
@@ -817,12 +848,13 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
     typedef std::remove_pointer_t<decltype(t)> T;
     return by_states(a->states, [&](auto ns, auto lpc) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
-      const bool split = p.split.chunks > 1;
-      if (split) {
+      const float* joined = p.split.chunks > FEW_CHUNKS ? ends : nullptr;
+      float* apart = p.split.chunks > 1 && p.split.chunks <= FEW_CHUNKS ? ends : nullptr;
+      if (p.split.chunks > 1) {
         scan_backward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, nullptr, nullptr);
-        scan_join<true><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
+        if (joined) scan_join<true><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
       }
-      scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, split ? ends : nullptr, nullptr, nullptr, rows, params);
+      scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, joined, apart, sums, rows, params);
       const int64_t row_blocks = ceil_div(count, 1024);
       const ReduceArgs r = {rows, tiles_of(a), a->batch * a->time * a->groups, params, a->batch * p.split.chunks, a->states, a->channels, a->dB, a->dC, a->dA, a->dD,
                             a->ddt_bias, row_blocks};

@@ -385,6 +385,7 @@ SCAN = [  # batch, time, channels, groups, states, D, z, dt_bias, softplus, star
     (2, 19, 40, 2, 32, False, True, False, True, True, True, True), (1, 24, 24, 1, 64, True, True, True, True, False, True, False),
     (1, 130, 130, 1, 8, True, True, True, True, True, True, False), (2, 65, 20, 1, 23, True, True, True, False, True, True, False),
     (1, 400, 32, 1, 16, True, True, True, True, True, True, False), (2, 9, 33, 1, 45, True, True, True, True, True, True, True),
+    (1, 300, 20, 2, 40, True, True, True, True, True, True, False),
 ]
 
 
