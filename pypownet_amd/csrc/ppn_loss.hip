@@ -342,6 +342,65 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
   a.lse[row] = lse;
 }
 
+// float16: scale[0], the power of two dl is multiplied by (it brings the largest |dloss| to 2^14), and scale[1] = 1 / scale[0].
+__global__ void __launch_bounds__(1024) loss_scale(const float* dloss, const float* lse, int64_t rows, float* scale) {
+  __shared__ float tops[1024];
+  float top = 0.0f;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    const float g = fabsf(dloss[i]);
+    if (lse[i] != INFINITY && g < INFINITY && g > top) top = g;
+  }
+  tops[threadIdx.x] = top;
+  __syncthreads();
+  for (int half = 512; half; half >>= 1) {
+    if (threadIdx.x < half) tops[threadIdx.x] = fmaxf(tops[threadIdx.x], tops[threadIdx.x + half]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    top = tops[0];
+    int e = 0;
+    if (top > 0.0f) frexpf(top, &e);
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    scale[0] = top > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
+    scale[1] = top > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
+  }
+}
+
+// The transposed copies of hidden and weight, [cols x rows_padded] with zeros in the padding, for the second products: 64 x 64 tiles through LDS, `across`
+// of them along the rows, by workgroups in the launch that makes dl (of 999 x 12099 x 392: 31 us together, 25 and 13 apart).  A row of hidden without a gradient (lse +infinity) becomes zeros:
+// whatever stands in it, its product with dl's zeros is zero.
+struct TransposeJob { const void* in; int64_t in_row, rows, cols; void* out; int64_t rows_padded; const float* lse; unsigned across, blocks; };
+template <typename T> constexpr int TRANSPOSE_BYTES = 64 * (64 + 4 / sizeof(T)) * sizeof(T);
+template <typename T> __device__ inline void transpose(const TransposeJob& job, unsigned id, char* lds) {
+  typedef T Line[64 + 4 / sizeof(T)];
+  Line* tile = (Line*)lds;
+  const int64_t r0 = (int64_t)(id % job.across) * 64, c0 = (int64_t)(id / job.across) * 64;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const T* in = (const T*)job.in;
+  T part[16];
+  float lse[16];
+  const int64_t column = c0 + x < job.cols ? c0 + x : job.cols - 1;
+  const float* marks = job.lse ? job.lse : (const float*)job.out;      // (read in its place and not looked at)
+  const int64_t mark_step = job.lse ? 1 : 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {      // (loads without a branch, all in flight)
+    const int64_t r = r0 + y + 4 * i, row = r < job.rows ? r : job.rows - 1;
+    part[i] = in[row * job.in_row + column];
+    lse[i] = marks[row * mark_step];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const bool out = r0 + y + 4 * i >= job.rows || c0 + x >= job.cols || (job.lse && lse[i] == INFINITY);
+    tile[y + 4 * i][x] = out ? (T)0.0f : part[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 64; i += 4) {
+    const int64_t c = c0 + y + i, r = r0 + x;
+    if (c < job.cols && r < job.rows_padded) ((T*)job.out)[c * job.rows_padded + r] = tile[x][y + i];
+  }
+}
+
 // Two rows' (of a lane's column) values as one word, and the exchange that turns four rows of one column into two rows of two columns: lanes of
 // even columns keep the first two rows, those of odd ones the last two.
 __device__ inline unsigned pair(__bf16 a, __bf16 b) { return (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16; }
@@ -351,13 +410,22 @@ __device__ inline unsigned from_neighbour(unsigned v) { return (unsigned)__built
 // Backward, first product: dl of the columns first .. first + N of the catalogue, [rows x cols_padded] and [N x rows_padded], zeros in the padding.
 // The target's own entry, (e^-loss - 1) dloss, is written over its tile's value at the end.
 template <typename T, int MI, int NI, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArgs g, unsigned tiles_m, unsigned tiles_n) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArgs g, unsigned tiles_m, unsigned tiles_n, TransposeJob one, TransposeJob two) {
   typedef Product<T, MI, NI, WM, WN> P;
   struct Row { float lse2, up; };
-  constexpr int OUT = sizeof(T) == 2 ? P::BM * P::BN * 2 : 0;
+  static_assert(P::THREADS == 256, "transpose()");
+  constexpr int OUT = sizeof(T) == 2 ? P::BM * P::BN * 2 : TRANSPOSE_BYTES<T>;
   __shared__ __align__(16) char lds[P::LDS_BYTES > OUT ? P::LDS_BYTES : OUT];
+  static_assert(sizeof lds >= TRANSPOSE_BYTES<T>, "transpose()");
   __shared__ __align__(16) unsigned mask[P::BM][P::BN / 32];
   __shared__ __align__(16) Row rows[P::BM];
+  const unsigned tiles = tiles_m * tiles_n;
+  if (blockIdx.x >= tiles) {
+    const unsigned id = blockIdx.x - tiles;
+    if (id < one.blocks) transpose<T>(one, id, lds);
+    else transpose<T>(two, id - one.blocks, lds);
+    return;
+  }
   unsigned tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = (int64_t)tm * P::BM, n0 = (int64_t)tn * P::BN;
@@ -366,7 +434,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_grad(Operands o, GradArg
     const float lse = g.lse[row];
     const bool live = m0 + r < o.M && lse != INFINITY;                   // a row without a gradient, or past the last one: zeros
     stage_mask<P::BN>(mask, r, g.allowed, g.allowed_row, row, g.first / 32, n0, o.N, live);
-    rows[r] = Row{lse * LOG2E, live ? g.dloss[row] * g.scale[0] : 0.0f};
+    rows[r] = Row{lse * LOG2E, live ? g.dloss[row] * (g.scale ? g.scale[0] : 1.0f) : 0.0f};
   }
   P p;
   p.run(o, lds, m0, n0, 0, o.K);
@@ -500,7 +568,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_sums(SumJob one, SumJob 
   const bool whole = m0 + P::BM <= o.M && n0 + P::BN <= o.N;
   if (job.out) {
     T* out = (T*)job.out + m0 * o.N + n0;
-    const float unscale = scale[1];
+    const float unscale = scale ? scale[1] : 1.0f;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -539,7 +607,7 @@ __global__ void __launch_bounds__(256) loss_finish(FinishJob one, FinishJob two,
   if (i >= job.count) return;
   float v = 0.0f;
   for (int64_t s = 0; s < job.slots; ++s) v += job.sums[s * job.count + i];
-  ((T*)job.out)[i] = (T)(v * scale[1]);
+  ((T*)job.out)[i] = (T)(scale ? v * scale[1] : v);
 }
 
 // [rows x cols] with any row stride -> [rows x cols_padded], zeros in the padding.
@@ -549,52 +617,6 @@ __global__ void __launch_bounds__(256) loss_pad(const T* in, int64_t in_row, int
   if (i >= rows * cols_padded) return;
   const int64_t r = i / cols_padded, c = i - r * cols_padded;
   out[i] = c < cols ? in[r * in_row + c] : (T)0.0f;
-}
-
-// In front of the backward products: the transposed copies of hidden and weight, [cols x rows_padded] with zeros in the padding (64 x 64 tiles
-// through LDS, `across` of them along the rows), and dl's scale.  A row of hidden without a gradient (lse +infinity) becomes zeros: whatever
-// stands in it, its product with dl's zeros is zero.
-struct TransposeJob { const void* in; int64_t in_row, rows, cols; void* out; int64_t rows_padded; const float* lse; int64_t across, blocks; };
-struct ScaleJob { const float* dloss; const float* lse; int64_t rows; bool needed; float* scale; };      // scale[0]: a power of two, scale[1] = 1 / it
-template <typename T>
-__global__ void __launch_bounds__(256) loss_prepare(TransposeJob one, TransposeJob two, ScaleJob sc) {
-  __shared__ T tile[64][64 + 4 / sizeof(T)];
-  __shared__ float tops[256];
-  if (blockIdx.x >= one.blocks + two.blocks) {
-    float top = 0.0f;
-    if (sc.needed)
-      for (int64_t i = threadIdx.x; i < sc.rows; i += 256) {
-        const float g = fabsf(sc.dloss[i]);
-        if (sc.lse[i] != INFINITY && g < INFINITY && g > top) top = g;
-      }
-    tops[threadIdx.x] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 256; ++i) top = tops[i] > top ? tops[i] : top;
-      int e = 0;
-      if (top > 0.0f) frexpf(top, &e);
-      e = e < -100 ? -100 : e > 100 ? 100 : e;
-      sc.scale[0] = top > 0.0f ? ldexpf(1.0f, 14 - e) : 1.0f;
-      sc.scale[1] = top > 0.0f ? ldexpf(1.0f, e - 14) : 1.0f;
-    }
-    return;
-  }
-  const bool second = blockIdx.x >= one.blocks;
-  const TransposeJob job = second ? two : one;
-  const int64_t id = (int64_t)blockIdx.x - (second ? one.blocks : 0), r0 = id % job.across * 64, c0 = id / job.across * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const T* in = (const T*)job.in;
-#pragma unroll
-  for (int i = 0; i < 64; i += 4) {
-    const int64_t r = r0 + y + i, c = c0 + x;
-    tile[y + i][x] = r < job.rows && c < job.cols && !(job.lse && job.lse[r] == INFINITY) ? in[r * job.in_row + c] : (T)0.0f;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 64; i += 4) {
-    const int64_t c = c0 + y + i, r = r0 + x;
-    if (c < job.cols && r < job.rows_padded) ((T*)job.out)[c * job.rows_padded + r] = tile[x][y + i];
-  }
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------------------------------
@@ -761,7 +783,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_backward: the workspace is too small");
   char* w = (char*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
-  float* scale = (float*)(w + p.scale);
+  float* scale = a->type == PPN_T_F16 ? (float*)(w + p.scale) : nullptr;
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     const void* hidden = a->hidden;
@@ -776,16 +798,19 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
       weight = w + p.weight, weight_row = p.features_padded;
     }
     const int64_t down = ceil_div(a->features, 64), hidden_across = ceil_div(p.rows_padded, 64), weight_across = ceil_div(p.actions_padded, 64);
-    const TransposeJob th = {a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden_t, p.rows_padded, a->lse, hidden_across, a->dweight ? hidden_across * down : 0};
-    const TransposeJob tw = {a->weight, a->weight_row, a->actions, a->features, w + p.weight_t, p.actions_padded, nullptr, weight_across, a->dhidden ? weight_across * down : 0};
-    if (th.blocks + tw.blocks > 0x7ffffff0) return fail(PPN_E_INVALID, "loss: an operand is too large");
-    loss_prepare<T><<<dim3(th.blocks + tw.blocks + 1), dim3(256), 0, s>>>(th, tw, ScaleJob{a->dloss, a->lse, a->rows, a->type == PPN_T_F16, scale});
+    TransposeJob th = {a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden_t, p.rows_padded, a->lse, (unsigned)hidden_across, a->dweight ? (unsigned)(hidden_across * down) : 0u};
+    TransposeJob tw = {a->weight, a->weight_row, a->actions, a->features, w + p.weight_t, p.actions_padded, nullptr, (unsigned)weight_across, a->dhidden ? (unsigned)(weight_across * down) : 0u};
+    if ((hidden_across + weight_across) * down > 0x3fffffff) return fail(PPN_E_INVALID, "loss: an operand is too large");
+    if (scale) loss_scale<<<dim3(1), dim3(1024), 0, s>>>(a->dloss, a->lse, a->rows, scale);
     for (int64_t first = 0; first < a->actions; first += p.piece) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 64);
       const Operands o = {hidden, hidden_row, a->rows, (const T*)weight + first * weight_row, weight_row, n, p.features_padded};
       const GradArgs g = {a->allowed, a->allowed_row, a->target, a->lse, a->loss, a->dloss, scale, w + p.dl, p.piece, w + p.dlt, p.rows_padded, first, p.rows_padded, np};
       const int64_t tm = ceil_div(a->rows, p.grad.m), tn = ceil_div(n, p.grad.n);
-      by_large_tile(p.grad, [&](auto t) { loss_grad<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(tm * tn), dim3(256), 0, s>>>(o, g, tm, tn); });
+      by_large_tile(p.grad, [&](auto t) {
+        loss_grad<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(tm * tn + th.blocks + tw.blocks), dim3(256), 0, s>>>(o, g, tm, tn, th, tw);
+      });
+      th.blocks = tw.blocks = 0;
       const int64_t across = ceil_div(a->features, p.sums.n);
       // (the last piece is shorter: a share that begins past its end adds nothing, and every slot has been written by the first piece)
       auto job = [&](const Operands& q, int64_t at, void* out, bool wanted, bool add) {
