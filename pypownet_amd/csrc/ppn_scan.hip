@@ -412,10 +412,13 @@ __global__ void __launch_bounds__(64) scan_join(ppn_scan_args a, int64_t chunks,
 // partial sums per tile of channels, added up by scan_reduce; dA, dD and ddt_bias stay in registers over the wave's rows and leave one
 // row of partial sums for each environment and chunk.  Both reductions run in a fixed order.
 //
-// ADJOINT: only what a chunk adds to the adjoint in front of it, and its sum of delta, for chunks that are worked on at once.
-template <typename T, int NS, int LPC, bool ADJOINT>
+// ENDS: only what a chunk adds to the adjoint in front of it, and its sum of delta, for chunks that are worked on at once.  JOINING: gradients, behind
+// join_chunks (a kernel of its own: its registers cost the others 26 us of 690 in a training step).
+enum { GRADIENTS, JOINING, ENDS };
+template <typename T, int NS, int LPC, int MODE>
 __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t chunk, int64_t chunks, const float* entering, float* ends, float* sums, float* rows_out,
                                                                     float* params_out) {
+  constexpr bool ADJOINT = MODE == ENDS;
   constexpr int STATES = Shape<NS, LPC>::STATES, KEPT = NS == 8 ? ROWS : ROWS / 2;
   __shared__ __align__(16) float sb[ADJOINT ? 4 : ROWS * STATES], sc[ROWS * STATES];
   const Place p = place<NS, LPC>(a);
@@ -446,7 +449,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
   if constexpr (!ADJOINT) {
     if (entering) load_plane<NS, LPC>(entering + cell * plane, a.states, a.channels, p.d, p.part, e);
     else if (a.dfinal) load_states<NS>(a.dfinal + (p.b * a.channels + p.d) * a.states, a.states, p.part, e);
-    if (ends) join_chunks<NS, LPC>(a, p, chunks, ends, sums, (int)chunks - 1, (int)(chunks - 1 - k), -1, A2, e);
+    if constexpr (MODE == JOINING) join_chunks<NS, LPC>(a, p, chunks, ends, sums, (int)chunks - 1, (int)(chunks - 1 - k), -1, A2, e);
   }
   const float bias = a.dt_bias ? a.dt_bias[p.d] : 0.0f, skip = a.D ? a.D[p.d] : 0.0f;
   const unsigned mine = p.d * (unsigned)sizeof(T);
@@ -849,12 +852,14 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
     return by_states(a->states, [&](auto ns, auto lpc) {
       constexpr int NS = decltype(ns)::value, LPC = decltype(lpc)::value;
       const float* joined = p.split.chunks > FEW_CHUNKS ? ends : nullptr;
-      float* apart = p.split.chunks > 1 && p.split.chunks <= FEW_CHUNKS ? ends : nullptr;
       if (p.split.chunks > 1) {
-        scan_backward<T, NS, LPC, true><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, nullptr, nullptr);
+        scan_backward<T, NS, LPC, ENDS><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, nullptr, nullptr);
         if (joined) scan_join<true><<<dim3(ceil_div(cells, 64)), dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunks, ends, sums);
       }
-      scan_backward<T, NS, LPC, false><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, joined, apart, sums, rows, params);
+      if (p.split.chunks > 1 && !joined)
+        scan_backward<T, NS, LPC, JOINING><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, rows, params);
+      else
+        scan_backward<T, NS, LPC, GRADIENTS><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, joined, nullptr, nullptr, rows, params);
       const int64_t row_blocks = ceil_div(count, 1024);
       const ReduceArgs r = {rows, tiles_of(a), a->batch * a->time * a->groups, params, a->batch * p.split.chunks, a->states, a->channels, a->dB, a->dC, a->dA, a->dD,
                             a->ddt_bias, row_blocks};
