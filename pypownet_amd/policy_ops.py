@@ -31,6 +31,10 @@ _FLOAT = torch.float32
 _packers = {name: struct.Struct('%dq' % len(fields)) for name, fields in _lib.POLICY_STRUCTS.items()}
 _CONV, _CONV_STEP, _SCAN, _SCAN_STEP, _LOSS = (_packers[n] for n in ('ppn_conv_args', 'ppn_conv_step_args', 'ppn_scan_args', 'ppn_scan_step_args',
                                                                       'ppn_loss_args'))
+# The blocks of the window forms in two parts: what the forward pass takes, and what only the backward pass does (from dy on; zeros forward).
+_CONV_FRONT, _SCAN_FRONT = (struct.Struct('%dq' % _lib.POLICY_STRUCTS[n].index('dy')) for n in ('ppn_conv_args', 'ppn_scan_args'))
+_CONV_BACK, _SCAN_BACK = struct.Struct('%dq' % ((_CONV.size - _CONV_FRONT.size) // 8)), struct.Struct('%dq' % ((_SCAN.size - _SCAN_FRONT.size) // 8))
+_CONV_NO_BACK, _SCAN_NO_BACK = bytes(_CONV_BACK.size), bytes(_SCAN_BACK.size)
 _library = None
 
 
@@ -193,16 +197,16 @@ def _step_ids(env_ids, rows, environments, device):
 
 # ---- short causal convolution --------------------------------------------------------------------------------------------------------
 
-def _conv_args(x, weight, bias, initial, starts, silu, y=None, final=None, dy=None, dfinal=None, dx=None, dweight=None, dbias=None, dinitial=None):
+def _conv_front(x, weight, bias, initial, starts, silu, y, final):
     b, t, d = x.shape
-    return _CONV.pack(_CONV.size, _TYPES[x.dtype], silu, b, t, d, weight.shape[1], *_at(x), weight.data_ptr(), _ptr(bias), _ptr(initial), *_at(starts),
-                      *_at(y), _ptr(final), *_at(dy), _ptr(dfinal), *_at(dx), _ptr(dweight), _ptr(dbias), _ptr(dinitial), 0, 0)
+    return _CONV_FRONT.pack(_CONV.size, _TYPES[x.dtype], silu, b, t, d, weight.shape[1], *_at(x), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                            0 if initial is None else initial.data_ptr(), *_at(starts), *_at(y), 0 if final is None else final.data_ptr())
 
 
 def _conv_forward(x, weight, bias, initial, starts, silu, want_final):
     y = _window_like(x)
     final = x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2])) if want_final else None
-    _call(_load().ppn_conv_forward, _conv_args(x, weight, bias, initial, starts, silu, y, final), x.device)
+    _call(_load().ppn_conv_forward, _conv_front(x, weight, bias, initial, starts, silu, y, final) + _CONV_NO_BACK, x.device)
     return y, final
 
 
@@ -229,7 +233,8 @@ class _ShortConv(torch.autograd.Function):
         dinitial = None if initial is None else torch.empty_like(initial)
         lib = _load()
         _with_workspace(lib.ppn_conv_backward_workspace, lib.ppn_conv_backward,
-                        _conv_args(x, weight, bias, initial, starts, ctx.silu, None, None, dy, dfinal, dx, dweight, dbias, dinitial), x.device)
+                        _conv_front(x, weight, bias, initial, starts, ctx.silu, None, None) +
+                        _CONV_BACK.pack(*_at(dy), _ptr(dfinal), *_at(dx), dweight.data_ptr(), _ptr(dbias), _ptr(dinitial), 0, 0), x.device)
         return dx, dweight, dbias, dinitial, None, None, None
 
 
@@ -257,13 +262,23 @@ def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state
     uint8) marks first rows of episodes, in front of which every tap is zero.  Returns y, or ``(y, final_state)``: the last ``taps - 1`` rows of the
     episode that is running at the window's end, i.e. the next window's ``initial_state`` and ``short_conv_step``'s state.  Differentiable in
     x, weight, bias and initial_state; the parameters' gradients are summed in a fixed order."""
-    _leading('x', x)
-    b, t, d = _window_rows(x)
-    device = x.device
+    try:      # as it is mostly called; the rest is looked at one by one
+        b, t, d = x.shape
+        taps = weight.shape[1]
+        dtype, device = x.dtype, x.device
+        usual = (x.is_cuda and dtype in _TYPES and d > 0 and 2 <= taps <= 8 and weight.dtype is _FLOAT and weight.shape == (d, taps) and weight.device == device
+                 and (bias is None or bias.dtype is _FLOAT and bias.shape == (d,) and bias.device == device)
+                 and (initial_state is None or initial_state.dtype is dtype and initial_state.shape == (b, taps - 1, d) and initial_state.device == device))
+    except (AttributeError, ValueError, IndexError):
+        usual = False
+    if not usual:
+        _leading('x', x)
+        b, t, d = _window_rows(x)
+        device = x.device
+        taps = _conv_parameters(d, weight, bias, device)
+        if initial_state is not None:
+            _like('initial_state', initial_state, (b, taps - 1, d), x.dtype, device)
     silu = _activation(activation)
-    taps = _conv_parameters(d, weight, bias, device)
-    if initial_state is not None:
-        _like('initial_state', initial_state, (b, taps - 1, d), x.dtype, device)
     if starts is not None:
         starts = _flags('starts', starts, (b, t), device)
     if _wants_grad(x, weight, bias, initial_state):
@@ -313,13 +328,13 @@ def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, 
 
 # ---- selective scan ------------------------------------------------------------------------------------------------------------------
 
-def _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, soft, y=None, final=None, marks=None, dy=None, dfinal=None, dx=None, ddt=None, dz=None,
-               dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dinitial=None):
+def _scan_front(x, dt, A, B, C, D, z, dt_bias, starts, initial, soft, y, final, marks):
     b, t, d = x.shape
-    return _SCAN.pack(_SCAN.size, _TYPES[x.dtype], soft, b, t, d, B.shape[2], A.shape[1], *_at(x), *_at(dt), A.data_ptr(),
-                      B.data_ptr(), *B.stride()[:3], C.data_ptr(), *C.stride()[:3], _ptr(D), _ptr(dt_bias),
-                      *_at(z), *_at(starts), _ptr(initial), *_at(y), _ptr(final), _ptr(marks), *_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz),
-                      _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dinitial), 0, 0)
+    b_batch, b_time, b_group, _ = B.stride()
+    c_batch, c_time, c_group, _ = C.stride()
+    return _SCAN_FRONT.pack(_SCAN.size, _TYPES[x.dtype], soft, b, t, d, B.shape[2], A.shape[1], *_at(x), *_at(dt), A.data_ptr(), B.data_ptr(), b_batch,
+                            b_time, b_group, C.data_ptr(), c_batch, c_time, c_group, _ptr(D), _ptr(dt_bias), *_at(z), *_at(starts), _ptr(initial), *_at(y),
+                            _ptr(final), _ptr(marks))
 
 
 _CHECKPOINT_ROWS = 8
@@ -329,11 +344,11 @@ def _scan_forward(inputs, want_final, train):
     x, A = inputs[0], inputs[2]
     lib = _load()
     y = _window_like(x)
-    final = torch.empty((x.shape[0],) + tuple(A.shape), dtype=torch.float32, device=x.device) if want_final else None
+    final = A.new_empty((x.shape[0], *A.shape)) if want_final else None
     marks = None
     if train:      # (ppn_scan_checkpoint_bytes)
-        marks = torch.empty((x.shape[0], -(-x.shape[1] // _CHECKPOINT_ROWS), A.shape[1], A.shape[0]), dtype=torch.float32, device=x.device)
-    _with_workspace(lib.ppn_scan_forward_workspace, lib.ppn_scan_forward, _scan_args(*inputs, y, final, marks), x.device)
+        marks = A.new_empty((x.shape[0], -(-x.shape[1] // _CHECKPOINT_ROWS), A.shape[1], A.shape[0]))
+    _with_workspace(lib.ppn_scan_forward_workspace, lib.ppn_scan_forward, _scan_front(*inputs, y, final, marks) + _SCAN_NO_BACK, x.device)
     return y, final, marks
 
 
@@ -373,8 +388,9 @@ class _SelectiveScan(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         lib = _load()
         _with_workspace(lib.ppn_scan_backward_workspace, lib.ppn_scan_backward,
-                        _scan_args(x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft, None, None, marks, dy, dfinal, dx, ddt, dz, dB, dC, dA, dD, dbias,
-                                   dinitial), x.device)
+                        _scan_front(x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft, None, None, marks) +
+                        _SCAN_BACK.pack(*_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias),
+                                        _ptr(dinitial), 0, 0), x.device)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
 
 
@@ -529,8 +545,9 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
     ``hidden [rows, features]`` and ``weight [actions, features]`` of one type, ``target [rows]`` int64.  ``allowed [rows, ceil(actions / 32)]``
     int32 has one bit per action (``pack_allowed``), all actions when None.  A row whose target is ``ignore_index``, or that allows nothing, has loss 0
     and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
-    NaN.  ``-loss`` is the log-probability of the action ``target``.  Differentiable in hidden and weight (the result is kept for that: not to be changed in
-    place); sums run in a fixed order."""
+    NaN.  What a row does not allow is not looked at (behind the loss, a weight row that is not finite still makes NaN of dhidden).  ``-loss`` is the
+    log-probability of the action ``target``.  Differentiable in hidden and weight (the result is kept for that: not to be changed in place); sums
+    run in a fixed order."""
     _leading('hidden', hidden)
     if hidden.dim() != 2 or hidden.shape[1] == 0:
         raise ValueError('hidden must be [rows, features], got %s' % list(hidden.shape))
