@@ -739,8 +739,9 @@ int64_t states_of(const ppn_scan_args* a) {
 }
 
 // Chunks of time that are worked on at once: one while the waves of (environment, tile) alone fill the chip, since splitting walks the rows
-// twice; else as many as bring `wanted` waves, of at least 16 rows.  Forward 3072 (2 x 8724 rows x 768: 138, 139, 143 and 154 us at 2048, 3072,
-// 4096 and 6144; 75 x 167 rows x 200: 54, 50, 48 at the first three), backward 4096 (the latter: 107, 103, 96 us at 1024, 2048, 4096).
+// twice; else as many as bring `wanted` waves, of at least 16 rows.  Forward 3200 (2 x 8724 rows
+// x 768: 137, 153, 138 and 142 us at 2000, 2600, 3200 and 4000; 75 x 167 rows x 200: 54, 54, 53, 53), backward 4096 (the latter: 107, 103, 96 us at
+// 1024, 2048, 4096).
 struct Split { int64_t chunk, chunks; };
 // Up to this many chunks, each wave joins the ones before its own by itself, else a launch in between does (75 x 167 rows x 200, 11 chunks: a training step
 // takes 194 us against 202, its kernels 156 either way).
@@ -753,7 +754,7 @@ Split split_time(const ppn_scan_args* a, int64_t waves, int64_t wanted) {
   chunks = a->time ? ceil_div(a->time, chunk) : 1;
   return {chunk, chunks < 1 ? 1 : chunks};
 }
-Split forward_split(const ppn_scan_args* a) { return split_time(a, a->batch * a->groups * tiles_of(a), 3072); }
+Split forward_split(const ppn_scan_args* a) { return split_time(a, a->batch * a->groups * tiles_of(a), 3200); }
 
 struct BackwardPlan { Split split; int64_t rows_bytes, params_bytes, ends_bytes, sums_bytes; };
 BackwardPlan plan_backward(const ppn_scan_args* a) {
