@@ -868,3 +868,20 @@ def test_gpu_step_in_a_graph():
         want = step(eager_c, eager_s)
         torch.cuda.synchronize()
         assert torch.equal(y, want) and torch.equal(conv, eager_c) and torch.equal(state, eager_s)
+
+
+@pytest.mark.gpu
+def test_gpu_gradients_of_gradients_are_refused():
+    """A graph of the backward pass may be asked for (the gradients are the same); differentiating through it is an error, not a wrong number."""
+    from pypownet_amd import policy_ops as ops
+    leaves, starts, target, bits = _block_inputs()
+    want = torch.autograd.grad(_block(leaves, starts, target, bits).sum(), leaves)
+    got = torch.autograd.grad(_block(leaves, starts, target, bits).sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(got[0].sum(), leaves[0])
+    gen = torch.Generator().manual_seed(41)
+    h, w = rand(gen, 5, 8).cuda().requires_grad_(True), rand(gen, 9, 8).cuda().requires_grad_(True)
+    dh, = torch.autograd.grad(ops.action_cross_entropy(h, w, torch.arange(5, device='cuda')).sum(), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dh.sum(), h)
