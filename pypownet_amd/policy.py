@@ -225,8 +225,9 @@ def imitate(env, policy, optimizer, memory, steps, candidates=8, layout='full'):
     for _ in range(steps):
         obs, first, allowed = env.policy_rows(policy, layout=layout)
         choice = policy.act(obs, acting, starts=first, allowed=allowed)
-        others = torch.multinomial(allowed.float(), candidates - 2, replacement=True) if candidates > 2 else choice[:, :0]
-        tried = torch.cat([torch.zeros_like(choice)[:, None], choice[:, None], others], dim=1)
+        tried = torch.stack([torch.zeros_like(choice), choice], dim=1)
+        if candidates > 2:
+            tried = torch.cat([tried, torch.multinomial(allowed.float(), candidates - 2, replacement=True)], dim=1)
         rewards, done, _, _ = env.search(policy.vectors[tried])
         rewards = torch.where(done, torch.full_like(rewards, -math.inf), rewards)      # (an action that ends the episode is the last to take)
         best = rewards.argmax(dim=1)

@@ -226,7 +226,8 @@ def test_gpu_policy_acts_on_environments(sample):
 
 
 @pytest.mark.gpu
-def test_gpu_policy_learns_from_the_search():
+@pytest.mark.parametrize('candidates', [2, 5])
+def test_gpu_policy_learns_from_the_search(candidates):
     """Acting, searching, recording and one update, as a user runs them; the memory behind the window is that of the rows that were played."""
     env = environments(48, 'default30')
     c = ActionCatalogue(env.case)
@@ -236,7 +237,7 @@ def test_gpu_policy_learns_from_the_search():
     memory = policy.memory(48)
     optimizer = torch.optim.SGD(policy.parameters(), lr=1e-3)
     for _ in range(2):
-        loss, reward = imitate(env, policy, optimizer, memory, steps=9, candidates=5)
+        loss, reward = imitate(env, policy, optimizer, memory, steps=9, candidates=candidates)
         assert torch.isfinite(loss) and float(loss) > 0 and np.isfinite(reward)
         assert all(torch.isfinite(m).all() for m in memory.windows + memory.states)
     for (name, p), old in zip(policy.named_parameters(), before):
