@@ -10,8 +10,8 @@
 //   dl and dl^T against transposed copies of weight and hidden -> the two gradients.
 // The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size.
 //
-// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 485 us (835 TFLOP/s), the second 765 us (530; it
-// writes 1.6 GB), the third 940 us for both (860).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
+// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 470 us (860 TFLOP/s), the second 790 us (510; it
+// writes 1.6 GB, and the transposed copies), the third 935 us for both (870).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
 // alone, 466 and 325 us for the other two.  4096 rows: 112 us, and 83 of those are the product without its epilogue (10 vector instructions a logit),
 // which the other workgroups of a CU cover in part.
 //
