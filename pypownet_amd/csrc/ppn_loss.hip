@@ -79,20 +79,25 @@ template <typename T, int MI, int NI, int WM, int WN> struct Product {
 
   __device__ static int spot(int row, int part) { return row * LINE + ((part ^ (row & 7)) << 4); }
 
-  // 8 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().
+  // 8 lines into LDS at byte `to`.  The transfer is counted by the wave's vector memory counter and nothing else waits for it: see run().  A scalar
+  // write of M0 (where the lines go) needs one wait state before the load that reads it; the compiler does not look into assembly for that.
+  // (__builtin_amdgcn_global_load_lds would bring it along, but makes branches of the choice of `zeros` and 64-bit vector additions of the addresses.)
   __device__ static void transfer(unsigned to, const char* base, unsigned offset) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
   }
 
   // The same with an address a lane, for the last stage where it is not a whole line: what is past its end is read from `zeros`.
   __device__ static void transfer(unsigned to, const char* address) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(address) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(address) : "memory", "m0");
   }
 
-  // The same for all lanes of the wave, and in scalar registers.
+  // The same for all lanes of the wave, and in scalar registers; with the five wait states between a vector instruction's write of a scalar register
+  // and a memory operation (in the assembly above) that reads it.
   __device__ static const char* scalar(const char* p) {
     const uint64_t v = (uint64_t)p;
-    return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+    uint64_t r = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+    asm volatile("s_nop 4" : "+s"(r));
+    return (const char*)r;
   }
 
   __device__ void run(const Operands& o, char* lds, int64_t m0, int64_t n0, int64_t k0, int64_t k1) {

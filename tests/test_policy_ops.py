@@ -218,6 +218,80 @@ def test_policy_kernels_mir_has_no_vector_code_in_front_of_an_exec_restore():
     assert r.stdout.count(' 0 vector instruction(s) in front of one') == 3, r.stdout
 
 
+def missing_waits(assembly):
+    """Lines of one unit's assembly where a wait state is missing that the compiler does not add for inline assembly: a transfer into LDS needs one
+    between a scalar write of M0 and itself, a memory operation in inline assembly five between a vector instruction's write of a scalar register and
+    itself.  Instructions count as one, s_nop n as n + 1; what was written lately is followed along the branches."""
+    import re
+
+    def scalars(text):
+        return [r for a, b, c in re.findall(r'\bs(?:\[(\d+):(\d+)\]|(\d+)\b)', text) for r in (range(int(a), int(b) + 1) if a else [int(c)])]
+    lines, inline = [], False
+    for line in assembly.splitlines():
+        inline = '#ASMSTART' in line or inline and '#ASMEND' not in line
+        text = line.split(';')[0].strip()
+        if text.endswith(':') or text and not text.startswith('.'):
+            op, _, rest = text.partition(' ')
+            lines.append((text, op, [t.strip() for t in rest.split(',')], rest, inline))
+    arriving, found, again = {}, set(), True      # label -> register (or 'm0') -> wait states since it was written, of the branches to it
+    while again:
+        again, since = False, {}
+        for text, op, operands, rest, inline in lines:
+            if op.endswith(':'):
+                since = {r: min(since.get(r, 9), arriving.get(op[:-1], {}).get(r, 9)) for r in {*since, *arriving.get(op[:-1], {})}}
+                continue
+            if '_load_lds_' in op and 'm0' in since and since['m0'] < 1:
+                found.add('M0: ' + text)
+            if inline and op.startswith(('global_', 'buffer_', 'flat_', 'scratch_')) and any(r in since for r in scalars(rest)):
+                found.add('vector write: ' + text)
+            passed = int(operands[0], 0) + 1 if op == 's_nop' else 1
+            since = {r: n + passed for r, n in since.items() if n + passed < 5}
+            if op.startswith('v_'):
+                since.update({r: 0 for r in scalars(operands[0]) + (scalars(operands[1]) if '_co_' in op else [])})
+            elif op.startswith(('s_branch', 's_cbranch')):
+                before = arriving.setdefault(operands[0], {})
+                for r, n in since.items():
+                    if n < before.get(r, 9):
+                        before[r], again = n, True
+                if op == 's_branch':
+                    since = {}
+            elif op == 's_endpgm':
+                since = {}
+            elif op.startswith('s_'):
+                for r in scalars(operands[0]):
+                    since.pop(r, None)
+                if operands[0] == 'm0':
+                    since['m0'] = 0
+    return sorted(found)
+
+
+def test_missing_waits_are_found():
+    def asm(*lines):
+        return '\n'.join([';;#ASMSTART', *lines, ';;#ASMEND'])
+    move, load = 's_mov_b32 m0, s20', 'global_load_lds_dwordx4 v1, s[4:5]'
+    assert len(missing_waits(asm(move, load))) == 1 and not missing_waits(asm(move, 's_nop 0', load)) and not missing_waits(asm(move, 'v_mov_b32 v2, 0', load))
+    first = 'v_readfirstlane_b32 s5, v3\n'
+    assert len(missing_waits(first + asm('s_nop 3', load))) == 1 and not missing_waits(first + asm('s_nop 4', load))
+    assert not missing_waits(first + 's_add_u32 s5, s5, 4\n' + asm(load)) and not missing_waits('v_readfirstlane_b32 s6, v3\n' + asm(load))
+    over = first + 's_branch .L1\n.L0:\n' + asm(load) + '\ns_endpgm\n.L1:\n'
+    assert not missing_waits(over) and len(missing_waits(over + 's_cbranch_scc1 .L0\n')) == 1 and not missing_waits(over + 's_nop 3\ns_branch .L0\n')
+
+
+def test_loss_kernels_assembly_has_its_wait_states(tmp_path):
+    import __graft_entry__ as g
+    hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
+    if not os.path.exists(hipcc):
+        pytest.skip('no hipcc')
+    csrc, out = os.path.join(ROOT, 'pypownet_amd', 'csrc'), str(tmp_path / 'unit.s')
+    subprocess.run([hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', *g.POLICY_FLAGS, '--cuda-device-only', '-S', os.path.join(csrc, 'ppn_loss.hip'),
+                    '-o', out], check=True, stderr=subprocess.DEVNULL, timeout=300)
+    assembly = open(out).read()
+    assert assembly.count('global_load_lds_dwordx4') > 0 and missing_waits(assembly) == []
+    for unit in g.POLICY_UNITS:      # (the only unit whose inline assembly reads or writes memory)
+        text = open(os.path.join(csrc, unit + '.hip')).read()
+        assert unit == 'ppn_loss' or not any(w in text for w in ('global_load', 'global_store', 'buffer_load', 'buffer_store')), unit
+
+
 def test_cpu_tensors_are_refused():
     from pypownet_amd import policy_ops as ops
     x = torch.zeros((2, 3, 4))
