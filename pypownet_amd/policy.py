@@ -175,7 +175,8 @@ class RecurrentPolicy(torch.nn.Module):
 
     def window(self, observations, starts=None, memory=None):
         """``observations [batch, time, observation_length]`` -> (features [batch, time, features], the memory behind the last row).  ``starts`` marks
-        first rows of episodes; ``memory`` (untouched) is what was remembered in front of the first row, nothing when None.  Differentiable."""
+        first rows of episodes; ``memory`` (untouched) is what was remembered in front of the first row, nothing when None.  Differentiable: the
+        backward pass reads that memory again, so acting must not move it on in between (autograd raises); act on a copy, as ``imitate`` does."""
         if memory is not None:
             self._check_memory(memory, observations.shape[0])
         rows = self._inlet(observations)

@@ -22,6 +22,7 @@ import struct
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .engine import EngineError
@@ -291,7 +292,7 @@ def short_conv(x, weight, bias=None, activation=None, starts=None, initial_state
 
 def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, starts=None):
     """One row of each of ``x``'s environments: ``x [rows, channels]``, ``state [environments, taps - 1, channels]`` (x's type, contiguous) moved on in
-    place, parameters as for ``short_conv``.  ``env_ids [rows]`` says whose rows they are (``BatchedRunEnv.recv``'s ids; row i is environment i when
+    place (a window that began with this very tensor cannot be learned from behind that: autograd raises), parameters as for ``short_conv``.  ``env_ids [rows]`` says whose rows they are (``BatchedRunEnv.recv``'s ids; row i is environment i when
     None); a negative id is padding: y = 0 and no state is touched.  An id out of range, or one that an earlier row has, gives NaN and touches no
     state.  ``starts [rows]`` empties the window first.  Returns y [rows, channels]."""
     try:      # as a loop calls it; the rest is looked at one by one
@@ -323,6 +324,7 @@ def short_conv_step(x, state, weight, bias=None, activation=None, env_ids=None, 
     _call(_load().ppn_conv_step, _CONV_STEP.pack(_CONV_STEP.size, _TYPES[x.dtype], _activation(activation), n, environments, d, before + 1, x.data_ptr(), row,
                                                  weight.data_ptr(), 0 if bias is None else bias.data_ptr(), state.data_ptr(),
                                                  0 if env_ids is None else env_ids.data_ptr(), 0 if starts is None else starts.data_ptr(), y.data_ptr(), d), device)
+    increment_version(state)      # (a window that began with this state and is still to be learned from has lost it: autograd says so)
     return y
 
 
@@ -363,20 +365,21 @@ class _SelectiveScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         x, dt, A, B, C, D, z, dt_bias, initial = _scan_layout(x, dt, A, B, C, D, z, dt_bias, initial)
         y, final, marks = _scan_forward((x, dt, A, B, C, D, z, dt_bias, starts, initial, soft), want_final, True)
-        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, initial, starts, marks)
-        ctx.soft = soft
+        # (the backward pass restarts from the checkpoints: the initial state itself may have moved on by then)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, starts, marks)
+        ctx.soft, ctx.begun = soft, initial is not None
         return y, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
-        x, dt, A, B, C, D, z, dt_bias, initial, starts, marks = ctx.saved_tensors
+        x, dt, A, B, C, D, z, dt_bias, starts, marks = ctx.saved_tensors
         if dy is None and dfinal is None:
             return (None,) * 12
         dfinal = None if dfinal is None else dfinal.contiguous()
         dx, ddt, dz = _window_like(x), _window_like(dt), None if z is None else _window_like(z)
         dA, dD = torch.empty_like(A), None if D is None else torch.empty_like(D)
-        dbias, dinitial = None if dt_bias is None else torch.empty_like(dt_bias), None if initial is None else torch.empty_like(initial)
+        dbias, dinitial = None if dt_bias is None else torch.empty_like(dt_bias), A.new_empty((x.shape[0], *A.shape)) if ctx.begun else None
         dB, dC = B.new_empty(B.shape), C.new_empty(C.shape)
         if x.shape[0] == 0 or x.shape[1] == 0:          # no rows: the state passes through
             for v in (dA, dD, dbias):
@@ -388,7 +391,7 @@ class _SelectiveScan(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         lib = _load()
         _with_workspace(lib.ppn_scan_backward_workspace, lib.ppn_scan_backward,
-                        _scan_front(x, dt, A, B, C, D, z, dt_bias, starts, initial, ctx.soft, None, None, marks) +
+                        _scan_front(x, dt, A, B, C, D, z, dt_bias, starts, None, ctx.soft, None, None, marks) +
                         _SCAN_BACK.pack(*_at(dy), _ptr(dfinal), *_at(dx), *_at(ddt), *_at(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias),
                                         _ptr(dinitial), 0, 0), x.device)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dinitial, None, None, None
@@ -494,6 +497,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
           _SCAN_STEP.pack(_SCAN_STEP.size, _TYPES[dtype], 1 if dt_softplus else 0, n, environments, d, groups, states, x.data_ptr(), strides[0], dt.data_ptr(),
                           strides[1], A.data_ptr(), B.data_ptr(), b_row, b_group, C.data_ptr(), c_row, c_group, _ptr(D), _ptr(dt_bias), _ptr(z), gate,
                           state.data_ptr(), _ptr(env_ids), _ptr(starts), y.data_ptr(), d), device)
+    increment_version(state)
     return y
 
 

@@ -279,3 +279,24 @@ def test_gpu_policy_with_environments_at_their_own_pace():
     assert (steps == 6).all()
     assert all(torch.isfinite(m).all() for m in memory.windows + memory.states)
     assert (memory.states[0].abs().amax(dim=(1, 2)) > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+def test_gpu_acting_between_a_loss_and_its_backward_pass(dtype):
+    """Acting moves a memory on in place; a window that began with it cannot be learned from any more, and says so.  From a copy of it, it can."""
+    c = ActionCatalogue(load_env('default14')[0])
+    torch.manual_seed(10)
+    policy = RecurrentPolicy(c, 538, features=16, layers=2, dtype=dtype).cuda()
+    b, t = 4, 9
+    obs, target = rows_of('x', b, t, 538).cuda(), torch.zeros((b, t), dtype=torch.int64, device='cuda')
+    memory = policy.memory(b)
+    policy.act(obs[:, 0], memory)
+    copy = PolicyMemory([w.clone() for w in memory.windows], [s.clone() for s in memory.states])
+    want = torch.autograd.grad(policy.loss(obs, target, memory=copy)[0].mean(), list(policy.parameters()))
+    again, _ = policy.loss(obs, target, memory=copy)
+    shared, _ = policy.loss(obs, target, memory=memory)
+    policy.act(obs[:, 1], memory)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(again.mean(), list(policy.parameters())), want))
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        shared.mean().backward()

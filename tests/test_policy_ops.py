@@ -959,3 +959,35 @@ def test_gpu_gradients_of_gradients_are_refused():
     dh, = torch.autograd.grad(ops.action_cross_entropy(h, w, torch.arange(5, device='cuda')).sum(), h, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dh.sum(), h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_a_state_stepped_between_a_window_and_its_backward_pass(dtype):
+    """The convolution's backward pass reads its initial rows again: moving them on in between is an error, as with torch's own operations in place.  The
+    scan's does not: its gradients are those of the state the window began with."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(41)
+    b, t, d, n = 3, 11, 24, 8
+    x, w = rand(gen, b, t, d, dtype=dtype).cuda().requires_grad_(True), rand(gen, d, 4).cuda().requires_grad_(True)
+    window = rand(gen, b, 3, d, dtype=dtype).cuda()
+    y = ops.short_conv(x, w, activation='silu', initial_state=window)
+    ops.short_conv_step(x.detach()[:, 0], window, w.detach(), activation='silu')
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.float().sum().backward()
+    A, bc = -torch.rand((d, n), generator=gen).cuda().requires_grad_(True) - 0.1, [rand(gen, b, t, 1, n, dtype=dtype).cuda() for _ in range(2)]
+    first = rand(gen, b, d, n).cuda()
+    for stepped in (False, True):
+        state = first.clone().requires_grad_(True)
+        y = ops.selective_scan(x, x, A, *bc, dt_softplus=True, initial_state=state)
+        before = state._version
+        if stepped:
+            with torch.no_grad():
+                ops.selective_scan_step(x.detach()[:, 0], x.detach()[:, 0], A.detach(), bc[0][:, 0], bc[1][:, 0], state, dt_softplus=True)
+            assert state._version > before
+        grads = torch.autograd.grad(y, [x, state], torch.ones_like(y))
+        if stepped:
+            assert all(torch.equal(p, q) for p, q in zip(grads, kept))
+        kept = grads
+    with torch.inference_mode():      # (a tensor without a version counter)
+        ops.short_conv_step(x.detach()[:, 0], torch.zeros((b, 3, d), dtype=dtype, device='cuda'), w.detach())
