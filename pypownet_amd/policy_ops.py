@@ -15,14 +15,16 @@ Tensors are float32, bfloat16 or float16 on the GPU, all activations of a call o
 ``dt_bias``) and states are float32 -- the convolution's window excepted, which holds rows and has their type.  Kernels are queued on torch's
 current stream of the tensors' device; nothing synchronises.  Workspaces come from torch's allocator, so the calls can be captured into a
 graph -- a training step as usual with its own leaves: capturing a backward pass of leaves that an eager graph still holds ends in an error of torch's
-autograd, here as with any other function.  Arguments the kernels do not take are refused with TypeError / ValueError before anything is launched; gradients of gradients are
-not available.
+autograd, here as with any other function.  Arguments the kernels do not take are refused with TypeError / ValueError before anything is
+launched; gradients of gradients, forward-mode derivatives and tracing are not available, and refused.
 """
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
+from torch.jit import is_tracing
 
 from . import _lib
 from .engine import EngineError
@@ -146,6 +148,10 @@ def _at(t):
 
 
 def _wants_grad(*tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError('forward-mode derivatives are not available')
+    if is_tracing():
+        raise ValueError('these operators cannot be traced: their kernels are not torch operations')
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

@@ -991,3 +991,34 @@ def test_gpu_a_state_stepped_between_a_window_and_its_backward_pass(dtype):
         kept = grads
     with torch.inference_mode():      # (a tensor without a version counter)
         ops.short_conv_step(x.detach()[:, 0], torch.zeros((b, 3, d), dtype=dtype, device='cuda'), w.detach())
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_derivatives_and_tracing_are_refused():
+    """... not answered without the tangent, or with a recording that holds no kernel."""
+    import torch.autograd.forward_ad as forward
+    from pypownet_amd import policy_ops as ops
+    r = lambda *s: torch.randn(s, device='cuda')      # noqa: E731
+    x, row, w, A, bc, bc_row = r(2, 5, 8), r(2, 8), r(8, 4), -torch.rand((8, 4), device='cuda'), r(2, 5, 1, 4), r(2, 1, 4)
+    target = torch.zeros((2,), dtype=torch.int64, device='cuda')
+    calls = {
+        'conv': (lambda v: ops.short_conv(v, w), x), 'conv weight': (lambda v: ops.short_conv(x, v), w), 'conv step': (lambda v: ops.short_conv_step(v, r(2, 3, 8), w), row),
+        'scan': (lambda v: ops.selective_scan(v, x, A, bc, bc), x), 'scan D': (lambda v: ops.selective_scan(x, x, A, bc, bc, D=v), r(8)),
+        'scan step': (lambda v: ops.selective_scan_step(v, row, A, bc_row, bc_row, r(2, 8, 4)), row),
+        'scan state': (lambda v: ops.selective_scan_step(row, row, A, bc_row, bc_row, v), r(2, 8, 4)),
+        'loss': (lambda v: ops.action_cross_entropy(v, r(6, 8), target), row),
+    }
+    for name, (call, v) in calls.items():
+        plain = call(v.clone())
+        for mode in (torch.no_grad(), torch.enable_grad()):
+            with mode, forward.dual_level():
+                with pytest.raises(ValueError, match='forward-mode'):
+                    call(forward.make_dual(v.clone(), torch.ones_like(v)))
+                    pytest.fail(name)
+                assert call(v.clone()).shape == plain.shape      # (a level without a tangent of ours is no reason to refuse)
+        with pytest.raises(Exception):
+            torch.func.jvp(call, (v.clone(),), (torch.ones_like(v),))
+            pytest.fail(name)
+        with pytest.raises(ValueError, match='traced'), torch.no_grad():
+            torch.jit.trace(call, (v.clone(),), check_trace=False)
+            pytest.fail(name)
