@@ -727,6 +727,9 @@ int check(const ppn_loss_args* a) {
   return PPN_OK;
 }
 
+// Rows of allowed lie apart, or are all the same one (stride 0).
+bool mask_fits(const ppn_loss_args* a) { return !a->allowed || a->rows <= 1 || a->allowed_row == 0 || a->allowed_row >= ceil_div(a->actions, 32); }
+
 template <typename T> int pad_rows(const void* in, int64_t row, int64_t rows, int64_t cols, void* out, int64_t cols_padded, hipStream_t s) {
   const int64_t blocks = ceil_div(rows * cols_padded, 256);
   if (blocks > 0x7fffffff) return fail(PPN_E_INVALID, "loss: an operand is too large");
@@ -748,7 +751,7 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
   if (int rc = check(a)) return rc;
   if (a->rows == 0) return PPN_OK;
   if (!a->hidden || !a->weight || !a->target || !a->loss || !a->lse) return fail(PPN_E_INVALID, "ppn_loss_forward: hidden, weight, target, loss and lse are needed");
-  if (a->allowed && a->allowed_row < ceil_div(a->actions, 32)) return fail(PPN_E_INVALID, "ppn_loss_forward: a row of allowed has too few words");
+  if (!mask_fits(a)) return fail(PPN_E_INVALID, "ppn_loss_forward: a row of allowed has too few words");
   const ForwardPlan p = plan_forward(a);
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_forward: the workspace is too small");
   char* w = (char*)a->workspace;
@@ -783,7 +786,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
   if (a->rows == 0) return fail(PPN_E_INVALID, "ppn_loss_backward: there are no rows");
   if (!a->hidden || !a->weight || !a->target || !a->loss || !a->lse || !a->dloss)
     return fail(PPN_E_INVALID, "ppn_loss_backward: hidden, weight, target, loss, lse and dloss are needed");
-  if (a->allowed && a->allowed_row < ceil_div(a->actions, 32)) return fail(PPN_E_INVALID, "ppn_loss_backward: a row of allowed has too few words");
+  if (!mask_fits(a)) return fail(PPN_E_INVALID, "ppn_loss_backward: a row of allowed has too few words");
   const BackwardPlan p = plan_backward(a);
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_backward: the workspace is too small");
   char* w = (char*)a->workspace;

@@ -553,7 +553,7 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
         loss[i] = log sum_v exp(hidden[i] . weight[v]) - hidden[i] . weight[target[i]]          over the actions v that ``allowed`` has in row i
 
     ``hidden [rows, features]`` and ``weight [actions, features]`` of one type, ``target [rows]`` int64.  ``allowed [rows, ceil(actions / 32)]``
-    int32 has one bit per action (``pack_allowed``), all actions when None.  A row whose target is ``ignore_index``, or that allows nothing, has loss 0
+    int32 has one bit per action (``pack_allowed``; one row expanded over all is fine), all actions when None.  A row whose target is ``ignore_index``, or that allows nothing, has loss 0
     and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
     NaN.  What a row does not allow is not looked at (behind the loss, a weight row that is not finite still makes NaN of dhidden).  ``-loss`` is the
     log-probability of the action ``target``.  Differentiable in hidden and weight (the result is kept for that: not to be changed in place); sums
@@ -570,6 +570,8 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
     if allowed is not None:
         _like('allowed', allowed, (n, (v + 31) // 32), torch.int32, hidden.device)
         allowed = _rows(allowed)
+        if 0 < allowed.stride(0) < allowed.shape[1]:      # (rows that overlap: the entry point takes rows apart, or one for all)
+            allowed = allowed.contiguous()
     target = target.contiguous()
     ignore_index = int(ignore_index)
     if _wants_grad(hidden, weight):

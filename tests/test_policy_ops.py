@@ -1022,3 +1022,24 @@ def test_gpu_forward_mode_derivatives_and_tracing_are_refused():
         with pytest.raises(ValueError, match='traced'), torch.no_grad():
             torch.jit.trace(call, (v.clone(),), check_trace=False)
             pytest.fail(name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_action_cross_entropy_with_one_mask_for_all_rows(dtype):
+    """A row of bits expanded over the rows, or rows of bits that overlap, are as good as copies of them."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(42)
+    n, v, f = 70, 177, 40
+    h, w = rand(gen, n, f, dtype=dtype).cuda().requires_grad_(True), rand(gen, v, f, scale=0.3, dtype=dtype).cuda().requires_grad_(True)
+    mask = torch.rand((1, v), generator=gen) < 0.6
+    mask[0, 5] = True
+    target, up = torch.full((n,), 5, device='cuda'), rand(gen, n).cuda()
+    one = ops.pack_allowed(mask.cuda())
+    words = torch.randint(-2 ** 31, 2 ** 31, (n + 5,), generator=gen).to(torch.int32).cuda() | 32
+    for bits in (one.expand(n, -1), words.as_strided((n, 6), (1, 1)), one.expand(n, -1)[:1]):
+        rows = bits.shape[0]
+        loss = ops.action_cross_entropy(h[:rows], w, target[:rows], allowed=bits)
+        want = ops.action_cross_entropy(h[:rows], w, target[:rows], allowed=bits.contiguous().clone())
+        assert torch.equal(loss, want) and torch.isfinite(loss).all()
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, [h, w], up[:rows]), torch.autograd.grad(want, [h, w], up[:rows])))
