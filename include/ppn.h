@@ -574,8 +574,8 @@ int ppn_scan_step(const ppn_scan_step_args* a, void* stream);
 /* Cross entropy over a catalogue of actions, without keeping the logits:
  *   loss[i] = log sum_{v allowed} exp(hidden[i] . weight[v]) - hidden[i] . weight[target[i]]
  * allowed: bit v & 31 of word v >> 5 of row i (NULL: every action; allowed_row 0: one row for all).  target = ignore_index, or a row with nothing
- * allowed: loss 0, no gradient.  A target that is not allowed: loss +inf.  A target outside 0..actions-1: loss NaN, and so
- * its gradients.  lse (log of the sum; saved for the backward pass): +inf where the row has no gradient.
+ * allowed: loss 0, no gradient.  A target that is not allowed: loss +inf.  A target outside 0..actions-1, or no
+ * allowed logit above -inf: loss NaN, and so its gradients.  lse (log of the sum; saved for the backward pass): +inf where the row has no gradient.
  * Backward: loss and lse as the forward pass left them and dloss[rows] in; dhidden [rows x features], dweight [actions x features] (each or NULL) out, contiguous. */
 typedef struct ppn_loss_args {
   int64_t struct_bytes, type, rows, actions, features, ignore_index;

@@ -20,6 +20,8 @@
 // probabilities, so dl is scaled by a power of two that brings the largest |dloss| to 2^14, and the scale is taken out at the end.
 #include "ppn_policy.h"
 
+#include <float.h>
+
 namespace ppn_policy {
 namespace {
 
@@ -270,10 +272,18 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) loss_stats(Operands o, StatsA
     }
     sum_over_16(sum);
     // lanes 0..3 of each 16 have a row to write
-    const float t = column & 2 ? (column & 1 ? top[3] : top[2]) : (column & 1 ? top[1] : top[0]);
+    float t = column & 2 ? (column & 1 ? top[3] : top[2]) : (column & 1 ? top[1] : top[0]);
     const float u = column & 2 ? (column & 1 ? sum[3] : sum[2]) : (column & 1 ? sum[1] : sum[0]);
     const int row = p.row_of(i, column);
-    if (column < 4 && m0 + row < o.M) out[row] = make_float2(t, u);
+    if (column < 4 && m0 + row < o.M) {
+      if (t == -INFINITY) {      // nothing allowed here, or allowed logits of minus infinity: the latter leave the lowest number
+        unsigned any = 0;
+#pragma unroll
+        for (int j = 0; j < NI; j += 2) any |= mask[row][p.wave_n / 32 + j / 2];
+        if (any) t = -FLT_MAX;
+      }
+      out[row] = make_float2(t, u);
+    }
   }
 }
 
@@ -287,7 +297,8 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
   {
     const int64_t row = first + (threadIdx.x & 15) < a.rows ? first + (threadIdx.x & 15) : a.rows - 1;
     float top = -INFINITY, sum = 0.0f;
-    // (a tile without an allowed action has the sum 0 and the maximum -infinity; one with a NaN has the sum NaN whatever its maximum)
+    // (a tile without an allowed action has the sum 0 and the maximum -infinity; one whose allowed logits are all -infinity the sum 0 and the lowest
+    // number; one with a NaN has the sum NaN whatever its maximum)
     constexpr int AHEAD = 4;
     for (int64_t c = threadIdx.x / 16; c < columns; c += 16 * AHEAD) {
       float2 v[AHEAD];
@@ -340,8 +351,9 @@ __global__ void __launch_bounds__(256) loss_join(ppn_loss_args a, const float2* 
   float loss = 0.0f, lse = INFINITY;
   if (at != a.ignore_index && !nothing) {
     const bool legal = known && (!a.allowed || ((a.allowed[row * a.allowed_row + (at >> 5)] >> (at & 31)) & 1));
-    loss = !known ? NAN : legal ? whole - wanted[threadIdx.x] : INFINITY;
-    lse = !known || whole == INFINITY ? NAN : whole;      // (an infinite logit: the shares are not defined)
+    const bool undefined = !known || fabsf(whole) == INFINITY;      // (a logit of infinity, or none above -infinity: there are no shares)
+    loss = !known ? NAN : !legal ? INFINITY : undefined ? NAN : whole - wanted[threadIdx.x];
+    lse = undefined ? NAN : whole;
   }
   a.loss[row] = loss;
   a.lse[row] = lse;

@@ -555,7 +555,7 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
     ``hidden [rows, features]`` and ``weight [actions, features]`` of one type, ``target [rows]`` int64.  ``allowed [rows, ceil(actions / 32)]``
     int32 has one bit per action (``pack_allowed``; one row expanded over all is fine), all actions when None.  A row whose target is ``ignore_index``, or that allows nothing, has loss 0
     and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
-    NaN.  What a row does not allow is not looked at (behind the loss, a weight row that is not finite still makes NaN of dhidden).  ``-loss`` is the
+    NaN, and so does a row whose allowed logits are all -inf.  What a row does not allow is not looked at (behind the loss, a weight row that is not finite still makes NaN of dhidden).  ``-loss`` is the
     log-probability of the action ``target``.  Differentiable in hidden and weight (the result is kept for that: not to be changed in place); sums
     run in a fixed order."""
     _leading('hidden', hidden)

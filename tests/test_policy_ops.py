@@ -1043,3 +1043,33 @@ def test_gpu_action_cross_entropy_with_one_mask_for_all_rows(dtype):
         want = ops.action_cross_entropy(h[:rows], w, target[:rows], allowed=bits.contiguous().clone())
         assert torch.equal(loss, want) and torch.isfinite(loss).all()
         assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, [h, w], up[:rows]), torch.autograd.grad(want, [h, w], up[:rows])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('v', [3, 200, 20000])
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_action_cross_entropy_where_every_allowed_logit_is_minus_infinity(dtype, v):
+    """... is not a row that allows nothing: its loss is not defined, and says so."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(43)
+    n, f = 260, 24
+    h, w = rand(gen, n, f, dtype=dtype).abs() + 0.125, rand(gen, v, f, scale=0.3, dtype=dtype)
+    w[1:] = -float('inf')                                     # action 0 alone has a finite logit
+    mask = torch.rand((n, v), generator=gen) < 0.5
+    mask[:, 1] = True
+    mask[:, 0] = torch.arange(n) % 3 != 0
+    mask[7] = False
+    mask[8] = torch.arange(v) == 1
+    target = torch.zeros((n,), dtype=torch.int64)
+    target[4] = 1
+    target[mask[:, 0].logical_not()] = 1
+    target[7], target[10] = 1, -100
+    want = loss_definition(h.double(), w.double(), target, mask)
+    lost = torch.isnan(want)
+    assert lost[3] and lost[8] and want[7] == 0 and want[10] == 0 and want[4] == float('inf') and want[5] == 0
+    hg = h.cuda().requires_grad_(True)
+    loss = ops.action_cross_entropy(hg, w.cuda(), target.cuda(), allowed=ops.pack_allowed(mask.cuda()))
+    got = loss.detach().double().cpu()
+    assert torch.equal(torch.isnan(got), lost)
+    # (the logarithm of one exponential: zero but for the rounding of logits below 16 in size, summed over 24 features)
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and (got[torch.isfinite(want)].abs() <= 2 * (f + 16) * STEP * 16).all()
