@@ -106,8 +106,8 @@ template <int V, int LPC> struct Kept {
 
 // ---- staging -----------------------------------------------------------------------------------------------------------------------
 // The rows are taken in blocks of ROWS without a branch that a memory operation hangs on: the wait for a block's loads would otherwise be a
-// wait for every store before them too.  A block past the end of the time axis (or of the chunk) repeats its last row with a step
-// size of zero, which leaves the state as it is and writes the last row's values again; a lane past the last channel, and the second and
+// wait for every store before them too.  A block past the end of the time axis (or of the chunk) repeats its last row, which leaves the state as it
+// is and writes the last row's values again; a lane past the last channel, and the second and
 // later lanes of a channel, write what the channel's own lane writes.
 
 // Addresses are a pointer that is the same for the wave, in scalar registers, and an unsigned 32-bit byte offset.  A block's rows lie within such
@@ -243,14 +243,18 @@ template <typename T> __device__ inline void step_sizes(const Column<T>& dt, flo
   for (int j = 1; j < ROWS; ++j) delta[j] = j < rows ? delta[j] : 0.0f;
 }
 
-// The state behind a row; a row that begins an episode drops the state before, whatever is in it (a branch the whole wave takes).
-template <int NS> __device__ inline void advance(const float (&before)[NS], float (&h)[NS], float delta, float w, const float (&A2)[NS], const float (&bv)[NS], bool begin) {
+// The state behind a row; a row that begins an episode drops the state before, whatever is in it, and a repeated row (past the block's last one) leaves it,
+// whatever the row holds: a step size of zero times an infinity would not (branches the whole wave takes).
+template <int NS> __device__ inline void advance(const float (&before)[NS], float (&h)[NS], float delta, float w, const float (&A2)[NS], const float (&bv)[NS], bool begin, bool real) {
   if (begin) {
 #pragma unroll
     for (int n = 0; n < NS; ++n) h[n] = w * bv[n];
-  } else {
+  } else if (real) {
 #pragma unroll
     for (int n = 0; n < NS; ++n) h[n] = __builtin_amdgcn_exp2f(delta * A2[n]) * before[n] + w * bv[n];
+  } else {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[n] = before[n];
   }
 }
 
@@ -351,7 +355,7 @@ __global__ void __launch_bounds__(64, 4) scan_forward(ppn_scan_args a, int64_t c
       const float step = anew(delta[j]);
       read_states<NS>(sb + j * STATES + p.part * NS, bv);
       const float xv = widened(x.v[j]);
-      advance<NS>(h, h, step, step * xv, A2, bv, (now >> j) & 1);
+      advance<NS>(h, h, step, step * xv, A2, bv, (now >> j) & 1, j < rows);
       if constexpr (MODE != SUMMARY) {
         float cv[NS], s = 0.0f;
         read_states<NS>(sc + j * STATES + p.part * NS, cv);
@@ -484,7 +488,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
       float bv[NS];
       const float step = anew(delta[j]);
       read_states<NS>(sb + j * STATES + p.part * NS, bv);
-      advance<NS>(before, after, step, step * widened(x.v[j]), A2, bv, (now >> j) & 1);
+      advance<NS>(before, after, step, step * widened(x.v[j]), A2, bv, (now >> j) & 1, true);      // (what is behind the last row is not looked at)
     };
 #pragma unroll
     for (int j = ROWS - 1; j >= 0; --j) {
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
         if (begin) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) e[n] = 0.0f;
-        } else {
+        } else if (j < rows) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) e[n] = __builtin_amdgcn_exp2f(step * A2[n]) * (e[n] + u * cv[n]);
         }
@@ -529,7 +533,7 @@ __global__ void __launch_bounds__(64, 2) scan_backward(ppn_scan_args a, int64_t 
         if (begin) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) e[n] = 0.0f;
-        } else {
+        } else if (j < rows) {
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
             e[n] *= __builtin_amdgcn_exp2f(step * A2[n]);

@@ -1073,3 +1073,33 @@ def test_gpu_action_cross_entropy_where_every_allowed_logit_is_minus_infinity(dt
     assert torch.equal(torch.isnan(got), lost)
     # (the logarithm of one exponential: zero but for the rounding of logits below 16 in size, summed over 24 features)
     assert torch.equal(torch.isinf(got), torch.isinf(want)) and (got[torch.isfinite(want)].abs() <= 2 * (f + 16) * STEP * 16).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t,n', [(1, 16), (5, 12), (13, 16), (16, 16), (61, 16), (61, 40)])
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_selective_scan_rows_past_the_last_one_do_not_count(dtype, t, n):
+    """Lengths that are no multiple of a block: a last row that is infinite, and channels that forget at once (A = -infinity), keep their values."""
+    case = (2, t, 70, 1, n, True, True, True, True, False, True, False)
+    v, _, dy, dfinal = scan_inputs(case, dtype, seed=44)
+    v['B'], v['C'], v['D'], v['z'] = v['B'].abs(), v['C'].abs(), v['D'].abs(), v['z'].abs() + 0.5
+    v['A'][3] = -float('inf')
+    if n == 16:      # (elsewhere an infinity times the zeros that fill the last lane's states is NaN)
+        v['x'][1, -1, 5] = float('inf')
+    y64, last64 = scan_definition(*[v[k].double() for k in ORDER[:8]], True, None, v['initial'].double())
+    assert torch.isinf(y64[1, -1, 5]) == (n == 16) and torch.isfinite(y64[:, :, 3]).all()
+    own = {k: v[k].cuda().requires_grad_(True) for k in ORDER}
+    chain = min(t, 64) * 12 + n + 32
+    for keep in (False, True):
+        with torch.set_grad_enabled(keep):
+            y, last = own_scan(own, True, None)
+        close('y', y, y64, dtype, chain, 4 * float(y64[torch.isfinite(y64)].abs().max()))
+        close('final', last, last64, torch.float32, chain, 4 * float(last64[torch.isfinite(last64)].abs().max()))
+    # behind the infinity nothing is finite, but for the channel that forgets in the other environment
+    ref = {k: v[k].double() for k in ORDER}
+    ref['x'].requires_grad_(True)
+    y64, last64 = scan_definition(*[ref[k] for k in ORDER[:8]], True, None, ref['initial'])
+    want, = torch.autograd.grad([y64, last64], ref['x'], [dy.double(), dfinal.double()])
+    got, = torch.autograd.grad([y, last], own['x'], [dy.cuda(), dfinal.cuda()])
+    assert torch.isfinite(want[0, :, 3]).all()
+    close('dx', got[0, :, 3], want[0, :, 3], dtype, 2 * chain + 32, 8 * float(want[0].abs().max()))
