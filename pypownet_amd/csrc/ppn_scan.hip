@@ -258,6 +258,13 @@ template <int NS> __device__ inline void advance(const float (&before)[NS], floa
   }
 }
 
+// What a chunk leaves of a state that enters it: exp2(rate) h, where the exponential may pass 32 bits and the product need not (A > 0 or delta < 0; a state
+// of zero stays zero).  In two halves: what 2^256 does to a number is beyond 32 bits anyway.
+__device__ inline float carried(float rate, float h) {
+  const float half = __builtin_amdgcn_exp2f(0.5f * rate);
+  return h == 0.0f ? h : half * (half * h);
+}
+
 // What enters a chunk, from what the chunks before it do (`count` of them, from `first` in steps of `step`), in h: as scan_join, in the wave that goes on
 // with it.
 template <int NS, int LPC>
@@ -278,7 +285,7 @@ __device__ inline void join_chunks(const ppn_scan_args& a, const Place& p, int64
     for (int j = 0; j < AHEAD; ++j)
       if (i0 + j < count) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = cut[j] != 0.0f ? own[j][n] : own[j][n] + __builtin_amdgcn_exp2f(total[j] * A2[n]) * h[n];
+        for (int n = 0; n < NS; ++n) h[n] = cut[j] != 0.0f ? own[j][n] : own[j][n] + carried(total[j] * A2[n], h[n]);
       }
   }
 }
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(64) scan_join(ppn_scan_args a, int64_t chunks,
       if (i0 + j >= chunks) break;
       const int64_t k = BACKWARD ? chunks - 1 - (i0 + j) : i0 + j;
       p[k * per] = h;
-      h = cut[j] != 0.0f ? own[j] : own[j] + __builtin_amdgcn_exp2f(total[j] * A2) * h;
+      h = cut[j] != 0.0f ? own[j] : own[j] + carried(total[j] * A2, h);
     }
   }
 }

@@ -1103,3 +1103,36 @@ def test_gpu_selective_scan_rows_past_the_last_one_do_not_count(dtype, t, n):
     got, = torch.autograd.grad([y, last], own['x'], [dy.cuda(), dfinal.cuda()])
     assert torch.isfinite(want[0, :, 3]).all()
     close('dx', got[0, :, 3], want[0, :, 3], dtype, 2 * chain + 32, 8 * float(want[0].abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [48, 300, 1000])
+def test_gpu_selective_scan_chunks_that_grow(t):
+    """A state that grows by e^6 a row: what a chunk of rows does to a state outgrows 32 bits, but the states and gradients do not, since they are zero for so long
+    (in front of the last eight rows, and behind the first eight)."""
+    b, d, n = 1, 40, 8
+    gen = torch.Generator().manual_seed(45)
+    v = dict(x=rand(gen, b, t, d), dt=torch.ones((b, t, d)), A=5.9 + 0.1 * torch.rand((d, n), generator=gen), B=rand(gen, b, t, 1, n), C=rand(gen, b, t, 1, n))
+    v.update({k: None for k in ORDER if k not in v})
+    v['x'][:, :-8] = 0
+    dy = rand(gen, b, t, d)
+    y64, last64 = scan_definition(*[None if v[k] is None else v[k].double() for k in ORDER[:8]], False, None, None)
+    own = {k: None if v[k] is None else v[k].cuda().requires_grad_(True) for k in ORDER}
+    y, last = own_scan(own, False, None)
+    assert not y[:, :-8].any()
+    # eight rows of an exponential (argument 6) and two operations; sums of 8
+    big = float(y64.abs().max())
+    close('y', y, y64, torch.float32, 8 * 12 + n + 32, 4 * big)
+    close('final', last, last64, torch.float32, 8 * 12 + 32, 4 * float(last64.abs().max()))
+    with torch.no_grad():
+        assert torch.equal(own_scan(own, False, None)[0], y)
+    # gradients: those of the first eight rows' outputs (behind them there is none, in front of them no state)
+    up = dy.clone()
+    up[:, 8:] = 0
+    names = ['x', 'dt', 'A', 'B', 'C']
+    ref = {k: v[k].double().requires_grad_(True) for k in names}
+    yr, _ = scan_definition(*[ref.get(k) for k in ORDER[:8]], False, None, None)
+    want = torch.autograd.grad(yr, [ref[k] for k in names], up.double())
+    got = torch.autograd.grad(y, [own[k] for k in names], up.cuda())
+    for k, p, q in zip(names, got, want):
+        close('d' + k, p, q, torch.float32, 2 * (8 * 12 + n + 32), 8 * float(want[0].abs().max()) + float(q.abs().max()))
