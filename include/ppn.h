@@ -477,8 +477,9 @@ int ppn_kernel_time(ppn_engine* e, int32_t reset, double* total_ms, int64_t* lau
  * this thread's last refusal.  Safe from several threads at once.  Every struct is 64-bit fields only and begins
  * with struct_bytes = sizeof(it).  Strides count elements; the channel / state stride is always 1.  Sums, states,
  * statistics and parameters are 32-bit floats; `type` is the type of the activations.  Out of range, and refused: more than 2^22
- * channels, rows of time (scan) more than 2^27 elements apart, more than 8 taps or 64 states, 2^18 rows of a step call with ids, 2^22 rows, 2^23 actions or 2^20
- * features of a loss. */
+ * channels (2^24 in a step call), rows of time (scan) more than 2^27 elements apart, more than 8 taps or 64 states, 2^18 rows of a step call with ids, 2^22 rows,
+ * 2^23 actions or 2^20 features of a loss, and whatever would take 2^32 lanes in a launch (rows of a step call: 2^24; waves of 64 channels of an environment: 2^26;
+ * 256 x 128 or 128 x 128 tiles of rows and actions: 2^24). */
 enum { PPN_T_F32 = 0, PPN_T_BF16 = 1, PPN_T_F16 = 2 };
 const char* ppn_policy_error(void);
 

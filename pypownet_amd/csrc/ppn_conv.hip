@@ -448,7 +448,7 @@ extern "C" int ppn_conv_forward(const ppn_conv_args* a, void* stream) {
       const int64_t lanes = a->channels / (w ? WIDE : 1);
       const int64_t span = a->time ? span_for(a->batch, a->time, lanes, 131072) : 1, stretches = a->time ? ceil_div(a->time, span) : 1;
       const int64_t width = slab_width(lanes);
-      if (a->batch * stretches > 0x7fff0000) return fail(PPN_E_INVALID, "convolution: too many environments");
+      if (too_many(ceil_div(a->batch * stretches, 256 / width), 256)) return fail(PPN_E_INVALID, "convolution: too many environments");
       const dim3 grid(ceil_div(a->batch * stretches, 256 / width), ceil_div(lanes, width));
       if (w) conv_forward<T, K, WIDE><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a, span, (int)stretches);
       else conv_forward<T, K, 1><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a, span, (int)stretches);
@@ -500,6 +500,7 @@ extern "C" int ppn_conv_step(const ppn_conv_step_args* a, void* stream) {
       constexpr int K = decltype(k)::value;
       const dim3 grid(a->rows, ceil_div(a->channels / (w ? vec : 1), 256));
       if (grid.y > 65535) return fail(PPN_E_INVALID, "ppn_conv_step: too many channels");
+      if (too_many(a->rows, 256)) return fail(PPN_E_INVALID, "ppn_conv_step: too many rows");
       if (w) conv_step<T, K, WIDE><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
       else conv_step<T, K, 1><<<grid, dim3(256), 0, (hipStream_t)stream>>>(*a);
       return launched("ppn_conv_step");

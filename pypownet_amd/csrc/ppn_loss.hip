@@ -742,11 +742,23 @@ int check(const ppn_loss_args* a) {
 // Rows of allowed lie apart, or are all the same one (stride 0).
 bool mask_fits(const ppn_loss_args* a) { return !a->allowed || a->rows <= 1 || a->allowed_row == 0 || a->allowed_row >= ceil_div(a->actions, 32); }
 
-template <typename T> int pad_rows(const void* in, int64_t row, int64_t rows, int64_t cols, void* out, int64_t cols_padded, hipStream_t s) {
-  const int64_t blocks = ceil_div(rows * cols_padded, 256);
-  if (blocks > 0x7fffffff) return fail(PPN_E_INVALID, "loss: an operand is too large");
-  loss_pad<T><<<dim3(blocks), dim3(256), 0, s>>>((const T*)in, row, rows, cols, (T*)out, cols_padded);
-  return PPN_OK;
+template <typename T> void pad_rows(const void* in, int64_t row, int64_t rows, int64_t cols, void* out, int64_t cols_padded, hipStream_t s) {
+  loss_pad<T><<<dim3(ceil_div(rows * cols_padded, 256)), dim3(256), 0, s>>>((const T*)in, row, rows, cols, (T*)out, cols_padded);
+}
+
+// Every launch of a call, before the first of them.
+template <typename Plan> bool pads_fit(const ppn_loss_args* a, const Plan& p) {
+  return (p.hidden < 0 || !too_many(ceil_div(a->rows * p.features_padded, 256), 256)) && (p.weight < 0 || !too_many(ceil_div(a->actions * p.features_padded, 256), 256));
+}
+bool launches_fit(const ppn_loss_args* a, const ForwardPlan& p) {
+  return pads_fit(a, p) && !too_many(ceil_div(a->rows, p.config.m) * ceil_div(a->actions, p.config.n), 256);
+}
+bool launches_fit(const ppn_loss_args* a, const BackwardPlan& p) {
+  const int64_t down = ceil_div(a->features, 64), across = ceil_div(a->features, p.sums.n);
+  const int64_t grad = ceil_div(a->rows, p.grad.m) * ceil_div(p.piece, p.grad.n) + (ceil_div(p.rows_padded, 64) + ceil_div(p.actions_padded, 64)) * down;
+  const int64_t sums = across * (ceil_div(a->rows, p.sums.m) * p.dh_slots + ceil_div(p.piece, p.sums.m) * p.dw_slots);
+  const int64_t finish = ceil_div(a->rows * a->features, 256) + ceil_div(p.piece * a->features, 256);
+  return pads_fit(a, p) && !too_many(grad, 256) && !too_many(sums, 256) && !too_many(finish, 256);
 }
 
 }  // namespace
@@ -766,22 +778,22 @@ extern "C" int ppn_loss_forward(const ppn_loss_args* a, void* stream) {
   if (!mask_fits(a)) return fail(PPN_E_INVALID, "ppn_loss_forward: a row of allowed has too few words");
   const ForwardPlan p = plan_forward(a);
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_forward: the workspace is too small");
+  if (!launches_fit(a, p)) return fail(PPN_E_INVALID, "loss: too many rows for as many actions and features");
   char* w = (char*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
     Operands o = {a->hidden, a->hidden_row, a->rows, a->weight, a->weight_row, a->actions, p.features_padded};
     if (p.hidden >= 0) {
-      if (int rc = pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s)) return rc;
+      pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s);
       o.A = w + p.hidden, o.lda = p.features_padded;
     }
     if (p.weight >= 0) {
-      if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
+      pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s);
       o.B = w + p.weight, o.ldb = p.features_padded;
     }
     const StatsArgs st = {a->allowed, a->allowed_row, (float2*)(w + p.partial), p.columns};
     const int64_t tm = ceil_div(a->rows, p.config.m), tn = ceil_div(a->actions, p.config.n);
-    if (tm * tn > 0x7fffffff) return fail(PPN_E_INVALID, "loss: too many rows");
     by_tile(p.config, [&](auto t) { loss_stats<T, decltype(t)::mi, decltype(t)::ni, decltype(t)::wm, decltype(t)::wn><<<dim3(tm * tn), dim3(256), 0, s>>>(o, st, tm, tn); });
     loss_join<T><<<dim3(ceil_div(a->rows, 16)), dim3(256), 0, s>>>(*a, st.partial, p.columns);
     return launched("ppn_loss_forward");
@@ -801,6 +813,7 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
   if (!mask_fits(a)) return fail(PPN_E_INVALID, "ppn_loss_backward: a row of allowed has too few words");
   const BackwardPlan p = plan_backward(a);
   if (!a->workspace || a->workspace_bytes < p.bytes) return fail(PPN_E_INVALID, "ppn_loss_backward: the workspace is too small");
+  if (!launches_fit(a, p)) return fail(PPN_E_INVALID, "loss: too many rows for as many actions and features");
   char* w = (char*)a->workspace;
   hipStream_t s = (hipStream_t)stream;
   float* scale = a->type == PPN_T_F16 ? (float*)(w + p.scale) : nullptr;
@@ -810,17 +823,16 @@ extern "C" int ppn_loss_backward(const ppn_loss_args* a, void* stream) {
     const void* weight = a->weight;
     int64_t hidden_row = a->hidden_row, weight_row = a->weight_row;
     if (p.hidden >= 0) {
-      if (int rc = pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s)) return rc;
+      pad_rows<T>(a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden, p.features_padded, s);
       hidden = w + p.hidden, hidden_row = p.features_padded;
     }
     if (p.weight >= 0) {
-      if (int rc = pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s)) return rc;
+      pad_rows<T>(a->weight, a->weight_row, a->actions, a->features, w + p.weight, p.features_padded, s);
       weight = w + p.weight, weight_row = p.features_padded;
     }
     const int64_t down = ceil_div(a->features, 64), hidden_across = ceil_div(p.rows_padded, 64), weight_across = ceil_div(p.actions_padded, 64);
     TransposeJob th = {a->hidden, a->hidden_row, a->rows, a->features, w + p.hidden_t, p.rows_padded, a->lse, (unsigned)hidden_across, a->dweight ? (unsigned)(hidden_across * down) : 0u};
     TransposeJob tw = {a->weight, a->weight_row, a->actions, a->features, w + p.weight_t, p.actions_padded, nullptr, (unsigned)weight_across, a->dhidden ? (unsigned)(weight_across * down) : 0u};
-    if ((hidden_across + weight_across) * down > 0x3fffffff) return fail(PPN_E_INVALID, "loss: an operand is too large");
     if (scale) loss_scale<<<dim3(1), dim3(1024), 0, s>>>(a->dloss, a->lse, a->rows, scale);
     for (int64_t first = 0; first < a->actions; first += p.piece) {
       const int64_t n = a->actions - first < p.piece ? a->actions - first : p.piece, np = padded(n, 64);

@@ -74,6 +74,8 @@ int by_type(int64_t type, F f) {
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// A launch counts its lanes along an axis in 32 bits.
+inline bool too_many(int64_t workgroups, int64_t lanes) { return workgroups > 0xffffffffll / lanes; }
 inline int64_t size_of(int64_t type) { return type == PPN_T_F32 ? 4 : 2; }
 inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p) % (uint64_t)bytes == 0; }
 

@@ -816,7 +816,8 @@ extern "C" int ppn_scan_forward(const ppn_scan_args* a, void* stream) {
   const Split s = forward_split(a);
   if (a->workspace_bytes < ppn_scan_forward_workspace(a) || (s.chunks > 1 && !a->workspace)) return fail(PPN_E_INVALID, "ppn_scan_forward: the workspace is too small");
   const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels;
-  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff) return fail(PPN_E_INVALID, "scan: too many channels of too many environments");
+  if (too_many(waves, 64) || (s.chunks > FEW_CHUNKS && too_many(ceil_div(cells, 64), 64)))
+    return fail(PPN_E_INVALID, "scan: too many channels of too many environments");
   const dim3 grid(waves, s.chunks);
   float* ends = (float*)a->workspace;
   float* sums = ends + cells * s.chunks;
@@ -857,7 +858,9 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
   float* ends = (float*)(w + p.rows_bytes + p.params_bytes);
   float* sums = (float*)(w + p.rows_bytes + p.params_bytes + p.ends_bytes);
   const int64_t waves = a->batch * a->groups * tiles_of(a), cells = a->batch * a->states * a->channels, count = a->batch * a->time * a->groups * 2 * states_of(a);
-  if (waves > 0x7fffffff || ceil_div(cells, 64) > 0x7fffffff || ceil_div(count, 1024) > 0x70000000) return fail(PPN_E_INVALID, "scan: too many rows");
+  const int64_t row_blocks = ceil_div(count, 1024), blocks = row_blocks + ceil_div((a->states + 2) * a->channels, 32);
+  if (too_many(waves, 64) || (p.split.chunks > FEW_CHUNKS && too_many(ceil_div(cells, 64), 64)) || too_many(blocks, 256))
+    return fail(PPN_E_INVALID, "scan: too many rows");
   const dim3 grid(waves, p.split.chunks);
   return by_type(a->type, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
@@ -872,10 +875,9 @@ extern "C" int ppn_scan_backward(const ppn_scan_args* a, void* stream) {
         scan_backward<T, NS, LPC, JOINING><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, nullptr, ends, sums, rows, params);
       else
         scan_backward<T, NS, LPC, GRADIENTS><<<grid, dim3(64), 0, (hipStream_t)stream>>>(*a, p.split.chunk, p.split.chunks, joined, nullptr, nullptr, rows, params);
-      const int64_t row_blocks = ceil_div(count, 1024);
       const ReduceArgs r = {rows, tiles_of(a), a->batch * a->time * a->groups, params, a->batch * p.split.chunks, a->states, a->channels, a->dB, a->dC, a->dA, a->dD,
                             a->ddt_bias, row_blocks};
-      scan_reduce<T, NS * LPC><<<dim3(row_blocks + ceil_div((a->states + 2) * a->channels, 32)), dim3(256), 0, (hipStream_t)stream>>>(r);
+      scan_reduce<T, NS * LPC><<<dim3(blocks), dim3(256), 0, (hipStream_t)stream>>>(r);
       return launched("ppn_scan_backward");
     });
   });
@@ -890,6 +892,7 @@ extern "C" int ppn_scan_step(const ppn_scan_step_args* a, void* stream) {
   if (a->env_ids && a->rows > MOST_IDS) return fail(PPN_E_INVALID, "ppn_scan_step: at most %d rows with env_ids", MOST_IDS);
   if (a->rows == 0) return PPN_OK;
   if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || !a->state || !a->environments) return fail(PPN_E_INVALID, "ppn_scan_step: x, dt, A, B, C, state (of one environment at least) and y are needed");
+  if (too_many(a->rows, 256)) return fail(PPN_E_INVALID, "ppn_scan_step: too many rows");
   const int64_t four = 4 * size_of(a->type);
   const bool wide = a->states % 4 == 0 && aligned(a->state, 16) && aligned(a->A, 16) && aligned(a->B, four) && aligned(a->C, four) && a->B_row % 4 == 0 &&
                     a->C_row % 4 == 0 && a->B_group % 4 == 0 && a->C_group % 4 == 0;

@@ -1136,3 +1136,27 @@ def test_gpu_selective_scan_chunks_that_grow(t):
     got = torch.autograd.grad(y, [own[k] for k in names], up.cuda())
     for k, p, q in zip(names, got, want):
         close('d' + k, p, q, torch.float32, 2 * (8 * 12 + n + 32), 8 * float(want[0].abs().max()) + float(q.abs().max()))
+
+
+def test_entry_points_refuse_what_no_launch_can_hold():
+    """2^32 lanes along an axis, before anything is launched: the pointers here are none."""
+    from pypownet_amd import _lib
+    lib = _lib.load_library()
+    step = dict(rows=1 << 24, environments=1 << 24, channels=4, x=16, y=16, state=16)
+    assert lib.ppn_conv_step(packed_args('ppn_conv_step_args', taps=4, weight=16, **step), None) == -1 and b'rows' in lib.ppn_policy_error()
+    assert lib.ppn_scan_step(packed_args('ppn_scan_step_args', groups=1, states=4, dt=16, A=16, B=16, C=16, **step), None) == -1 and b'rows' in lib.ppn_policy_error()
+    conv = dict(batch=1 << 26, time=1, channels=1, taps=2, x=16, weight=16, y=16)
+    assert lib.ppn_conv_forward(packed_args('ppn_conv_args', **conv), None) == -1 and b'environments' in lib.ppn_policy_error()
+    scan = dict(channels=1, groups=1, states=1, x=16, dt=16, A=16, B=16, C=16, y=16, dy=16, dx=16, ddt=16, dB=16, dC=16, checkpoints=16, workspace=256, workspace_bytes=1 << 62)
+    for sizes in (dict(batch=1 << 26, time=1), dict(batch=1 << 15, time=1 << 15)):
+        if sizes['time'] == 1:
+            assert lib.ppn_scan_forward(packed_args('ppn_scan_args', **scan, **sizes), None) == -1 and b'environments' in lib.ppn_policy_error()
+        assert lib.ppn_scan_backward(packed_args('ppn_scan_args', **scan, **sizes), None) == -1 and b'rows' in lib.ppn_policy_error()
+    loss = dict(hidden=16, weight=16, target=16, loss=16, lse=16, dloss=16, dhidden=16, dweight=16, workspace=256, workspace_bytes=1 << 62)
+    for rows, actions, features, backward in ((1 << 22, 1 << 18, 8, False), (1, 1 << 23, 1023, True), (1 << 22, 1 << 10, 1 << 14, True)):
+        args = packed_args('ppn_loss_args', rows=rows, actions=actions, features=features, hidden_row=features, weight_row=features, **loss)
+        calls = [lib.ppn_loss_backward] if backward else []
+        if actions != 1 << 10:
+            calls.append(lib.ppn_loss_forward)
+        for call in calls:
+            assert call(args, None) == -1 and b'too many rows' in lib.ppn_policy_error(), (rows, actions, features)
