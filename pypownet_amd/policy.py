@@ -192,7 +192,7 @@ class RecurrentPolicy(torch.nn.Module):
         [batch, time, words] as ``policy_ops.pack_allowed`` makes them.  Returns (loss, memory behind the window)."""
         b, t = observations.shape[:2]
         hidden, after = self.window(observations, starts, memory)
-        bits = None if allowed is None else allowed.reshape(b * t, -1)
+        bits = None if allowed is None else allowed.reshape(b * t, allowed.shape[-1])
         return ops.action_cross_entropy(hidden.reshape(b * t, self.features), self.head.to(self.dtype), actions.reshape(b * t), bits).view(b, t), after
 
     @torch.no_grad()

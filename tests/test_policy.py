@@ -300,3 +300,20 @@ def test_gpu_acting_between_a_loss_and_its_backward_pass(dtype):
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(again.mean(), list(policy.parameters())), want))
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         shared.mean().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('b,t', [(0, 5), (3, 0)])
+def test_gpu_policy_loss_of_no_rows(b, t):
+    c = ActionCatalogue(load_env('default14')[0])
+    policy = RecurrentPolicy(c, 538, features=16, layers=1).cuda()
+    words = (len(c) + 31) // 32
+    memory = policy.memory(b)
+    if b:
+        policy.act(torch.randn((b, 538), device='cuda'), memory)
+    kept = [m.clone() for m in memory.windows + memory.states]
+    loss, after = policy.loss(torch.zeros((b, t, 538), device='cuda'), torch.zeros((b, t), dtype=torch.int64, device='cuda'),
+                              torch.zeros((b, t, words), dtype=torch.int32, device='cuda'), torch.zeros((b, t), dtype=torch.bool, device='cuda'), memory)
+    assert loss.shape == (b, t) and all(torch.equal(m, k) for m, k in zip(after.windows + after.states, kept))
+    loss.sum().backward()
+    assert all(p.grad is not None and not p.grad.any() for p in policy.parameters())
