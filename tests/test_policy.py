@@ -317,3 +317,28 @@ def test_gpu_policy_loss_of_no_rows(b, t):
     assert loss.shape == (b, t) and all(torch.equal(m, k) for m, k in zip(after.windows + after.states, kept))
     loss.sum().backward()
     assert all(p.grad is not None and not p.grad.any() for p in policy.parameters())
+
+
+@pytest.mark.gpu
+def test_gpu_the_memory_behind_imitate_is_that_of_the_rows_played(monkeypatch):
+    import copy
+    env = environments(20, 'default30')
+    c = ActionCatalogue(env.case)
+    torch.manual_seed(11)
+    policy = RecurrentPolicy(c, env.engine.observation_length(), features=32).cuda()
+    memory = policy.memory(20)
+    optimizer = torch.optim.SGD(policy.parameters(), lr=1e-2)
+    seen, rows = [], env.policy_rows
+
+    def recording(*args, **kw):
+        seen.append(rows(*args, **kw))
+        return seen[-1]
+    monkeypatch.setattr(env, 'policy_rows', recording)
+    for _ in range(2):
+        seen.clear()
+        before, old = copy.deepcopy(policy), PolicyMemory([w.clone() for w in memory.windows], [s.clone() for s in memory.states])
+        imitate(env, policy, optimizer, memory, steps=7, candidates=3)
+        assert len(seen) == 7
+        _, after = before.window(torch.stack([o for o, _, _ in seen], dim=1), torch.stack([s for _, s, _ in seen], dim=1), old)
+        for mine, want, had in zip(memory.windows + memory.states, after.windows + after.states, old.windows + old.states):
+            assert torch.equal(mine, want) and not torch.equal(mine, had)

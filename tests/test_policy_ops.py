@@ -1160,3 +1160,18 @@ def test_entry_points_refuse_what_no_launch_can_hold():
             calls.append(lib.ppn_loss_forward)
         for call in calls:
             assert call(args, None) == -1 and b'too many rows' in lib.ppn_policy_error(), (rows, actions, features)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('d,k,silu', [(1, 2, True), (24, 4, True), (250, 3, False), (1032, 8, True), (256, 4, True), (512, 5, False)])
+def test_gpu_short_conv_step_is_the_window_bit_for_bit(d, k, silu, dtype):
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(46)
+    b, t = 3, 9
+    x, weight, bias = rand(gen, b, t, d, dtype=dtype).cuda(), rand(gen, d, k).cuda(), rand(gen, d).cuda()
+    starts, state = (torch.rand((b, t), generator=gen) < 0.2).cuda(), rand(gen, b, k - 1, d, dtype=dtype).cuda()
+    activation = 'silu' if silu else None
+    y = ops.short_conv(x, weight, bias, activation=activation, starts=starts, initial_state=state)
+    for i in range(t):
+        assert torch.equal(ops.short_conv_step(x[:, i], state, weight, bias, activation=activation, starts=starts[:, i]), y[:, i]), i
