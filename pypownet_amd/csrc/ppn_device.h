@@ -100,7 +100,7 @@ __device__ __forceinline__ int ppn_opaque_uniform(int x) { __asm__ volatile("" :
 // One wavefront plays one environment and every decision between phases is the same in all 64 lanes.  At the head of such a loop --
 // never inside a LANE_LOOP or under a per-lane condition -- the statement is a side-effecting, convergent instruction that all 64
 // lanes execute together.  What it prevents (tools/ubench/README_gpu_only_failures.md, "Round 6: the root cause of (iii)";
-// tools/ubench/convergent_threading_repro.hip is the same thing in twenty lines):
+// tools/ubench/convergent_threading_repro.hip is the remedy in twenty lines):
 //   a work loop that ENDS with `if (lane == 0) publish(...)` and BEGINS with `if (lane == 0) item = atomicAdd(...);
 //   item = readfirstlane(item);` has, per thread, two branches on the same condition in a row across the back edge.  LLVM's SimplifyCFG
 //   threads them: lanes 1..63 jump from the tail straight to the block that holds readfirstlane (their `item` is the constant 0), lane
@@ -110,22 +110,14 @@ __device__ __forceinline__ int ppn_opaque_uniform(int x) { __asm__ volatile("" :
 //   wave-uniform values (the chronic slot and row: the address fault rocgdb caught, EXEC = 0xfffffffffffffffe).
 // With a side-effecting statement in the loop header there is no empty block to thread through, the loop has ONE back edge, and the
 // wave reconverges there by construction.  Any such statement does it (an empty `asm volatile`, `__builtin_amdgcn_wave_barrier()`,
-// this one: all three verified on the engine kernel and on the reproducer); this form also re-arms EXEC and fences memory for the
+// this one: all three verified); this form also re-arms EXEC and fences memory for the
 // compiler, one scalar instruction where the phase boundary is a compiler fence anyway.
 // Rule for this code base: a loop whose iterations begin or end with lane-0-only code carries PPN_WAVE_FULL at its head (work loops
 // of the persistent / rollout / server kernels, episode loop, cascade loop, around every solve, Newton and fast-decoupled loops).
 // (The two older GPU-only incidents -- round 2: line-end tables inside the matrix region; round 3: B'/B'' assembly -- behaved
 //  differently (no lane missing at the loop heads, -O3 only) and are NOT explained by this; see the README.)
 // -DPPN_EXEC_CHECK additionally records (bit `id` of the environment's prof[31], count in prof[30]) lanes found missing there.
-#if defined(PPN_WAVE_FULL_OFF)      // (the kernels as they were written until round 5: for the reproducer only)
-#define PPN_WAVE_FULL(prof_, id) ((void)0)
-#elif defined(PPN_WAVE_FULL_BARRIER_ONLY)      // (reproducer: the compiler fence without the EXEC write)
-#define PPN_WAVE_FULL(prof_, id) __asm__ volatile("" ::: "memory")
-#elif defined(PPN_WAVE_FULL_EXEC_ONLY)         // (reproducer: the EXEC write without the compiler fence)
-#define PPN_WAVE_FULL(prof_, id) __asm__ volatile("s_mov_b64 exec, -1")
-#elif defined(PPN_WAVE_FULL_WAVE_BARRIER)      // (reproducer: the compiler's own convergent no-op)
-#define PPN_WAVE_FULL(prof_, id) __builtin_amdgcn_wave_barrier()
-#elif defined(PPN_EXEC_CHECK)      // (= 2: inside the step body -- ids 4 and up -- lanes found parked are recorded but NOT switched on: where does it start?)
+#if defined(PPN_EXEC_CHECK)      // (= 2: inside the step body -- ids 4 and up -- lanes found parked are recorded but NOT switched on: where does it start?)
 #define PPN_WAVE_FULL(prof_, id) do { const u64 ex_ = __builtin_amdgcn_read_exec(); \
     if (PPN_EXEC_CHECK != 2 || (id) < 4) __asm__ volatile("s_mov_b64 exec, -1" ::: "memory"); \
     if (ex_ != ~0ull && (prof_) != nullptr && (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) == __builtin_ctzll(ex_)) { (prof_)[31] |= 1ll << (id); (prof_)[30] += 1; } } while (0)

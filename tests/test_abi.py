@@ -126,6 +126,23 @@ def test_wave_full_statement_keeps_the_work_loop_in_one_piece():
     assert atomics(1) == (2, 1)      # (__builtin_amdgcn_wave_barrier(): the same protection)
 
 
+def test_the_work_loop_without_a_remedy_is_not_built():
+    """Its kernel does not end by itself: no build makes it, and one that is left from an earlier build is removed."""
+    import subprocess
+    import __graft_entry__ as g
+    hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
+    if not os.path.exists(hipcc):
+        pytest.skip('no hipcc')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src, left = os.path.join(root, 'tools', 'ubench', 'convergent_threading_repro.hip'), os.path.join(root, 'build', 'convergent_threading_repro_fix0')
+    refused = subprocess.run([hipcc, '--offload-arch=gfx950', '-fsyntax-only', '-DFIX=0', src], capture_output=True, text=True, timeout=300)
+    assert refused.returncode != 0 and 'FIX must be' in refused.stderr
+    os.makedirs(os.path.dirname(left), exist_ok=True)
+    open(left, 'w').close()
+    g.build_guards()
+    assert not os.path.exists(left) and os.path.exists(left[:-1] + '3')
+
+
 def test_kernels_ir_has_no_lane_dependent_cycle_around_a_convergent_operation():
     """tools/dev/ir_lint_convergent.py over the optimised IR of all six kernel translation units (hipcc -emit-llvm, ~30 s in
     parallel): no cycle that holds a convergent operation (readfirstlane, readlane, barriers, DPP ...) may be left or re-entered on a

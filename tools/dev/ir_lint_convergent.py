@@ -7,7 +7,7 @@ be left and re-entered by all 64 lanes together; `simplifycfg` broke exactly tha
 `if (lane == 0)` at the loop's tail into `if (lane == 0)` at its head.
 
     python tools/dev/ir_lint_convergent.py file.ll [file.ll ...]          # IR from hipcc -O3 --cuda-device-only -emit-llvm -S
-    python tools/dev/ir_lint_convergent.py --build [--flags -DPPN_WAVE_FULL_OFF]      # emits the IR of the six kernel translation units first
+    python tools/dev/ir_lint_convergent.py --build [--flags ...]      # emits the IR of the six kernel translation units first
 
 Divergence is approximated by a taint: the lane index (mbcnt, workitem.id), results of atomics, loads through tainted addresses,
 and everything computed from them; readfirstlane / readlane / ballot results are uniform; a phi is tainted if an incoming value is,
