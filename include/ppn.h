@@ -577,6 +577,8 @@ int ppn_scan_step(const ppn_scan_step_args* a, void* stream);
  * allowed: bit v & 31 of word v >> 5 of row i (NULL: every action; allowed_row 0: one row for all).  target = ignore_index, or a row with nothing
  * allowed: loss 0, no gradient.  A target that is not allowed: loss +inf.  A target outside 0..actions-1, or no
  * allowed logit above -inf: loss NaN, and so its gradients.  lse (log of the sum; saved for the backward pass): +inf where the row has no gradient.
+ * The backward workspace holds copies of hidden and weight, and twice 256 MB or 1024 actions x rows of the type, whichever is more, and
+ * up to 128 MB or one 32-bit dhidden and dweight.
  * Backward: loss and lse as the forward pass left them and dloss[rows] in; dhidden [rows x features], dweight [actions x features] (each or NULL) out, contiguous. */
 typedef struct ppn_loss_args {
   int64_t struct_bytes, type, rows, actions, features, ignore_index;

@@ -8,7 +8,8 @@
 //   logits -> running maximum and sum of exponentials per row and tile (nothing else leaves the chip),
 //   logits -> dl of a piece of the catalogue, rounded to the operands' type and laid out both ways (dl and its transpose),
 //   dl and dl^T against transposed copies of weight and hidden -> the two gradients.
-// The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size.
+// The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size: 256 MB and as much for its transpose, or
+// 1024 actions' worth where the rows make that more.
 //
 // 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 470 us (860 TFLOP/s), the second 790 us (510; it
 // writes 1.6 GB, and the transposed copies), the third 935 us for both (870).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
@@ -694,7 +695,8 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   p.features_padded = padded(a->features, part(a));
   p.rows_padded = padded(a->rows, 64);
   p.actions_padded = padded(a->actions, 64);
-  // A piece's dl and its transpose take 256 MB each.  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
+  // A piece's dl and its transpose take 256 MB each, or 1024 actions times the rows where that is more (above 131072 rows in 16 bits, 65536 in 32: the
+  // rows are not taken in pieces).  The smaller the piece, the shorter the inner dimension of dhidden's product and the fewer tiles
   // of dweight's: 16384 rows of 24129 actions took 3.65, 3.02, 2.71 and 2.44 ms behind the loss at 32, 64, 128 and 256 MB; with both products in a
   // launch 256, 512 and 1024 MB are within 2 % of each other.
   p.piece = padded((int64_t)(256 << 20) / (p.rows_padded * size), 128);

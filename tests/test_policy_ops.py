@@ -1175,3 +1175,22 @@ def test_gpu_short_conv_step_is_the_window_bit_for_bit(d, k, silu, dtype):
     y = ops.short_conv(x, weight, bias, activation=activation, starts=starts, initial_state=state)
     for i in range(t):
         assert torch.equal(ops.short_conv_step(x[:, i], state, weight, bias, activation=activation, starts=starts[:, i]), y[:, i]), i
+
+
+@pytest.mark.parametrize('kind,size', [(0, 4), (1, 2), (2, 2)])
+def test_the_loss_workspace_stays_within_what_is_said(kind, size):
+    """Backward: copies of both operands (twice where their rows are not whole 16 bytes), dl and its transpose, 32-bit sums."""
+    from pypownet_amd import _lib
+    lib = _lib.load_library()
+    for rows in (1, 63, 256, 4096, 16384, 20480, 61440, 131072, 245760, 1 << 22):
+        for actions in (1, 347, 12099, 24129, 1 << 20):
+            for features in (24, 64, 250, 512, 4096):
+                args = packed_args('ppn_loss_args', type=kind, rows=rows, actions=actions, features=features, hidden=16, weight=16, hidden_row=features,
+                                   weight_row=features)
+                up = lambda v, to: -(-v // to) * to      # noqa: E731
+                operands = (up(rows, 64) + up(actions, 64)) * up(features, 8) * size * 2
+                # (a piece is a multiple of 128 actions, so up to 127 more rows of the transpose)
+                dl = 2 * max((256 << 20) + 128 * up(rows, 64) * size, 1024 * up(rows, 64) * size)
+                piece = min(up(actions, 64), max(1024, up((256 << 20) // (up(rows, 64) * size), 128)))
+                sums = max(128 << 20, 4 * (rows + piece) * features)
+                assert 0 < lib.ppn_loss_backward_workspace(args) <= operands + dl + sums + 4096, (rows, actions, features)
