@@ -383,7 +383,9 @@ int check(const ppn_conv_args* a) {
 }
 
 // Four channels a lane (16 bytes, or 8 of the 16-bit types: eight channels' weights, sums and rows would leave half the waves) where they fill a wave
-// and every row of every tensor begins on such a border; else one.
+// and every row of every tensor begins on such a border; else one.  A wave of fewer channels does some of them twice.  One against four channels a lane,
+// forward and training step of 63 million elements in bfloat16, in us: 53 and 111, 195 and 394 at 64 channels; 48 and 59, 193 and 218 at 128; 61 and
+// 47, 245 and 176 at 192 (left to one, as 32 bits is even: 102 and 102, 277 and 269).  In 32 bits at 128 channels: 111 and 110, 299 and 283.
 constexpr int WIDE = 4;
 bool wide(const ppn_conv_args* a, bool backward) {
   const int64_t vec = WIDE, bytes = WIDE * size_of(a->type);

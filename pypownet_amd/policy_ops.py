@@ -434,7 +434,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 
     ``initial_state [batch, channels, states]`` float32, zeros when None; h is zero in front of a row marked in ``starts [batch, time]``.  Returns y, or
     ``(y, final_state)``, the next window's ``initial_state`` and ``selective_scan_step``'s state.  Differentiable in every tensor but ``starts``; sums
-    run in a fixed order, so gradients repeat bit for bit.  A differentiable call keeps the states in front of every 8th row for the backward pass."""
+    run in a fixed order, so gradients repeat bit for bit.  A differentiable call keeps the states in front of every 8th row for the backward pass.
+    Rows of time may lie at most 2^27 elements apart in memory.  Where an input is infinite, what depends on it is infinite or NaN."""
     _leading('x', x)
     b, t, d = shape = _window_rows(x)
     dtype, device = x.dtype, x.device
@@ -557,7 +558,11 @@ def action_cross_entropy(hidden, weight, target, allowed=None, ignore_index=-100
     and no gradient; a target that is not allowed has loss +inf (its gradient is that of the logarithm alone); a target outside 0 .. actions - 1 gives
     NaN, and so does a row whose allowed logits are all -inf.  What a row does not allow is not looked at (behind the loss, a weight row that is not finite still makes NaN of dhidden).  ``-loss`` is the
     log-probability of the action ``target``.  Differentiable in hidden and weight (the result is kept for that: not to be changed in place); sums
-    run in a fixed order."""
+    run in a fixed order.  The gradients are products of 16-bit operands where the tensors are 16-bit: the logits' gradient is rounded to that type in
+    between (half a step of each entry, about as much again as the results' own rounding; in float16 entries below 2^-28 of
+    the largest upstream gradient lose digits).
+
+    Workspace behind the loss: about 0.5 GB, or 2 x 1024 x rows elements where that is more."""
     _leading('hidden', hidden)
     if hidden.dim() != 2 or hidden.shape[1] == 0:
         raise ValueError('hidden must be [rows, features], got %s' % list(hidden.shape))
