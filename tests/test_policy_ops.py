@@ -1194,3 +1194,40 @@ def test_the_loss_workspace_stays_within_what_is_said(kind, size):
                 piece = min(up(actions, 64), max(1024, up((256 << 20) // (up(rows, 64) * size), 128)))
                 sums = max(128 << 20, 4 * (rows + piece) * features)
                 assert 0 < lib.ppn_loss_backward_workspace(args) <= operands + dl + sums + 4096, (rows, actions, features)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_action_cross_entropy_of_many_rows(dtype):
+    """A window of thousands of environments: pieces of the catalogue at their smallest, the inner dimension of dweight's product at its longest."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(47)
+    n, v, f = 140003, 1100, 24
+    hidden, weight = rand(gen, n, f, dtype=dtype).cuda(), rand(gen, v, f, scale=0.3, dtype=dtype).cuda()
+    target, dloss = torch.randint(0, v, (n,), generator=gen).cuda(), rand(gen, n).cuda()
+    own = [hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)]
+    loss = ops.action_cross_entropy(own[0], own[1], target)
+    grads = torch.autograd.grad(loss, own, dloss)
+    h, w, g = hidden.double(), weight.double(), dloss.double()[:, None]
+    size = max(float((h[i:i + 20000].abs() @ w.abs().t()).max()) for i in range(0, n, 20000))
+    slack_w, total_w, want_w = (torch.zeros((v, f), dtype=torch.float64, device='cuda') for _ in range(3))
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    probability = 2 * (f + 32) * STEP * (size + 16)      # (limits as in test_gpu_action_cross_entropy_in_pieces)
+    for i in range(0, n, 20000):
+        rows = slice(i, min(n, i + 20000))
+        logits = h[rows] @ w.t()
+        p, at = torch.softmax(logits, 1), torch.arange(logits.shape[0], device='cuda')
+        close('loss', loss[rows], (torch.logsumexp(logits, 1) - logits[at, target[rows]]).cpu(), torch.float32, f + 64, size + 16)
+        p[at, target[rows]] -= 1
+        dl = p * g[rows]
+        each = (half(dtype) + probability) * dl.abs() + probability * g[rows].abs() * (p < 0)
+        if dtype == torch.float16:
+            each = each + float(dloss.abs().max()) * 2.0 ** -38
+        want = dl @ w
+        limit = each @ w.abs() + half(dtype) * want.abs() * 1.01 + 2 * (v + 8) * STEP * (dl.abs() @ w.abs()) + tiny
+        assert ((grads[0][rows].double() - want).abs() <= limit).all()
+        slack_w += each.t().contiguous() @ h[rows].abs()
+        total_w += dl.abs().t().contiguous() @ h[rows].abs()
+        want_w += dl.t().contiguous() @ h[rows]
+    limit = slack_w + half(dtype) * want_w.abs() * 1.01 + 2 * (n + 8) * STEP * total_w + tiny
+    assert ((grads[1].double() - want_w).abs() <= limit).all()
