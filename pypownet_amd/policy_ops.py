@@ -542,9 +542,10 @@ class _ActionCrossEntropy(torch.autograd.Function):
         dweight = weight.new_empty(weight.shape) if ctx.needs_input_grad[1] else None
         if hidden.shape[0] == 0:
             return dhidden, None if dweight is None else dweight.zero_(), None, None, None
+        dloss = dloss.contiguous()      # (a name of its own: the copy that sum() and mean() make needed has to outlive the launches)
         lib = _load()
         _with_workspace(lib.ppn_loss_backward_workspace, lib.ppn_loss_backward,
-                        _loss_args(hidden, weight, target, allowed, ctx.ignore, loss, lse, dloss.contiguous(), dhidden, dweight), hidden.device)
+                        _loss_args(hidden, weight, target, allowed, ctx.ignore, loss, lse, dloss, dhidden, dweight), hidden.device)
         return dhidden, dweight, None, None, None
 
 

@@ -1231,3 +1231,56 @@ def test_gpu_action_cross_entropy_of_many_rows(dtype):
         want_w += dl.t().contiguous() @ h[rows]
     limit = slack_w + half(dtype) * want_w.abs() * 1.01 + 2 * (n + 8) * STEP * total_w + tiny
     assert ((grads[1].double() - want_w).abs() <= limit).all()
+
+
+def _one_free_block():
+    """Small tensors in every free place of torch's small memory but one segment: what is allocated and freed there next is what is allocated behind it."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    kept, reserved = [], torch.cuda.memory_reserved()
+    while torch.cuda.memory_reserved() == reserved:
+        kept.append(torch.empty((512,), dtype=torch.uint8, device='cuda'))
+    kept.pop()
+    return kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('n,v,f', [(7, 40, 25), (300, 177, 65), (2000, 347, 64)])
+def test_gpu_upstream_gradients_that_are_no_memory_of_their_own(n, v, f, dtype):
+    """sum() and mean() hand back one number expanded over the rows, a slice of a larger gradient has strides: the copy that is made of it lives as long as
+    the kernels that read it are queued."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(49)
+    h, w = rand(gen, n, f, dtype=dtype).cuda().requires_grad_(True), rand(gen, v, f, scale=0.3, dtype=dtype).cuda().requires_grad_(True)
+    target, wide_up = torch.randint(0, v, (n,), generator=gen).cuda(), rand(gen, n, 3).cuda()
+    x, weight = rand(gen, 3, n, 24, dtype=dtype).cuda().requires_grad_(True), rand(gen, 24, 4).cuda().requires_grad_(True)
+    state, A = rand(gen, 3, 24, 8).cuda().requires_grad_(True), (-torch.rand((24, 8), generator=gen) - 0.1).cuda().requires_grad_(True)
+    bc = rand(gen, 3, n, 1, 8, dtype=dtype).cuda().requires_grad_(True)
+
+    def conv():
+        return ops.short_conv(x, weight, activation='silu', initial_state=x[:, :3], return_final_state=True)
+
+    def scan():
+        return ops.selective_scan(x, x, A, bc, bc, dt_softplus=True, initial_state=state, return_final_state=True)
+    loss = lambda: (ops.action_cross_entropy(h, w, target),)      # noqa: E731
+    one = torch.ones((), device='cuda')
+    for call, leaves in ((loss, [h, w]), (conv, [x, weight]), (scan, [x, A, bc, state])):
+        for k in range(3):
+            outs = call()
+            ups = [one.to(o.dtype).expand_as(o) if k < 2 else wide_up[:, 1] if o.dim() == 1 else rand(gen, *o.shape[::-1], dtype=o.dtype).cuda().permute(2, 1, 0) for o in outs]
+            kept = [u.contiguous().clone() for u in ups]
+            want = torch.autograd.grad(outs, leaves, kept)
+            del outs
+            outs = call()
+            full = _one_free_block() if k == 1 else None
+            got = torch.autograd.grad(outs, leaves, ups)
+            del full, outs
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), (call, k)
+    for reduce, up in ((lambda y: y.sum(), torch.ones((n,), device='cuda')), (lambda y: y.mean(), torch.full((n,), 1.0, device='cuda') / n)):
+        want = torch.autograd.grad(loss()[0], [h, w], up)
+        reduced = reduce(loss()[0])
+        full = _one_free_block()
+        got = torch.autograd.grad(reduced, [h, w])
+        del full
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
