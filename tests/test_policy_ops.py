@@ -1284,3 +1284,95 @@ def test_gpu_upstream_gradients_that_are_no_memory_of_their_own(n, v, f, dtype):
         got = torch.autograd.grad(reduced, [h, w])
         del full
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def _far(t, stride):
+    """The same values with what lies along the first axis `stride` elements apart."""
+    far = torch.empty(((t.shape[0] - 1) * stride + t[0].numel(),), dtype=t.dtype, device='cuda').as_strided(t.shape, (stride, *t[0].contiguous().stride()))
+    return far.copy_(t)
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    """Environments, rows and states more than 2^32 bytes apart in memory are the same as close together."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(48)
+    dtype, apart = torch.bfloat16, (1 << 31) + 64
+    b, t, d, n = 3, 13, 256, 16
+    v = dict(x=rand(gen, b, t, d, dtype=dtype), dt=rand(gen, b, t, d, dtype=dtype), B=rand(gen, b, t, 1, n, dtype=dtype), C=rand(gen, b, t, 1, n, dtype=dtype))
+    w, A, up, starts = rand(gen, d, 4).cuda(), -torch.rand((d, n), generator=gen).cuda() - 0.1, rand(gen, b, t, d, dtype=dtype), torch.rand((b, t), generator=gen) < 0.1
+    close_by, far = [{k: put(q.cuda()) for k, q in v.items()} for put in (lambda q: q.clone(), lambda q: _far(q, apart))]
+    up, starts = [up.cuda(), _far(up.cuda(), apart)], [starts.cuda(), _far(starts.cuda(), 1 << 32)]
+    results = []
+    for u, s, up_, starts_ in ((close_by, 0, *(q[0] for q in (up, starts))), (far, 1, *(q[1] for q in (up, starts)))):
+        for q in u.values():
+            q.requires_grad_(True)
+        y = ops.short_conv(u['x'], w, activation='silu', starts=starts_)
+        h = ops.selective_scan(u['x'], u['dt'], A, u['B'], u['C'], dt_softplus=True, starts=starts_)
+        results.append([y, h, *torch.autograd.grad(y, u['x'], up_), *torch.autograd.grad(h, list(u.values()), up_)])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+    del far, up, starts, results, u, up_, starts_, y, h
+    # one row of environments far into a state
+    environments = (1 << 32) // (d * n * 4) + 3
+    state, window = torch.zeros((environments, d, n), device='cuda'), torch.zeros(((1 << 32) // (3 * d * 2) + 3, 3, d), dtype=dtype, device='cuda')
+    rows = [v[k][:2, 0].cuda() for k in ('x', 'dt', 'B', 'C')]
+    for big, call in ((state, lambda s, ids: ops.selective_scan_step(*rows[:2], A, *rows[2:], s, dt_softplus=True, env_ids=ids)),
+                      (window, lambda s, ids: ops.short_conv_step(rows[0], s, w, env_ids=ids))):
+        last = big.shape[0] - 1
+        big[last] = rand(gen, *big.shape[1:], dtype=big.dtype).cuda()
+        small = big[[0, last]].contiguous()
+        assert torch.equal(call(big, torch.tensor([0, last], device='cuda')), call(small, None)) and torch.equal(big[[0, last]], small)
+        assert not big[1:last].any()
+    del state, window, big
+    rows, actions, f = 300, 177, 64
+    h, weight, target = rand(gen, rows, f, dtype=dtype).cuda(), rand(gen, actions, f, dtype=dtype).cuda(), torch.randint(0, actions, (rows,), generator=gen).cuda()
+    bits = ops.pack_allowed(torch.ones((rows, actions), dtype=torch.bool, device='cuda'))
+    results = []
+    for hh, ww, bb in ((h.clone(), weight.clone(), bits), (_far(h, 1 << 23), _far(weight, 1 << 23), _far(bits, 1 << 23)), (_far(h, (1 << 23) + 8), _far(weight, (1 << 23) + 8), bits)):
+        hh.requires_grad_(True), ww.requires_grad_(True)
+        loss = ops.action_cross_entropy(hh, ww, target, allowed=bb)
+        results.append([loss, *torch.autograd.grad(loss.sum(), [hh, ww])])
+        del hh, ww, bb
+    assert all(torch.equal(p, q) for p, q in zip(results[0], results[1])) and all(torch.equal(p, q) for p, q in zip(results[0], results[2]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gpu_results_do_not_depend_on_what_memory_held(dtype):
+    """Outputs, workspaces and checkpoints out of memory full of zeros, of NaN and of large numbers: the same bits."""
+    from pypownet_amd import policy_ops as ops
+    gen = torch.Generator().manual_seed(50)
+
+    def fill(byte):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        kept = [torch.full((1 << k,), byte, dtype=torch.uint8, device='cuda') for k in (9, 12, 14, 16, 17, 18, 19, 20, 21, 22, 23, 24, 26) for _ in range(8)]
+        del kept
+    calls = []
+    for b, t, d, k in ((3, 67, 20, 3), (2, 17, 520, 4), (5, 40, 136, 5)):
+        x, w, up = (q.cuda().requires_grad_(True) for q in (rand(gen, b, t, d, dtype=dtype), rand(gen, d, k), rand(gen, b, t, d, dtype=dtype)))
+        starts = (torch.rand((b, t), generator=gen) < 0.1).cuda()
+        calls.append((lambda x, w, s=starts: ops.short_conv(x, w, activation='silu', starts=s), [x, w], up))
+    for case in (SCAN[2], SCAN[3], SCAN[8], SCAN[10]):
+        v, starts, dy, _ = scan_inputs(case, dtype)
+        names = [k for k in ORDER if v[k] is not None]
+        leaves = [v[k].cuda().requires_grad_(True) for k in names]
+
+        def scan(*leaves, names=names, soft=case[8], starts=None if starts is None else starts.cuda()):
+            return own_scan({**dict.fromkeys(ORDER), **dict(zip(names, leaves))}, soft, starts)[0]
+        calls.append((scan, leaves, dy.cuda()))
+    for n, actions, f in ((65, 40, 25), (300, 177, 64), (700, 1100, 72)):
+        h, w, up = (q.cuda().requires_grad_(True) for q in (rand(gen, n, f, dtype=dtype), rand(gen, actions, f, scale=0.3, dtype=dtype), rand(gen, n)))
+        target = torch.randint(0, actions, (n,), generator=gen)
+        mask = torch.rand((n, actions), generator=gen) < 0.7
+        mask[torch.arange(n), target] = True
+        calls.append((lambda h, w, t=target.cuda(), m=ops.pack_allowed(mask.cuda()): ops.action_cross_entropy(h, w, t, allowed=m), [h, w], up))
+    for call, leaves, up in calls:
+        results = []
+        for byte in (0, 0xff, 0x41):
+            fill(byte)
+            y = call(*leaves)
+            fill(byte)
+            results.append([y.detach(), *torch.autograd.grad(y, leaves, up.detach())])
+        assert torch.isfinite(results[0][0]).all()
+        assert all(torch.equal(p, q) for other in results[1:] for p, q in zip(results[0], other))
