@@ -3,8 +3,8 @@
 // All three are bound by memory: 2 * taps multiply-adds per element against two elements moved (five in a training step).
 // A lane owns four neighbouring channels (one where rows are not aligned for that) and walks a stretch of time with the taps - 1 rows
 // before it in registers, so every row is read once; neighbouring lanes read neighbouring channels, a wave 512 B or 1 KB at a time.  A row marked in
-// `starts` empties the registers.  A window of 1024 x 60 rows of 1024 bfloat16 channels: forward 47 us (252 MB at 5.3 TB/s), backward 92 us (378 MB at
-// 4.1 TB/s) and 12 us for the sums; a large copy runs at 4.9 TB/s.
+// `starts` empties the registers.  A window of 1024 x 60 rows of 1024 bfloat16 channels: forward 47 us (252 MB at 5.3 TB/s), backward 89 us (378 MB at
+// 4.3 TB/s) and 7 us for the sums; a large copy runs at 4.9 TB/s.
 #include "ppn_policy.h"
 
 #include <stdarg.h>

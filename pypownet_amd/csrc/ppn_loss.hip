@@ -11,13 +11,13 @@
 // The catalogue is taken in pieces, so that dl needs a bounded workspace whatever the catalogue's size: 256 MB and as much for its transpose, or
 // 1024 actions' worth where the rows make that more.
 //
-// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 470 us (860 TFLOP/s), the second 790 us (510; it
-// writes 1.6 GB, and the transposed copies), the third 935 us for both (870).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
-// alone, 466 and 325 us for the other two.  4096 rows: 112 us, and 83 of those are the product without its epilogue (10 vector instructions a logit),
+// 16384 rows, 24129 actions, 512 features in bfloat16 (405 GFLOP a product): the first kind takes 433 us (935 TFLOP/s), the second 737 us (550; it
+// writes 1.6 GB, and the transposed copies), the third 900 us for both (900).  A large library product reaches 1250 TFLOP/s; at these shapes it takes 572 us for the logits
+// alone, 466 and 325 us for the other two.  4096 rows: 108 us, and 83 of those are the product without its epilogue (10 vector instructions a logit),
 // which the other workgroups of a CU cover in part.
 //
-// Rounding dl to 16 bits (as the operand of a 16-bit product it has to be) is off by half a step of each entry, 2^-9 for bfloat16 and
-// 2^-12 for float16, independent from entry to entry; the gradients' own rounding is as large.  float16's range would lose small
+// Rounding dl to 16 bits (as the operand of a 16-bit product it has to be) is off by at most half a step of each entry, 2^-8 of it for bfloat16
+// and 2^-11 for float16, independent from entry to entry; the gradients' own rounding is as large.  float16's range would lose small
 // probabilities, so dl is scaled by a power of two that brings the largest |dloss| to 2^14, and the scale is taken out at the end.
 #include "ppn_policy.h"
 
@@ -705,7 +705,8 @@ BackwardPlan plan_backward(const ppn_loss_args* a) {
   // dl: 256 x 128 where two rounds of them fill the chip (16384 x 8192: 255 us, 269 in 128 x 128; 999 x 12099: 27 and 25)
   p.grad = ceil_div(a->rows, 256) * ceil_div(p.piece, 128) >= 1024 ? LARGE : config_for(a->rows, p.piece);
   // The second products: the largest tile with which shares of at least 512 of the inner dimensions make 384 workgroups of the two, then the
-  // shortest share with which they are at most 512.  At 256 x 128, 128 and 64, in us: 48, 55, 113 for 999 x 12099 x 392; -, 35, 12 for 256 x 347 x
+  // shortest share with which they are at most 512.  (Where dhidden's tiles alone come near 512 that is the longest inner dimension, and dweight's product
+  // stays in one share: right, but on few workgroups.  Training steps of 16384, 20480 and 61440 rows x 24129 x 512 take 2.06, 3.3 and 20 ms.)  At 256 x 128, 128 and 64, in us: 48, 55, 113 for 999 x 12099 x 392; -, 35, 12 for 256 x 347 x
   // 128 in 32 bits.
   for (int i = 0; i < 3; ++i) {
     p.sums = i == 0 ? LARGE : i == 1 ? MEDIUM : SMALL;

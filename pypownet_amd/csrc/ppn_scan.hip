@@ -9,9 +9,9 @@
 // exchanged between lanes in the forward pass, and B and C (the same for all lanes of a wave) are read once per wave and 8 rows, widened
 // to 32 bits in LDS and broadcast from there.  Workgroups are single waves: no barrier is waited for.
 //
-// A window of 1024 x 60 rows of 512 bfloat16 channels with 16 states, for training: forward 205 us (60 % of the vector units' time; 520 MB, half of them
-// checkpoints), backward 554 us (75 %), the sums 27 us.  Twice 8724 rows of 768 float16 channels, no gradients: 54 us for the chunks' ends, 17 us to
-// join them, 67 us for y.  Fetching a block ahead, into registers or straight into LDS, made none of these faster.
+// A window of 1024 x 60 rows of 512 bfloat16 channels with 16 states, for training, behind a hundred others (the card's clock rises over the first tens):
+// forward 178 us (vector units 68 % busy; 520 MB, half of them checkpoints), backward 485 us (87 %), the sums 27 us.  Twice 8724 rows of 768 float16
+// channels, no gradients: 49 us for the chunks' ends, 18 us to join them, 62 us for y.  Fetching a block ahead, into registers or straight into LDS, made none of these faster.
 #include "ppn_policy.h"
 
 namespace ppn_policy {
